@@ -206,8 +206,10 @@ void op_adamw(const at::Tensor& p, const at::Tensor& m, const at::Tensor& v, con
 }
 
 void register_gemm_ops(py::module& m);
+void register_decoder_ops(py::module& m);
 void register_ops(py::module& m) {
   register_gemm_ops(m);
+  register_decoder_ops(m);
   m.def("ln_fwd", &op_ln_fwd, py::arg("x"), py::arg("res"), py::arg("sum_out"), py::arg("w"), py::arg("b"),
         py::arg("y"), py::arg("mean"), py::arg("rstd"), py::arg("eps"), py::arg("rbias") = py::none());
   m.def("ln_bwd", &op_ln_bwd, py::arg("dy"), py::arg("x"), py::arg("mean"), py::arg("rstd"), py::arg("w"),

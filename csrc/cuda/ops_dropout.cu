@@ -1,0 +1,424 @@
+// Dropout from a counter-based generator (sm_100a), alone and inside the
+// residual add + LayerNorm of a decoder block. No mask is stored: the backward
+// pass draws the same numbers again.
+//
+// Draws: Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers:
+// as easy as 1, 2, 3", 2011). Block b of 8 consecutive elements takes the
+// counter (b low, b high, site, step) under the key (seed low, seed high); its
+// 128 bits are eight 16-bit draws, the low half of each word first. An element
+// is kept when its draw is >= threshold = p * 65536 rounded to a whole number,
+// and multiplied by 65536 / (65536 - threshold), the inverse of the exact
+// probability to be kept. 16 bits per draw instead of 32 halve the generator's
+// share: ten rounds are about 60 integer instructions per 8 elements, which
+// leaves the bf16 kernel bound by bandwidth (4 bytes per element).
+//
+// (seed, step) are read from device memory, so a captured graph draws anew when
+// the step advances between replays; the forward kernel notes the two values it
+// used, and the backward reads those.
+#include "common.cuh"
+#include "decoder_api.h"
+
+namespace nexar {
+
+namespace {
+constexpr int kDropThreads = 256;
+
+struct DropKey {
+  uint32_t k0, k1, step;
+};
+NEXAR_D DropKey drop_key(const int64_t* state) {
+  const unsigned long long seed = (unsigned long long)state[0];
+  return DropKey{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)(unsigned long long)state[1]};
+}
+
+// The 128 bits of one block.
+NEXAR_D uint4 philox(unsigned long long block, uint32_t site, const DropKey& key) {
+  uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = site, c3 = key.step;
+  uint32_t k0 = key.k0, k1 = key.k1;
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const unsigned long long p0 = (unsigned long long)c0 * 0xD2511F53u;
+    const unsigned long long p1 = (unsigned long long)c2 * 0xCD9E8D57u;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+    c1 = (uint32_t)p1;
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+    c3 = (uint32_t)p0;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+// Bit e: element e of the block is kept.
+NEXAR_D uint32_t keep_bits(unsigned long long block, uint32_t site, const DropKey& key, uint32_t threshold) {
+  const uint4 w = philox(block, site, key);
+  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    m |= ((v[e] & 0xffffu) >= threshold ? 1u : 0u) << (2 * e);
+    m |= ((v[e] >> 16) >= threshold ? 1u : 0u) << (2 * e + 1);
+  }
+  return m;
+}
+
+template <typename T> struct alignas(16) Eight {
+  T e[8];
+};
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kDropThreads) k_dropout(const T* __restrict__ x, T* __restrict__ y, long long n,
+                                                          const int64_t* __restrict__ state, uint32_t site,
+                                                          uint32_t threshold, float scale,
+                                                          int64_t* __restrict__ snapshot) {
+  const DropKey key = drop_key(state);
+  if (snapshot && blockIdx.x == 0 && threadIdx.x < 2) snapshot[threadIdx.x] = state[threadIdx.x];
+  const long long blocks = (n + 7) / 8;
+  for (long long i = blockIdx.x * (long long)kDropThreads + threadIdx.x; i < blocks;
+       i += (long long)gridDim.x * kDropThreads) {
+    if (VEC && i * 8 + 8 <= n) {
+      Eight<T> v = *reinterpret_cast<const Eight<T>*>(x + i * 8);
+      const uint32_t keep = keep_bits((unsigned long long)i, site, key, threshold);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)  // selected, not multiplied: an infinity that is dropped leaves no NaN
+        v.e[e] = from_acc<T, float>((keep >> e) & 1u ? to_acc<float>(v.e[e]) * scale : 0.f);
+      *reinterpret_cast<Eight<T>*>(y + i * 8) = v;
+    } else {
+      const uint32_t keep = keep_bits((unsigned long long)i, site, key, threshold);
+      for (int e = 0; e < 8 && i * 8 + e < n; ++e)
+        y[i * 8 + e] = from_acc<T, float>((keep >> e) & 1u ? to_acc<float>(x[i * 8 + e]) * scale : 0.f);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- residual add + dropout + LayerNorm
+constexpr int kRowWarps = 8;
+
+NEXAR_D float row_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+NEXAR_D void unpack8(const uint4& r, float* f) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 t = __bfloat1622float2(h[k]);
+    f[2 * k] = t.x;
+    f[2 * k + 1] = t.y;
+  }
+}
+NEXAR_D uint4 pack8(const float* f) {
+  uint4 r;
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&r);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) h[k] = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
+  return r;
+}
+NEXAR_D uint4 stream16(const __nv_bfloat16* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }
+
+// One warp per row, NP packs of 8 columns per lane. The sum is rounded to the
+// stored bf16 before the statistics, as in the operator without dropout.
+template <int NP>
+__global__ void __launch_bounds__(kRowWarps * 32) k_dropout_ln_fwd(
+    const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ r, const __nv_bfloat16* __restrict__ rb,
+    __nv_bfloat16* __restrict__ sum_out, const __nv_bfloat16* __restrict__ w, const __nv_bfloat16* __restrict__ b,
+    __nv_bfloat16* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, int R, int C, float eps,
+    const int64_t* __restrict__ state, uint32_t site, uint32_t threshold, float scale,
+    int64_t* __restrict__ snapshot) {
+  if (blockIdx.x == 0 && threadIdx.x < 2) snapshot[threadIdx.x] = state[threadIdx.x];
+  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  if (row >= R) return;
+  const DropKey key = drop_key(state);
+  const size_t base = (size_t)row * C;
+  uint4 vx[NP], vr[NP];
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const int col = (lane + 32 * k) * 8;
+    if (col < C) {
+      vx[k] = stream16(x + base + col);
+      vr[k] = stream16(r + base + col);
+    }
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const int col = (lane + 32 * k) * 8;
+    if (col < C) {
+      float a[8], d[8];
+      unpack8(vx[k], a);
+      unpack8(vr[k], d);
+      if (rb) {
+        float t[8];
+        unpack8(*reinterpret_cast<const uint4*>(rb + col), t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] += t[e];
+      }
+      const uint32_t keep = keep_bits((base + col) >> 3, site, key, threshold);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] += (keep >> e) & 1u ? d[e] * scale : 0.f;
+      vx[k] = pack8(a);
+      *reinterpret_cast<uint4*>(sum_out + base + col) = vx[k];
+      unpack8(vx[k], a);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += a[e];
+    }
+  }
+  const float mu = row_sum(s) / C;
+  float q = 0.f;
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    if ((lane + 32 * k) * 8 < C) {
+      float a[8];
+      unpack8(vx[k], a);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q += (a[e] - mu) * (a[e] - mu);
+    }
+  }
+  const float rs = rsqrtf(row_sum(q) / C + eps);
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const int col = (lane + 32 * k) * 8;
+    if (col < C) {
+      float a[8], wf[8], bf[8];
+      unpack8(vx[k], a);
+      unpack8(*reinterpret_cast<const uint4*>(w + col), wf);
+      unpack8(*reinterpret_cast<const uint4*>(b + col), bf);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] = (a[e] - mu) * rs * wf[e] + bf[e];
+      *reinterpret_cast<uint4*>(y + base + col) = pack8(a);
+    }
+  }
+  if (lane == 0) {
+    mean[row] = mu;
+    rstd[row] = rs;
+  }
+}
+
+// Backward. A block of C/8 threads (whole warps) walks over its rows four at a
+// time; a thread owns 8 columns, so the column sums (dw, db, drb) stay in 24
+// registers however wide the row is. Each group of four rows costs one barrier
+// for the two row sums. The blocks' column sums go to `part` and are added in a
+// fixed order by k_dropout_ln_columns: no atomics, the same bits every run.
+constexpr int kBwdRows = 4;
+template <bool BIAS>
+__global__ void __launch_bounds__(256) k_dropout_ln_bwd(
+    const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ s, const float* __restrict__ mean,
+    const float* __restrict__ rstd, const __nv_bfloat16* __restrict__ w, const __nv_bfloat16* __restrict__ dres,
+    __nv_bfloat16* __restrict__ dx, __nv_bfloat16* __restrict__ dr, float* __restrict__ part, int R, int C,
+    const int64_t* __restrict__ state, uint32_t site, uint32_t threshold, float scale) {
+  __shared__ float red[2][8][2 * kBwdRows];  // two buffers: one barrier per group of rows
+  const int col = threadIdx.x * 8;
+  const bool mine = col < C;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const DropKey key = drop_key(state);
+  float aw[8], ab[8], ad[8], wf[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) aw[e] = ab[e] = ad[e] = wf[e] = 0.f;
+  if (mine) unpack8(*reinterpret_cast<const uint4*>(w + col), wf);
+  const uint4 z = make_uint4(0, 0, 0, 0);
+  uint4 vg[kBwdRows], vs[kBwdRows], vr[kBwdRows];
+  const int stride = gridDim.x * kBwdRows;
+  int row0 = blockIdx.x * kBwdRows;
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int k = 0; k < kBwdRows; ++k) {
+      const bool ok = mine && r0 + k < R;
+      const size_t off = (size_t)(r0 + k) * C + col;
+      vg[k] = ok ? stream16(dy + off) : z;
+      vs[k] = ok ? stream16(s + off) : z;
+      vr[k] = ok && dres ? stream16(dres + off) : z;
+    }
+  };
+  load(row0);
+  int buf = 0;
+  for (; row0 < R; row0 += stride, buf ^= 1) {
+    float mu[kBwdRows], rs[kBwdRows], sums[2 * kBwdRows];
+#pragma unroll
+    for (int k = 0; k < kBwdRows; ++k) {
+      const bool ok = row0 + k < R;
+      mu[k] = ok ? mean[row0 + k] : 0.f;
+      rs[k] = ok ? rstd[row0 + k] : 0.f;
+      float g[8], xh[8], s1 = 0.f, s2 = 0.f;
+      unpack8(vg[k], g);
+      unpack8(vs[k], xh);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        xh[e] = (xh[e] - mu[k]) * rs[k];
+        aw[e] += g[e] * xh[e];
+        ab[e] += g[e];
+        const float gw = g[e] * wf[e];
+        s1 += gw;
+        s2 += gw * xh[e];
+      }
+      sums[2 * k] = row_sum(s1);
+      sums[2 * k + 1] = row_sum(s2);
+    }
+    if (lane == 0) {
+#pragma unroll
+      for (int k = 0; k < 2 * kBwdRows; ++k) red[buf][warp][k] = sums[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2 * kBwdRows; ++k) {
+      float t = 0.f;
+      for (int i = 0; i < warps; ++i) t += red[buf][i][k];
+      sums[k] = t / C;
+    }
+    uint4 ox[kBwdRows], od[kBwdRows];
+#pragma unroll
+    for (int k = 0; k < kBwdRows; ++k) {
+      float g[8], xh[8], o[8];
+      unpack8(vg[k], g);
+      unpack8(vs[k], xh);
+      unpack8(vr[k], o);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        xh[e] = (xh[e] - mu[k]) * rs[k];
+        o[e] += rs[k] * (g[e] * wf[e] - sums[2 * k] - xh[e] * sums[2 * k + 1]);
+      }
+      ox[k] = pack8(o);
+      const uint32_t keep = keep_bits(((size_t)(row0 + k) * C + col) >> 3, site, key, threshold);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = (keep >> e) & 1u ? o[e] * scale : 0.f;
+      od[k] = pack8(o);
+      if constexpr (BIAS) {
+        const bool ok = row0 + k < R;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ad[e] += ok ? o[e] : 0.f;  // before the rounding of dr
+      }
+    }
+    const int done = row0;
+    load(row0 + stride);
+    if (mine) {
+#pragma unroll
+      for (int k = 0; k < kBwdRows; ++k) {
+        if (done + k < R) {
+          const size_t off = (size_t)(done + k) * C + col;
+          *reinterpret_cast<uint4*>(dx + off) = ox[k];
+          *reinterpret_cast<uint4*>(dr + off) = od[k];
+        }
+      }
+    }
+  }
+  if (mine) {
+    float4* p = reinterpret_cast<float4*>(part + (size_t)blockIdx.x * (BIAS ? 3 : 2) * C + col);
+    const int c4 = C / 4;
+    p[0] = make_float4(aw[0], aw[1], aw[2], aw[3]);
+    p[1] = make_float4(aw[4], aw[5], aw[6], aw[7]);
+    p[c4] = make_float4(ab[0], ab[1], ab[2], ab[3]);
+    p[c4 + 1] = make_float4(ab[4], ab[5], ab[6], ab[7]);
+    if constexpr (BIAS) {
+      p[2 * c4] = make_float4(ad[0], ad[1], ad[2], ad[3]);
+      p[2 * c4 + 1] = make_float4(ad[4], ad[5], ad[6], ad[7]);
+    }
+  }
+}
+
+// Column sums of the P partial rows of W = (2 or 3) C values, in a fixed order:
+// 16 lanes of 4 columns by 16 slices of the partial rows per block.
+__global__ void __launch_bounds__(256) k_dropout_ln_columns(const float* __restrict__ part, int P, int W, int C,
+                                                            __nv_bfloat16* dw, __nv_bfloat16* db,
+                                                            __nv_bfloat16* drb) {
+  __shared__ float4 red[16][16];
+  const int cg = threadIdx.x & 15, sl = threadIdx.x >> 4;
+  const int col = (blockIdx.x * 16 + cg) * 4;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (col < W) {
+#pragma unroll 4
+    for (int p = sl; p < P; p += 16) {
+      const float4 v = *reinterpret_cast<const float4*>(part + (size_t)p * W + col);
+      a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+    }
+  }
+  red[sl][cg] = a;
+  __syncthreads();
+  if (sl == 0 && col < W) {
+    for (int j = 1; j < 16; ++j) {
+      const float4 v = red[j][cg];
+      a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+    }
+    const int which = col / C, c = col % C;  // C % 4 == 0: four columns are of one output
+    __nv_bfloat16* o = which == 0 ? dw : (which == 1 ? db : drb);
+    o[c] = __float2bfloat16_rn(a.x);
+    o[c + 1] = __float2bfloat16_rn(a.y);
+    o[c + 2] = __float2bfloat16_rn(a.z);
+    o[c + 3] = __float2bfloat16_rn(a.w);
+  }
+}
+
+// Blocks of the backward: enough rows per block that its partial sums (12 C
+// bytes) stay small beside the rows (10 C bytes each), at most the number that
+// fits the GPU at once.
+int bwd_blocks(int R, int C) {
+  const int threads = (C / 8 + 31) / 32 * 32;
+  const int per_sm = threads <= 96 ? 4 : (threads <= 128 ? 3 : 2);
+  const int groups = (R + kBwdRows - 1) / kBwdRows;
+  return groups < 148 * per_sm ? (groups < 1 ? 1 : groups) : 148 * per_sm;
+}
+
+template <typename T>
+cudaError_t dropout_typed(const void* x, void* y, long long n, const int64_t* state, uint32_t site, uint32_t thr,
+                          float scale, int64_t* snapshot, cudaStream_t s) {
+  const long long blocks = ((n + 7) / 8 + kDropThreads - 1) / kDropThreads;
+  const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
+  const T* xi = reinterpret_cast<const T*>(x);
+  T* yo = reinterpret_cast<T*>(y);
+  if ((uintptr_t)x % 16 == 0 && (uintptr_t)y % 16 == 0)
+    k_dropout<T, true><<<grid, kDropThreads, 0, s>>>(xi, yo, n, state, site, thr, scale, snapshot);
+  else
+    k_dropout<T, false><<<grid, kDropThreads, 0, s>>>(xi, yo, n, state, site, thr, scale, snapshot);
+  return cudaGetLastError();
+}
+}  // namespace
+
+cudaError_t dropout(const void* x, void* y, long long n, int dtype, const int64_t* state, uint32_t site,
+                    uint32_t threshold, float scale, int64_t* snapshot, cudaStream_t s) {
+  if (n <= 0) return cudaErrorInvalidValue;
+  if (dtype == 0) return dropout_typed<__nv_bfloat16>(x, y, n, state, site, threshold, scale, snapshot, s);
+  if (dtype == 1) return dropout_typed<__half>(x, y, n, state, site, threshold, scale, snapshot, s);
+  return dropout_typed<float>(x, y, n, state, site, threshold, scale, snapshot, s);
+}
+
+cudaError_t dropout_ln_fwd(const __nv_bfloat16* x, const __nv_bfloat16* r, const __nv_bfloat16* rb,
+                           __nv_bfloat16* sum_out, const __nv_bfloat16* w, const __nv_bfloat16* b, __nv_bfloat16* y,
+                           float* mean, float* rstd, int R, int C, float eps, const int64_t* state, uint32_t site,
+                           uint32_t threshold, float scale, int64_t* snapshot, cudaStream_t s) {
+  if (C % 8 || C > 2048 || R < 1) return cudaErrorInvalidValue;
+  const int grid = (R + kRowWarps - 1) / kRowWarps;
+#define NEXAR_DROP_FWD(NP)                                                                                     \
+  k_dropout_ln_fwd<NP><<<grid, kRowWarps * 32, 0, s>>>(x, r, rb, sum_out, w, b, y, mean, rstd, R, C, eps, state, \
+                                                       site, threshold, scale, snapshot)
+  if (C <= 256) NEXAR_DROP_FWD(1);
+  else if (C <= 512) NEXAR_DROP_FWD(2);
+  else if (C <= 768) NEXAR_DROP_FWD(3);
+  else if (C <= 1024) NEXAR_DROP_FWD(4);
+  else if (C <= 1536) NEXAR_DROP_FWD(6);
+  else NEXAR_DROP_FWD(8);
+#undef NEXAR_DROP_FWD
+  return cudaGetLastError();
+}
+
+size_t dropout_ln_bwd_scratch_floats(int R, int C) { return (size_t)bwd_blocks(R, C) * 3 * C; }
+
+cudaError_t dropout_ln_bwd(const __nv_bfloat16* dy, const __nv_bfloat16* s_in, const float* mean, const float* rstd,
+                           const __nv_bfloat16* w, const __nv_bfloat16* dres, __nv_bfloat16* dx, __nv_bfloat16* dr,
+                           __nv_bfloat16* dw, __nv_bfloat16* db, __nv_bfloat16* drb, float* scratch, int R, int C,
+                           const int64_t* state, uint32_t site, uint32_t threshold, float scale, cudaStream_t s) {
+  if (C % 8 || C > 2048 || R < 1) return cudaErrorInvalidValue;
+  const int grid = bwd_blocks(R, C), threads = (C / 8 + 31) / 32 * 32;
+  if (drb)
+    k_dropout_ln_bwd<true><<<grid, threads, 0, s>>>(dy, s_in, mean, rstd, w, dres, dx, dr, scratch, R, C, state, site,
+                                                    threshold, scale);
+  else
+    k_dropout_ln_bwd<false><<<grid, threads, 0, s>>>(dy, s_in, mean, rstd, w, dres, dx, dr, scratch, R, C, state,
+                                                     site, threshold, scale);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const int W = (drb ? 3 : 2) * C;
+  k_dropout_ln_columns<<<(W + 63) / 64, 256, 0, s>>>(scratch, grid, W, C, dw, db, drb);
+  return cudaGetLastError();
+}
+
+}  // namespace nexar

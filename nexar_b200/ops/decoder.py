@@ -1,0 +1,294 @@
+"""Operators of a decoder block besides softmax attention: rotary positions,
+counter-based dropout and attention with a decay per head.
+
+Every function calls the sm_100a kernels on the current stream of its input's
+GPU and allocates its outputs and workspaces there, so calls can be captured
+into CUDA graphs and run on any stream or device.
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from typing import List, Optional, Tuple
+
+import torch
+
+from .. import _native
+
+
+# ---------------------------------------------------------------- rotary positions
+@dataclass(frozen=True)
+class RotaryScaling:
+    """How frequencies are stretched for contexts ``factor`` times longer than
+    the ``original_length`` a model was trained on.
+
+    ``linear``  every frequency divided by ``factor``;
+    ``ntk``     the base raised to base * factor^(dim / (dim - 2)), so the
+                fastest pair keeps its frequency and the slowest is divided by ``factor``;
+    ``bands``   pairs that turn more than ``high`` times in the original length
+                keep their frequency, those below ``low`` turns are divided by
+                ``factor``, linear in the turns between;
+    ``yarn``    the same idea with a ramp over the pair's index between
+                ``fast`` and ``slow`` turns, and cosine and sine times
+                ``magnitude`` (default 0.1 ln(factor) + 1).
+    """
+    kind: str
+    factor: float
+    original_length: int = 2048
+    low: float = 1.0
+    high: float = 4.0
+    fast: float = 32.0
+    slow: float = 1.0
+    magnitude: Optional[float] = None
+
+    def __post_init__(self):
+        if self.kind not in ("linear", "ntk", "bands", "yarn"):
+            raise ValueError(f"unknown rotary scaling {self.kind!r} (linear, ntk, bands, yarn)")
+        if not (self.factor >= 1.0 and math.isfinite(self.factor)) or self.original_length < 1:
+            raise ValueError("rotary scaling needs a finite factor >= 1 and an original length >= 1")
+        if not (0 < self.low < self.high) or not (0 < self.slow < self.fast):
+            raise ValueError("rotary scaling needs 0 < low < high and 0 < slow < fast")
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0,
+                       scaling: Optional[RotaryScaling] = None) -> Tuple[List[float], float]:
+    """(radians per token of each of the dim / 2 pairs, factor on cosine and sine)."""
+    if dim < 2 or dim % 2:
+        raise ValueError(f"rotary positions turn an even number of elements, got {dim}")
+    if not (base > 1.0 and math.isfinite(base)):
+        raise ValueError(f"rotary base must be a finite number above 1, got {base}")
+    n, magnitude = dim // 2, 1.0
+    if scaling is not None and scaling.kind == "ntk" and dim > 2:
+        base = base * scaling.factor ** (dim / (dim - 2))
+    freq = [base ** (-2.0 * i / dim) for i in range(n)]
+    if scaling is None or scaling.kind == "ntk":
+        return freq, magnitude
+    f, length = scaling.factor, scaling.original_length
+    if scaling.kind == "linear":
+        return [w / f for w in freq], magnitude
+    if scaling.kind == "bands":
+        keep = [min(max((length * w / (2 * math.pi) - scaling.low) / (scaling.high - scaling.low), 0.0), 1.0)
+                for w in freq]
+    else:
+        def pair_of(turns):  # the (fractional) pair that turns this often in the original length
+            return dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
+        first = max(math.floor(pair_of(scaling.fast)), 0)
+        last = min(math.ceil(pair_of(scaling.slow)), n - 1)
+        keep = [1.0 - min(max((i - first) / max(last - first, 1e-3), 0.0), 1.0) for i in range(n)]
+        magnitude = 0.1 * math.log(f) + 1.0 if scaling.magnitude is None else scaling.magnitude
+    return [w / f * (1.0 - k) + w * k for w, k in zip(freq, keep)], magnitude
+
+
+def rotary_table(length: int, dim: int, base: float = 10000.0, scaling: Optional[RotaryScaling] = None,
+                 device=None) -> torch.Tensor:
+    """fp32 [length, dim] table of (cos, sin) of every pair at positions 0 .. length - 1, angles
+    computed in 64 bits. Built once and passed to :func:`rotary` / :func:`rotary_qk`; ``dim`` is how
+    many elements of a head turn (the head size, or less for a partial rotation)."""
+    if length < 1:
+        raise ValueError(f"a rotary table needs at least one position, got {length}")
+    freq, magnitude = rotary_frequencies(dim, base, scaling)
+    device = torch.device("cuda") if device is None else torch.device(device)
+    if device.type != "cuda":
+        raise ValueError(f"rotary tables live on a GPU, got {device}")
+    table = torch.empty(length, dim, dtype=torch.float32, device=device)
+    _native.cuda().rotary_table(torch.tensor(freq, dtype=torch.float64, device=table.device), table, magnitude)
+    return table
+
+
+def _interleaved(layout: str) -> bool:
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"unknown rotary layout {layout!r} (half, interleaved)")
+    return layout == "interleaved"
+
+
+def _rotate(xs, table, positions, start, heads, interleaved, inverse):
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        if table.requires_grad:
+            raise ValueError("the rotary table takes no gradient")
+        return _Rotary.apply(table, positions, start, heads, interleaved, inverse, *xs)
+    return tuple(_native.cuda().rotary(xs[0], xs[1] if len(xs) > 1 else None, table, positions, start, heads,
+                                       interleaved, inverse))
+
+
+class _Rotary(torch.autograd.Function):
+    """The turn is orthogonal up to the table's magnitude m: its adjoint is the
+    turn by the opposite angles (with the same m)."""
+
+    @staticmethod
+    def forward(ctx, table, positions, start, heads, interleaved, inverse, *xs):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(table, positions)
+        ctx.how = (start, heads, interleaved, inverse)
+        return tuple(_native.cuda().rotary(xs[0], xs[1] if len(xs) > 1 else None, table, positions, start, heads,
+                                           interleaved, inverse))
+
+    @staticmethod
+    def backward(ctx, *dys):
+        table, positions = ctx.saved_tensors
+        start, heads, interleaved, inverse = ctx.how
+        given = [d for d in dys if d is not None]
+        got = iter(_rotate(given, table, positions, start, heads, interleaved, not inverse) if given else ())
+        return (None,) * 6 + tuple(None if d is None else next(got) for d in dys)
+
+
+def rotary(x, table, positions=None, start: int = 0, heads: Optional[int] = None, layout: str = "half"):
+    """Rotary positions of x [T, H, D] or [B, T, H, D] (bf16, fp16 or fp32, any strides): the first
+    ``table.shape[1]`` elements of a head turn by their position's angles, the rest is copied.
+
+    ``positions`` ([T] or [B, T], int64 or int32) gives each token's row of the table; without it
+    token t is at ``start + t``. A position outside the table gives NaN in the elements that turn.
+    ``heads``: only the first that many heads turn, the others are copied (a packed QKV projection
+    viewed as [B, T, H + 2 Hk, D] turns H + Hk of them). ``layout``: pairs (i, i + dim/2) ("half") or
+    (2i, 2i + 1) ("interleaved"). Returns a contiguous tensor; differentiable in x."""
+    if heads is not None and heads < 0:
+        raise ValueError(f"heads must not be negative, got {heads}")
+    return _rotate((x,), table, positions, start, -1 if heads is None else heads, _interleaved(layout), False)[0]
+
+
+def rotary_qk(q, k, table, positions=None, start: int = 0, layout: str = "half"):
+    """:func:`rotary` of queries [B, T, H, D] and keys [B, T, Hk, D] in one launch: returns both."""
+    return _rotate((q, k), table, positions, start, -1, _interleaved(layout), False)
+
+
+# ---------------------------------------------------------------- dropout
+class DropoutState:
+    """(seed, step) of the counter-based generator, two int64 values on the GPU.
+
+    Every call takes its numbers from (seed, step, site, element): ``site`` tells the calls of one
+    step apart, :meth:`advance` moves to the next step. The kernels read the values on the device, so a
+    captured graph that contains :meth:`advance` draws anew at every replay. Data-parallel ranks use
+    different seeds; calls with the same seed, step and site draw the same mask."""
+
+    def __init__(self, seed: int, device=None, step: int = 0):
+        device = torch.device("cuda") if device is None else torch.device(device)
+        self.tensor = torch.empty(2, dtype=torch.int64, device=device)
+        self.set(seed, step)
+
+    def set(self, seed: int, step: int = 0) -> None:
+        wrap = lambda v: (int(v) + (1 << 63)) % (1 << 64) - (1 << 63)  # noqa: E731
+        self.tensor.copy_(torch.tensor([wrap(seed), wrap(step)], dtype=torch.int64))
+
+    def advance(self) -> None:
+        self.tensor[1:].add_(1)
+
+
+def _check_dropout(p: float, state) -> None:
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability must be in [0, 1], got {p}")
+    if not isinstance(state, DropoutState):
+        raise TypeError("dropout needs a DropoutState")
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, state, site, p):
+        y, used = _native.cuda().dropout(x, state, site, p, True)
+        ctx.save_for_backward(used)
+        ctx.how = (site, p)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        (used,) = ctx.saved_tensors
+        return _drop(dy, used, *ctx.how), None, None, None
+
+
+def _drop(x, state, site, p):
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _Dropout.apply(x, state, site, p)
+    return _native.cuda().dropout(x, state, site, p, False)[0]
+
+
+def dropout(x, p: float, state: DropoutState, site: int = 0):
+    """Zero each element of x (bf16, fp16 or fp32) with probability ``p`` (rounded to a multiple of
+    2^-16) and scale the others by the inverse of the probability to be kept. No mask is stored: the
+    backward draws it again from the (seed, step) that the forward used. Returns a contiguous tensor."""
+    _check_dropout(p, state)
+    return _drop(x, state.tensor, site, p)
+
+
+# ---------------------------------------------------------------- attention with a decay per head
+def _decay_scale(scale, D):
+    return D ** -0.5 if scale is None else float(scale)
+
+
+def _no_decay_grad(log_decay):
+    if log_decay.requires_grad:
+        raise ValueError("decay attention: the decays are fixed; log_decay takes no gradient (detach it)")
+
+
+class _DecayAttention(torch.autograd.Function):
+    """q, k, v [B, T, H, D], or (packed) one qkv [B, T, 3, H, D] with k = v = None."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state, lengths, scale, return_state):
+        ctx.set_materialize_grads(False)
+        ctx.packed = k is None
+        a = q.unbind(2) if ctx.packed else (q, k, v)
+        o, final = _native.cuda().decay_fwd(*a, log_decay, state, lengths, scale, return_state)
+        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
+        ctx.scale = scale
+        return o, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, dstate):
+        q, k, v, log_decay, state, lengths = ctx.saved_tensors
+        a = q.unbind(2) if ctx.packed else (q, k, v)
+        if ctx.packed:
+            grads = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            d = grads.unbind(2)
+        else:
+            d = grads = tuple(torch.empty(q.shape, dtype=q.dtype, device=q.device) for _ in range(3))
+        if do is None:
+            do = torch.zeros(a[0].shape, dtype=q.dtype, device=q.device)
+        if dstate is not None:
+            dstate = dstate.contiguous()
+        ds0 = _native.cuda().decay_bwd(*a, do, log_decay, state, dstate, lengths, ctx.scale, *d,
+                                       ctx.needs_input_grad[4])
+        if ctx.packed:
+            return grads, None, None, None, ds0, None, None, None
+        return (*grads, None, ds0, None, None, None)
+
+
+def _decay(q, k, v, log_decay, state, lengths, scale, return_state):
+    _no_decay_grad(log_decay)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
+        out = _DecayAttention.apply(q, k, v, log_decay, state, lengths, scale, return_state)
+    else:
+        out = _native.cuda().decay_fwd(*(q.unbind(2) if k is None else (q, k, v)), log_decay, state, lengths, scale,
+                                       return_state)
+    return tuple(out) if return_state else out[0]
+
+
+def decay_attention(q, k, v, log_decay, state=None, lengths=None, scale: Optional[float] = None,
+                    return_state: bool = False):
+    """Causal linear attention with a decay for each head (tensor-core kernels, chunked over tokens):
+
+        S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,    o_t = scale S_t^T q_t.
+
+    q, k, v: bf16 [B, T, H, D] of the same shape, D 64 or 128, any strides. ``log_decay``: fp32 [H],
+    each finite and at most 0 (0: no decay); not trained. ``state``: fp32 [B, H, D, D] before the
+    first token (default zero). ``lengths``: int32 [B]; tokens from there on do not exist (not read, zero
+    output and gradients, the final state is the one behind the last token). ``scale`` defaults to D^-0.5.
+    Returns o [B, T, H, D] bf16, or (o, final state) with ``return_state``; differentiable in q, k, v
+    and state (lengths are kept by reference until the backward pass)."""
+    return _decay(q, k, v, log_decay, state, lengths, _decay_scale(scale, q.shape[-1]), return_state)
+
+
+def decay_attention_qkv(qkv, log_decay, state=None, lengths=None, scale: Optional[float] = None,
+                        return_state: bool = False):
+    """:func:`decay_attention` on a packed projection qkv [B, T, 3, H, D]; the gradient comes back
+    packed, in one buffer."""
+    if qkv.dim() != 5 or qkv.shape[2] != 3:
+        raise ValueError(f"decay_attention_qkv takes qkv [B, T, 3, H, D], got {tuple(qkv.shape)}")
+    return _decay(qkv, None, None, log_decay, state, lengths, _decay_scale(scale, qkv.shape[-1]), return_state)
+
+
+def decay_attention_step(q, k, v, log_decay, state, scale: Optional[float] = None):
+    """One token of :func:`decay_attention` for inference: q, k, v bf16 [B, H, D]; updates ``state``
+    (fp32 [B, H, D, D]) in place and returns o [B, H, D]."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+        raise ValueError("decay_attention_step has no gradient; call it under torch.no_grad() or train with "
+                         "decay_attention")
+    return _native.cuda().decay_step(q, k, v, log_decay, state, _decay_scale(scale, q.shape[-1]))

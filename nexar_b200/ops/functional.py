@@ -265,7 +265,56 @@ class _ResidualLayerNorm(torch.autograd.Function):
         return dx, dx, outs[0][1], outs[1][1], (outs[2][1] if ctx.rb is not None else None), None
 
 
-def residual_layer_norm(x, r, w, b, eps: float = 1e-5, rbias=None):
+class _ResidualDropoutLayerNorm(torch.autograd.Function):
+    """s = x + dropout(r (+ rb)) ; y = LayerNorm(s), the mask drawn inside the kernels.
+
+    The backward draws the same mask again from the (seed, step) that the
+    forward noted, and returns the gradients of both summands, the LayerNorm's
+    parameters and rb from one pass over the rows."""
+
+    @staticmethod
+    def forward(ctx, x, r, w, b, rb, eps, state, site, p):
+        ctx.set_materialize_grads(False)
+        x2, r2 = x.contiguous(), r.contiguous()
+        s, y, mean, rstd, used = _native.cuda().dropout_ln_fwd(x2, r2, rb, w, b, eps, state, site, p)
+        ctx.save_for_backward(s, w, mean, rstd, used)
+        ctx.b, ctx.rb = b, rb
+        ctx.how = (site, p)
+        ctx.shapes = (x.shape, r.shape)
+        return s, y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, ds, dy):
+        s, w, mean, rstd, used = ctx.saved_tensors
+        outs = []
+        for p in (w, ctx.b, ctx.rb):
+            g = _sink(p) if p is not None else None
+            outs.append((g, None) if g is not None or p is None else (None, torch.empty_like(p)))
+        dw, db, drb = (g if g is not None else t for g, t in outs)
+        dy = torch.zeros_like(s) if dy is None else dy.contiguous()
+        ds = None if ds is None else ds.contiguous()
+        dx, dr = _native.cuda().dropout_ln_bwd(dy, s, mean, rstd, w, ds, dw, db, drb, used, *ctx.how)
+        for p, (sink, _) in zip((w, ctx.b, ctx.rb), outs):
+            if sink is not None:
+                _ready(p)
+        return (dx.view(ctx.shapes[0]), dr.view(ctx.shapes[1]), outs[0][1], outs[1][1], outs[2][1], None, None, None,
+                None)
+
+
+def residual_layer_norm(x, r, w, b, eps: float = 1e-5, rbias=None, p: float = 0.0, dropout=None, site: int = 0):
+    """s = x + dropout(r + rbias), y = LayerNorm(s) w + b: returns (s, y).
+
+    ``dropout``: a :class:`~nexar_b200.ops.DropoutState`; with it and p > 0 each element of the residual
+    branch is zeroed with probability ``p`` and the others scaled, without a stored mask, by the
+    draws that :func:`~nexar_b200.ops.dropout` makes for the same (seed, step, ``site``)."""
+    if p or dropout is not None:
+        from .decoder import _check_dropout
+        _check_dropout(p, dropout)
+        if p:
+            if r.numel() != x.numel():
+                raise ValueError(f"residual_layer_norm: x has {x.numel()} elements, r {r.numel()}")
+            return _ResidualDropoutLayerNorm.apply(x, r, w, b, rbias, eps, dropout.tensor, site, p)
     return _ResidualLayerNorm.apply(x, r, w, b, rbias, eps)
 
 

@@ -1,0 +1,288 @@
+"""Attention with a decay per head against the written-out sums in 64 bits."""
+import pytest
+import torch
+
+import decoder_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+
+DECAYS = {"mixed": [0.0, -0.002, -0.03, -0.7], "steep": [-5.0, -30.0, -90.0, -1e4], "none": [0.0] * 4}
+
+
+def _inputs(dev, B, T, H, D, seed, decays="mixed"):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    q, k, v, do = (torch.randn(B, T, H, D, device=dev, generator=g).to(torch.bfloat16) for _ in range(4))
+    s0, ds = (torch.randn(B, H, D, D, device=dev, generator=g) for _ in range(2))
+    lam = torch.tensor((DECAYS[decays] * H)[:H], device=dev)
+    return q, k, v, do, s0, ds, lam
+
+
+def _check(got, want, size, T, D, what, state=False):
+    """size: the result's sum with every factor in absolute value. A bf16 output is rounded once (half a step). The
+    scores and the states that enter it are split into two bf16 parts: each factor keeps 16 bits (2^-16; twice,
+    and once more for products of two errors). All sums are fp32 over at most T + D + 64 terms (2^-24 each), and the
+    powers of the decay are fp32 values (2^-23 for their products). The state's keys are split into three parts (2^-23).
+    """
+    f32 = 2.0 ** -24
+    extra = ((T + D + 64) * f32 + 2.0 ** -21 + (0 if state else 3 * 2.0 ** -16)) * size
+    half = oracle.half_step(got.dtype)
+    oracle.assert_within(got, want, half * (want.abs() + extra) + extra + 1e-30, what)
+
+
+def _sizes(q, k, v, lam, s0, n, scale):
+    return oracle.decay_attention(q.abs(), k.abs(), v.abs(), lam, None if s0 is None else s0.abs(), n, scale)
+
+
+def _compare(dev, B, T, H, D, lengths=None, state=True, decays="mixed", views=None, train=True, scale=None, seed=0):
+    from nexar_b200 import ops
+    q, k, v, do, s0, ds, lam = _inputs(dev, B, T, H, D, seed + T + D, decays)
+    if views:
+        q, k, v = views(q, k, v)
+    if not state:
+        s0 = None
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=dev)
+    leaves = [t.requires_grad_(train) for t in (q, k, v) + ((s0,) if state else ())]
+    o, final = ops.decay_attention(q, k, v, lam, state=s0, lengths=n, scale=scale, return_state=True)
+    x = [t.detach().double().requires_grad_(True) for t in leaves]
+    s64 = x[3] if state else None
+    ow, fw = oracle.decay_attention(*x[:3], lam, s64, n, scale)
+    with torch.no_grad():
+        osz, fsz = _sizes(*x[:3], lam, s64, n, scale)
+    _check(o.detach(), ow.detach(), osz, T, D, "o")
+    _check(final.detach(), fw.detach(), fsz, T, D, "final state", True)
+    if not train:
+        return
+    got = torch.autograd.grad((o, final), leaves, (do, ds))
+    want = torch.autograd.grad((ow, fw), x, (do.double(), ds.double()))
+    a = [t.detach().abs().requires_grad_(True) for t in x]
+    osz, fsz = oracle.decay_attention(*a[:3], lam, a[3] if state else None, n, scale)
+    size = torch.autograd.grad((osz, fsz), a, (do.double().abs(), ds.double().abs()))
+    for i, name in enumerate(["dq", "dk", "dv"] + (["dstate"] if state else [])):
+        _check(got[i], want[i], size[i], T, D, name, name == "dstate")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 63, 64, 65, 127, 130])
+def test_short_sequences(cuda0, T, D):
+    _compare(cuda0, 2, T, 3, D)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,T,H", [(1, 1000, 1), (1, 257, 4), (3, 700, 2), (1, 2049, 2)])
+@pytest.mark.parametrize("state", [True, False])
+def test_split_over_the_tokens(cuda0, B, T, H, D, state):
+    """Few sequences and heads: several segments, the last one ragged."""
+    from nexar_b200 import _native  # noqa: F401
+    _compare(cuda0, B, T, H, D, state=state)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_heads_without_a_split(cuda0, D):
+    _compare(cuda0, 16, 190, 12, D)
+
+
+@pytest.mark.parametrize("decays", ["steep", "none"])
+@pytest.mark.parametrize("T", [70, 600])
+def test_steep_and_absent_decays(cuda0, decays, T):
+    _compare(cuda0, 1, T, 4, 64, decays=decays)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,lengths", [(100, [0, 1, 64, 99, 100, 37]), (900, [900, 0, 1, 128, 513, 899]), (5, [0, 0])])
+def test_lengths(cuda0, T, lengths, D):
+    _compare(cuda0, len(lengths), T, 2, D, lengths=lengths)
+
+
+def test_lengths_outside_the_range_are_clipped(cuda0):
+    from nexar_b200 import ops
+    q, k, v, _, s0, _, lam = _inputs(cuda0, 2, 80, 2, 64, 3)
+    far = ops.decay_attention(q, k, v, lam, s0, torch.tensor([99, -7], dtype=torch.int32, device=cuda0), return_state=True)
+    near = ops.decay_attention(q, k, v, lam, s0, torch.tensor([80, 0], dtype=torch.int32, device=cuda0), return_state=True)
+    assert all(torch.equal(a, b) for a, b in zip(far, near)) and torch.equal(near[1][1], s0[1])
+
+
+@pytest.mark.parametrize("T", [100, 1500])
+def test_rows_behind_a_sequence_are_not_read(cuda0, T):
+    """Infinities and NaN there change nothing and get zero gradients."""
+    from nexar_b200 import ops
+    q, k, v, do, s0, ds, lam = _inputs(cuda0, 2, T, 2, 64, 4)
+    n = torch.tensor([T - 41, 3], dtype=torch.int32, device=cuda0)
+    outs = []
+    for junk in (0.0, float("nan"), float("inf")):
+        x = [t.clone() for t in (q, k, v, do)]
+        for t in x:
+            t[0, T - 41:] = junk
+            t[1, 3:] = junk
+        leaves = [t.requires_grad_(True) for t in x[:3] + [s0.clone()]]
+        o, f = ops.decay_attention(*leaves[:3], lam, leaves[3], n, return_state=True)
+        outs.append([o, f, *torch.autograd.grad((o, f), leaves, (x[3], ds))])
+    for a, b, c in zip(*outs):
+        assert torch.equal(a, b) and torch.equal(a, c) and torch.isfinite(a).all()
+    assert not outs[0][0][1, 3:].any() and not outs[0][2][0, T - 41:].any()
+
+
+def test_strides_and_shared_heads(cuda0):
+    """Views of a packed projection, transposed, unaligned, and keys shared by all heads."""
+    def packed(q, k, v):
+        return torch.stack([q, k, v], 2).unbind(2)
+
+    def transposed(q, k, v):
+        return tuple(t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v))
+
+    def odd(q, k, v):
+        wide = torch.nn.functional.pad(torch.cat([q, k, v], -1), (1, 2))
+        return tuple(t.detach() for t in wide[..., 1:-2].split(q.shape[-1], -1))
+    for f in (packed, transposed, odd):
+        _compare(cuda0, 2, 77, 3, 64, views=f)
+    from nexar_b200 import ops
+    q, k, v, do, _, _, lam = _inputs(cuda0, 2, 50, 4, 64, 7)
+    shared = k[:, :, :1].clone().requires_grad_(True)
+    (got,) = torch.autograd.grad(ops.decay_attention(q, shared.expand(-1, -1, 4, -1), v, lam), shared, do)
+    full = shared.detach().expand(-1, -1, 4, -1).contiguous().requires_grad_(True)
+    (each,) = torch.autograd.grad(ops.decay_attention(q, full, v, lam), full, do)
+    assert torch.equal(got, each.sum(2, keepdim=True))
+
+
+def test_packed_form_is_the_same(cuda0):
+    from nexar_b200 import ops
+    q, k, v, do, s0, ds, lam = _inputs(cuda0, 2, 200, 3, 64, 8)
+    qkv = torch.stack([q, k, v], 2).requires_grad_(True)
+    x = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    o, f = ops.decay_attention_qkv(qkv, lam, state=s0, return_state=True)
+    o2, f2 = ops.decay_attention(*x, lam, state=s0, return_state=True)
+    assert torch.equal(o, o2) and torch.equal(f, f2)
+    (g,) = torch.autograd.grad((o, f), qkv, (do, ds))
+    assert torch.equal(g, torch.stack(torch.autograd.grad((o2, f2), x, (do, ds)), 2))
+    with torch.no_grad():
+        assert torch.equal(ops.decay_attention_qkv(qkv, lam, state=s0), o)
+
+
+def test_gradient_against_differences(cuda0):
+    from nexar_b200 import ops
+    q, k, v, do, s0, ds, lam = _inputs(cuda0, 1, 140, 2, 64, 9)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, s0)]
+    grads = torch.autograd.grad(ops.decay_attention(q, k, v, lam, s0, return_state=True), leaves, (do, ds))
+
+    def loss(q, k, v, s):
+        o, f = oracle.decay_attention(q, k, v, lam, s)
+        return (o * do.double()).sum() + (f * ds.double()).sum()
+    at = [t.detach().double() for t in leaves]
+    for i, got in enumerate(grads):
+        way = [torch.randn_like(t) if j == i else torch.zeros_like(t) for j, t in enumerate(at)]
+        want = oracle.directional(loss, at, way)  # linear in each input: no truncation error
+        size = (got.double().abs() * way[i].abs()).sum()
+        assert abs((got.double() * way[i]).sum() - want) <= 2 * 2.0 ** -8 * size, i
+
+
+@pytest.mark.parametrize("which", [(0,), (1,)])
+def test_partial_outputs(cuda0, which):
+    """Only the output or only the state has a gradient: the formula's with zeros for the other."""
+    from nexar_b200 import ops
+    q, k, v, do, s0, ds, lam = _inputs(cuda0, 2, 100, 2, 64, 10)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, s0)]
+    out = ops.decay_attention(q, k, v, lam, s0, return_state=True)
+    got = torch.autograd.grad([out[i] for i in which], leaves, [(do, ds)[i] for i in which])
+    do, ds = (t if i in which else torch.zeros_like(t) for i, t in enumerate((do, ds)))
+    x = [t.detach().double().requires_grad_(True) for t in leaves]
+    want = torch.autograd.grad(oracle.decay_attention(*x[:3], lam, x[3]), x, (do.double(), ds.double()))
+    a = [t.detach().abs().requires_grad_(True) for t in x]
+    size = torch.autograd.grad(oracle.decay_attention(*a[:3], lam, a[3]), a, (do.double().abs(), ds.double().abs()))
+    for i, name in enumerate(("dq", "dk", "dv", "dstate")):
+        _check(got[i], want[i], size[i], 100, 64, name, name == "dstate")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,H", [(1, 1), (3, 5), (40, 12)])
+def test_single_tokens(cuda0, B, H, D):
+    from nexar_b200 import ops
+    q, k, v, _, s0, _, lam = _inputs(cuda0, B, 1, H, D, 11)
+    q, k, v = (t[:, 0] for t in (q, k, v))
+    state = s0.clone()
+    o = ops.decay_attention_step(q, k, v, lam, state)
+    f32 = 2.0 ** -24
+    decay = lam.double().exp().view(1, H, 1, 1)
+    kv = k.double()[..., None] * v.double()[..., None, :]
+    want = decay * s0.double() + kv
+    size = decay * s0.double().abs() + kv.abs()
+    oracle.assert_within(state, want, 4 * f32 * size, "state")  # the decay, two products and their sum in fp32
+    ow = (q.double()[..., None, :] @ want)[..., 0, :] * D ** -0.5
+    extra = (D + 8) * f32 * (q.double().abs()[..., None, :] @ size)[..., 0, :] * D ** -0.5
+    half = oracle.half_step(torch.bfloat16)
+    oracle.assert_within(o, ow, half * (ow.abs() + extra) + extra, "o")
+
+
+def test_prompt_then_single_tokens(cuda0):
+    """A prompt in one call, then token by token, is the whole sequence in one call."""
+    from nexar_b200 import ops
+    B, T, H, D = 2, 300, 4, 64
+    q, k, v, _, _, _, lam = _inputs(cuda0, B, T, H, D, 12)
+    whole, last = ops.decay_attention(q, k, v, lam, return_state=True)
+    qkv = torch.stack([q, k, v], 2)
+    o, state = ops.decay_attention_qkv(qkv[:, :290], lam, return_state=True)
+    parts = [o]
+    for t in range(290, T):
+        parts.append(ops.decay_attention_step(*qkv[:, t].unbind(1), lam, state)[:, None])
+    want, fin = oracle.decay_attention(q.double(), k.double(), v.double(), lam)
+    osz, fsz = _sizes(q.double(), k.double(), v.double(), lam, None, None, None)
+    for got, st in ((whole, last), (torch.cat(parts, 1), state)):
+        _check(got, want, osz, T, D, "o")
+        _check(st, fin, fsz, T, D, "state", True)
+
+
+def test_repeats_and_graphs(cuda0):
+    """The same bits again, also from captured graphs that live side by side and on another stream."""
+    from nexar_b200 import ops
+    q, k, v, do, s0, ds, lam = _inputs(cuda0, 1, 1200, 2, 64, 13)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, s0)]
+
+    def run():
+        o, f = ops.decay_attention(q, k, v, lam, s0, return_state=True)
+        return [t.detach() for t in (o, f, *torch.autograd.grad((o, f), leaves, (do, ds)))]
+    want = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            graphs.append((g, run()))
+    for g, _ in graphs:
+        g.replay()
+    for _, out in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_step_marks_the_state_as_changed(cuda0):
+    from nexar_b200 import ops
+    q, k, v, do, s0, _, lam = _inputs(cuda0, 1, 10, 2, 64, 14)
+    q.requires_grad_(True)
+    o = ops.decay_attention(q, k, v, lam, state=s0)
+    with torch.no_grad():
+        ops.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], lam, s0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(o, q, do)
+
+
+def test_empty_and_refusals(cuda0):
+    from nexar_b200 import ops
+    q, k, v, _, s0, _, lam = _inputs(cuda0, 2, 8, 2, 64, 15)
+    o, f = ops.decay_attention(q[:, :0], k[:, :0], v[:, :0], lam, state=s0, return_state=True)
+    assert o.shape == (2, 0, 2, 64) and torch.equal(f, s0)
+    assert not ops.decay_attention(q[:, :0], k[:, :0], v[:, :0], lam, return_state=True)[1].any()
+    assert ops.decay_attention(q[:0], k[:0], v[:0], lam).shape == (0, 8, 2, 64)
+    n = torch.tensor([1, 2], device=cuda0, dtype=torch.int32)
+    bad = [lambda: ops.decay_attention(q.half(), k.half(), v.half(), lam), lambda: ops.decay_attention(q, k[:, :4], v, lam),
+           lambda: ops.decay_attention(q[..., :32], k[..., :32], v[..., :32], lam),
+           lambda: ops.decay_attention(q, k, v, lam.double()), lambda: ops.decay_attention(q, k, v, lam[:1]),
+           lambda: ops.decay_attention(q, k, v, lam.cpu()), lambda: ops.decay_attention(q, k, v.cpu(), lam),
+           lambda: ops.decay_attention(q, k, v, lam, state=s0.half()), lambda: ops.decay_attention(q, k, v, lam, state=s0[:1]),
+           lambda: ops.decay_attention(q, k, v, lam, state=s0.transpose(2, 3)),
+           lambda: ops.decay_attention(q, k, v, lam, lengths=n.long()), lambda: ops.decay_attention(q, k, v, lam, lengths=n[:1]),
+           lambda: ops.decay_attention_step(q, k, v, lam, s0), lambda: ops.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], lam, s0[:1]),
+           lambda: ops.decay_attention_step(q[:, 0], k[:, 0, :1], v[:, 0], lam, s0)]
+    for f in bad:
+        with pytest.raises(RuntimeError, match="nexar_b200"):
+            f()
