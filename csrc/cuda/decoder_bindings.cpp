@@ -2,6 +2,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <cmath>
 #include <limits>
@@ -156,10 +157,14 @@ std::tuple<at::Tensor, OptTensor> op_dropout(const at::Tensor& x_in, const at::T
   const Drop d = drop_of(p, site);
   const int64_t* st = drop_state(state, x_in);
   c10::cuda::CUDAGuard g(x_in.get_device());
-  const at::Tensor x = x_in.contiguous();
-  at::Tensor y = at::empty_like(x);
   OptTensor snap;
   if (note) snap = at::empty({2}, state.options());
+  if (d.threshold == 0) {  // nothing is dropped
+    if (snap) snap->copy_(state.view({2}));
+    return {x_in.clone(at::MemoryFormat::Contiguous), snap};
+  }
+  const at::Tensor x = x_in.contiguous();
+  at::Tensor y = at::empty_like(x);
   if (x.numel() > 0) {
     check(dropout(x.data_ptr(), y.data_ptr(), x.numel(), code, st, d.site, d.threshold, d.scale,
                   snap ? snap->data_ptr<int64_t>() : nullptr, stream_on(x)),
@@ -191,6 +196,7 @@ std::vector<at::Tensor> op_dropout_ln_fwd(const at::Tensor& x, const at::Tensor&
   need_rows(b, x, C, "bias");
   if (rb) need_rows(*rb, x, C, "rbias");
   const Drop d = drop_of(p, site);
+  TORCH_CHECK(d.threshold > 0, "nexar_b200: residual_layer_norm: a probability of ", std::to_string(p), " drops nothing");
   const int64_t* st = drop_state(state, x);
   c10::cuda::CUDAGuard g(x.get_device());
   at::Tensor s = at::empty_like(x), y = at::empty_like(x);
@@ -436,16 +442,198 @@ at::Tensor op_decay_step(const at::Tensor& q_in, const at::Tensor& k_in, const a
   if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();  // a graph that saved the old state notices
   return o;
 }
+
+// ---------------------------------------------------------------- autograd
+// The graph nodes live here: a small call costs its kernel, not the interpreter.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool any_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t && t->defined() && t->requires_grad()) return true;
+  return false;
+}
+const at::Tensor* ptr(const OptTensor& t) { return t ? &*t : nullptr; }
+at::Tensor or_none(const OptTensor& t) { return t ? *t : at::Tensor(); }
+OptTensor opt(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+// Gradients that come from kernels without a backward of their own: a second
+// derivative raises instead of being silently absent.
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list given;
+  for (at::Tensor& t : grads)
+    if (t.defined()) given.push_back(t.detach().requires_grad_(true));
+  auto node = std::make_shared<torch::autograd::DelayedError>(
+      std::string("nexar_b200: ") + what + " has no second derivative", (int64_t)given.size());
+  variable_list marked = (*node)(std::move(given));
+  size_t i = 0;
+  for (at::Tensor& t : grads)
+    if (t.defined()) t = marked[i++];
+  return grads;
+}
+
+std::vector<at::Tensor> rotate(const at::Tensor& x0, const OptTensor& x1, const at::Tensor& table,
+                               const OptTensor& positions, int64_t start, int64_t heads, bool interleaved,
+                               bool inverse);
+
+// The turn is orthogonal up to the table's magnitude: its adjoint is the turn by
+// the opposite angles with the same magnitude.
+struct RotaryFn : public torch::autograd::Function<RotaryFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x0, const OptTensor& x1,
+                               const at::Tensor& table, const OptTensor& positions, int64_t start, int64_t heads,
+                               bool interleaved, bool inverse) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({table, or_none(positions)});
+    ctx->saved_data["start"] = start;
+    ctx->saved_data["heads"] = heads;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    return op_rotary(x0, x1, table, positions, start, heads, interleaved, inverse);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    const auto saved = ctx->get_saved_variables();
+    variable_list out(8);
+    std::vector<at::Tensor> given;
+    for (const at::Tensor& d : dy)
+      if (d.defined()) given.push_back(d);
+    if (given.empty()) return out;
+    const auto got = rotate(given[0], given.size() > 1 ? OptTensor(given[1]) : OptTensor(), saved[0], opt(saved[1]),
+                            ctx->saved_data["start"].toInt(), ctx->saved_data["heads"].toInt(),
+                            ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["inverse"].toBool());
+    size_t i = 0;
+    for (size_t k = 0; k < dy.size(); ++k)
+      if (dy[k].defined()) out[k] = got[i++];
+    return out;
+  }
+};
+std::vector<at::Tensor> rotate(const at::Tensor& x0, const OptTensor& x1, const at::Tensor& table,
+                               const OptTensor& positions, int64_t start, int64_t heads, bool interleaved,
+                               bool inverse) {
+  TORCH_CHECK_VALUE(!table.requires_grad(), "nexar_b200: the rotary table takes no gradient");
+  if (any_grad({&x0, ptr(x1)})) return RotaryFn::apply(x0, x1, table, positions, start, heads, interleaved, inverse);
+  return op_rotary(x0, x1, table, positions, start, heads, interleaved, inverse);
+}
+
+at::Tensor drop(const at::Tensor& x, const at::Tensor& state, int64_t site, double p);
+
+struct DropoutFn : public torch::autograd::Function<DropoutFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& state, int64_t site,
+                            double p) {
+    auto [y, used] = op_dropout(x, state, site, p, true);
+    ctx->save_for_backward({*used});
+    ctx->saved_data["site"] = site;
+    ctx->saved_data["p"] = p;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    return {drop(dy[0], ctx->get_saved_variables()[0], ctx->saved_data["site"].toInt(), ctx->saved_data["p"].toDouble()),
+            at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+at::Tensor drop(const at::Tensor& x, const at::Tensor& state, int64_t site, double p) {
+  if (any_grad({&x})) return DropoutFn::apply(x, state, site, p);
+  return std::get<0>(op_dropout(x, state, site, p, false));
+}
+
+// s = x + drop(r + rb), y = LayerNorm(s) for parameters with ordinary gradients.
+struct DropoutLayerNormFn : public torch::autograd::Function<DropoutLayerNormFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& r, const OptTensor& rb,
+                               const at::Tensor& w, const at::Tensor& b, double eps, const at::Tensor& state,
+                               int64_t site, double p) {
+    ctx->set_materialize_grads(false);
+    auto out = op_dropout_ln_fwd(x.contiguous(), r.contiguous(), rb, w, b, eps, state, site, p);
+    ctx->save_for_backward({out[0], w, out[2], out[3], out[4], or_none(rb)});
+    ctx->saved_data["site"] = site;
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["r"] = r.sizes().vec();
+    return {out[0], out[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list d) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &s = saved[0], &w = saved[1], &rb = saved[5];
+    const at::Tensor dy = d[1].defined() ? d[1].contiguous() : at::zeros_like(s);
+    OptTensor ds, drb;
+    if (d[0].defined()) ds = d[0].contiguous();
+    if (rb.defined()) drb = at::empty_like(rb);
+    at::Tensor dw = at::empty_like(w), db = at::empty_like(w);
+    auto g = op_dropout_ln_bwd(dy, s, saved[2], saved[3], w, ds, dw, db, drb, saved[4],
+                               ctx->saved_data["site"].toInt(), ctx->saved_data["p"].toDouble());
+    return once({g[0], g[1].view(ctx->saved_data["r"].toIntVector()), or_none(drb), dw, db, at::Tensor(), at::Tensor(),
+                 at::Tensor(), at::Tensor()},
+                "residual_layer_norm with dropout");
+  }
+};
+variable_list dropout_layer_norm(const at::Tensor& x, const at::Tensor& r, const OptTensor& rb, const at::Tensor& w,
+                                 const at::Tensor& b, double eps, const at::Tensor& state, int64_t site, double p) {
+  return DropoutLayerNormFn::apply(x, r, rb, w, b, eps, state, site, p);
+}
+
+// q, k, v [B, T, H, D], or (k and v absent) one packed qkv [B, T, 3, H, D].
+struct DecayFn : public torch::autograd::Function<DecayFn> {
+  static std::vector<at::Tensor> parts(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v) {
+    return k.defined() ? std::vector<at::Tensor>{q, k, v} : q.unbind(2);
+  }
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const OptTensor& k, const OptTensor& v,
+                               const at::Tensor& log_decay, const OptTensor& state, const OptTensor& lengths,
+                               double scale, bool want_state) {
+    ctx->set_materialize_grads(false);
+    const auto a = parts(q, or_none(k), or_none(v));
+    auto [o, fin] = op_decay_fwd(a[0], a[1], a[2], log_decay, state, lengths, scale, want_state);
+    ctx->save_for_backward({q, or_none(k), or_none(v), log_decay, or_none(state), or_none(lengths)});
+    ctx->saved_data["scale"] = scale;
+    if (!want_state) return {o};
+    return {o, *fin};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list d) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &q = saved[0], &k = saved[1];
+    const auto a = parts(q, k, saved[2]);
+    variable_list out(8);
+    at::Tensor packed;
+    std::vector<at::Tensor> g;
+    if (k.defined()) {
+      for (int i = 0; i < 3; ++i) g.push_back(at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous)));
+    } else {
+      packed = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+      g = packed.unbind(2);
+    }
+    const at::Tensor dO = d[0].defined() ? d[0] : at::zeros(a[0].sizes(), q.options());
+    OptTensor ds;
+    if (d.size() > 1 && d[1].defined()) ds = d[1].contiguous();
+    const OptTensor ds0 = op_decay_bwd(a[0], a[1], a[2], dO, saved[3], opt(saved[4]), ds, opt(saved[5]),
+                                       ctx->saved_data["scale"].toDouble(), g[0], g[1], g[2],
+                                       saved[4].defined() && ctx->needs_input_grad(k.defined() ? 4 : 2));
+    out[0] = k.defined() ? g[0] : packed;
+    if (k.defined()) out[1] = g[1], out[2] = g[2];
+    out[4] = or_none(ds0);
+    return once(out, "decay attention");
+  }
+};
+variable_list decay(const at::Tensor& q, const OptTensor& k, const OptTensor& v, const at::Tensor& log_decay,
+                    const OptTensor& state, const OptTensor& lengths, double scale, bool want_state) {
+  TORCH_CHECK_VALUE(k || q.dim() == 5, "nexar_b200: decay_attention_qkv takes qkv [B, T, 3, H, D]");
+  TORCH_CHECK_VALUE(k || q.size(2) == 3, "nexar_b200: decay_attention_qkv takes qkv [B, T, 3, H, D]");
+  TORCH_CHECK_VALUE(!log_decay.requires_grad(),
+                    "nexar_b200: decay attention: the decays are fixed; log_decay takes no gradient (detach it)");
+  if (any_grad({&q, ptr(k), ptr(v), ptr(state)}))
+    return DecayFn::apply(q, k, v, log_decay, state, lengths, scale, want_state);
+  const auto a = DecayFn::parts(q, or_none(k), or_none(v));
+  auto [o, fin] = op_decay_fwd(a[0], a[1], a[2], log_decay, state, lengths, scale, want_state);
+  if (!want_state) return {o};
+  return {o, *fin};
+}
 }  // namespace
 
 void register_decoder_ops(py::module& m) {
-  m.def("rotary", &op_rotary);
+  m.def("rotary", &rotate);
   m.def("rotary_table", &op_rotary_table);
-  m.def("dropout", &op_dropout);
+  m.def("dropout", &drop);
+  m.def("dropout_ln", &dropout_layer_norm);
   m.def("dropout_ln_fwd", &op_dropout_ln_fwd);
   m.def("dropout_ln_bwd", &op_dropout_ln_bwd);
-  m.def("decay_fwd", &op_decay_fwd);
-  m.def("decay_bwd", &op_decay_bwd);
+  m.def("decay_attention", &decay);
   m.def("decay_step", &op_decay_step);
 }
 

@@ -15,78 +15,100 @@
 // (seed, step) are read from device memory, so a captured graph draws anew when
 // the step advances between replays; the forward kernel notes the two values it
 // used, and the backward reads those.
-#include "common.cuh"
 #include "decoder_api.h"
+#include "pack.cuh"
 
 namespace nexar {
 
 namespace {
 constexpr int kDropThreads = 256;
 
-struct DropKey {
-  uint32_t k0, k1, step;
-};
-NEXAR_D DropKey drop_key(const int64_t* state) {
-  const unsigned long long seed = (unsigned long long)state[0];
-  return DropKey{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)(unsigned long long)state[1]};
-}
-
-// The 128 bits of one block.
-NEXAR_D uint4 philox(unsigned long long block, uint32_t site, const DropKey& key) {
-  uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = site, c3 = key.step;
-  uint32_t k0 = key.k0, k1 = key.k1;
+// The generator under one (seed, step, site): the ten round keys are formed
+// once per thread and stay in registers.
+struct Draws {
+  uint32_t k0[10], k1[10], site, step;
+  NEXAR_D Draws(const int64_t* state, uint32_t site_) : site(site_) {
+    const unsigned long long seed = (unsigned long long)state[0];
+    step = (uint32_t)(unsigned long long)state[1];
 #pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const unsigned long long p0 = (unsigned long long)c0 * 0xD2511F53u;
-    const unsigned long long p1 = (unsigned long long)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
-    c1 = (uint32_t)p1;
-    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
-    c3 = (uint32_t)p0;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
+    for (int r = 0; r < 10; ++r) {
+      k0[r] = (uint32_t)seed + r * 0x9E3779B9u;
+      k1[r] = (uint32_t)(seed >> 32) + r * 0xBB67AE85u;
+      asm volatile("" : "+r"(k0[r]), "+r"(k1[r]));  // kept: formed again per block they cost 20 of 130 instructions
+    }
   }
-  return make_uint4(c0, c1, c2, c3);
-}
+  // The 128 bits of one block.
+  NEXAR_D uint4 operator()(unsigned long long block) const {
+    uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = site, c3 = step;
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+      const unsigned long long p0 = (unsigned long long)c0 * 0xD2511F53u;
+      const unsigned long long p1 = (unsigned long long)c2 * 0xCD9E8D57u;
+      c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0[r];
+      c1 = (uint32_t)p1;
+      c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1[r];
+      c3 = (uint32_t)p0;
+    }
+    return make_uint4(c0, c1, c2, c3);
+  }
+};
 
-// Bit e: element e of the block is kept.
-NEXAR_D uint32_t keep_bits(unsigned long long block, uint32_t site, const DropKey& key, uint32_t threshold) {
-  const uint4 w = philox(block, site, key);
-  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-  uint32_t m = 0;
+// v[e] = kept ? v[e] * scale : 0 for the block's 8 elements (selected, not
+// multiplied by 0: a dropped infinity leaves no NaN). The draws are compared
+// where they lie: a word is >= threshold << 16 exactly when its high half is >=
+// threshold, and so is the word moved up by 16 for its low half. `below` is
+// (threshold << 16) - 1, which fits 32 bits for thresholds 1 .. 65536.
+NEXAR_D void drop8(float* v, const uint4& w, uint32_t below, float scale) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    m |= ((v[e] & 0xffffu) >= threshold ? 1u : 0u) << (2 * e);
-    m |= ((v[e] >> 16) >= threshold ? 1u : 0u) << (2 * e + 1);
+    v[2 * e] = (u[e] << 16) > below ? v[2 * e] * scale : 0.f;
+    v[2 * e + 1] = u[e] > below ? v[2 * e + 1] * scale : 0.f;
   }
-  return m;
 }
 
-template <typename T> struct alignas(16) Eight {
-  T e[8];
-};
-
-template <typename T, bool VEC>
+// U blocks of 8 elements per thread, all loaded before the first is drawn for.
+template <typename T, bool VEC, int U>
 __global__ void __launch_bounds__(kDropThreads) k_dropout(const T* __restrict__ x, T* __restrict__ y, long long n,
                                                           const int64_t* __restrict__ state, uint32_t site,
                                                           uint32_t threshold, float scale,
                                                           int64_t* __restrict__ snapshot) {
-  const DropKey key = drop_key(state);
+  const uint32_t below = (threshold << 16) - 1;
   if (snapshot && blockIdx.x == 0 && threadIdx.x < 2) snapshot[threadIdx.x] = state[threadIdx.x];
-  const long long blocks = (n + 7) / 8;
-  for (long long i = blockIdx.x * (long long)kDropThreads + threadIdx.x; i < blocks;
-       i += (long long)gridDim.x * kDropThreads) {
-    if (VEC && i * 8 + 8 <= n) {
-      Eight<T> v = *reinterpret_cast<const Eight<T>*>(x + i * 8);
-      const uint32_t keep = keep_bits((unsigned long long)i, site, key, threshold);
+  const long long blocks = (n + 7) / 8, first = blockIdx.x * (long long)(U * kDropThreads) + threadIdx.x;
+  Pack<T, 8> v[U];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)  // selected, not multiplied: an infinity that is dropped leaves no NaN
-        v.e[e] = from_acc<T, float>((keep >> e) & 1u ? to_acc<float>(v.e[e]) * scale : 0.f);
-      *reinterpret_cast<Eight<T>*>(y + i * 8) = v;
+  for (int k = 0; k < U; ++k) {
+    const long long i = first + k * kDropThreads;
+    if (VEC && i * 8 + 8 <= n) {
+      v[k].load(x + i * 8);
+    } else {  // the last block of fewer than 8 elements, or any of them without alignment
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[k].set(e, i * 8 + 2 * e < n ? to_acc<float>(x[i * 8 + 2 * e]) : 0.f,
+                 i * 8 + 2 * e + 1 < n ? to_acc<float>(x[i * 8 + 2 * e + 1]) : 0.f);
+    }
+  }
+  const Draws draws(state, site);
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const long long i = first + k * kDropThreads;
+    if (i >= blocks) return;
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 t = v[k].get(e);
+      f[2 * e] = t.x, f[2 * e + 1] = t.y;
+    }
+    drop8(f, draws((unsigned long long)i), below, scale);
+    if (VEC && i * 8 + 8 <= n) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[k].set(e, f[2 * e], f[2 * e + 1]);
+      v[k].store(y + i * 8);
     } else {
-      const uint32_t keep = keep_bits((unsigned long long)i, site, key, threshold);
-      for (int e = 0; e < 8 && i * 8 + e < n; ++e)
-        y[i * 8 + e] = from_acc<T, float>((keep >> e) & 1u ? to_acc<float>(x[i * 8 + e]) * scale : 0.f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i * 8 + e < n) y[i * 8 + e] = from_acc<T, float>(f[e]);
     }
   }
 }
@@ -130,7 +152,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_dropout_ln_fwd(
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
   if (row >= R) return;
-  const DropKey key = drop_key(state);
+  const Draws draws(state, site);
+  const uint32_t below = (threshold << 16) - 1;
   const size_t base = (size_t)row * C;
   uint4 vx[NP], vr[NP];
 #pragma unroll
@@ -155,9 +178,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_dropout_ln_fwd(
 #pragma unroll
         for (int e = 0; e < 8; ++e) d[e] += t[e];
       }
-      const uint32_t keep = keep_bits((base + col) >> 3, site, key, threshold);
+      drop8(d, draws((base + col) >> 3), below, scale);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a[e] += (keep >> e) & 1u ? d[e] * scale : 0.f;
+      for (int e = 0; e < 8; ++e) a[e] += d[e];
       vx[k] = pack8(a);
       *reinterpret_cast<uint4*>(sum_out + base + col) = vx[k];
       unpack8(vx[k], a);
@@ -196,14 +219,14 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_dropout_ln_fwd(
   }
 }
 
-// Backward. A block of C/8 threads (whole warps) walks over its rows four at a
+// Backward. A block of C/8 threads (whole warps) walks over its rows two at a
 // time; a thread owns 8 columns, so the column sums (dw, db, drb) stay in 24
-// registers however wide the row is. Each group of four rows costs one barrier
+// registers however wide the row is. Each pair of rows costs one barrier
 // for the two row sums. The blocks' column sums go to `part` and are added in a
 // fixed order by k_dropout_ln_columns: no atomics, the same bits every run.
-constexpr int kBwdRows = 4;
+constexpr int kBwdRows = 2;
 template <bool BIAS>
-__global__ void __launch_bounds__(256) k_dropout_ln_bwd(
+__global__ void __launch_bounds__(256, 2) k_dropout_ln_bwd(
     const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ s, const float* __restrict__ mean,
     const float* __restrict__ rstd, const __nv_bfloat16* __restrict__ w, const __nv_bfloat16* __restrict__ dres,
     __nv_bfloat16* __restrict__ dx, __nv_bfloat16* __restrict__ dr, float* __restrict__ part, int R, int C,
@@ -212,7 +235,8 @@ __global__ void __launch_bounds__(256) k_dropout_ln_bwd(
   const int col = threadIdx.x * 8;
   const bool mine = col < C;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const DropKey key = drop_key(state);
+  const Draws draws(state, site);
+  const uint32_t below = (threshold << 16) - 1;
   float aw[8], ab[8], ad[8], wf[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) aw[e] = ab[e] = ad[e] = wf[e] = 0.f;
@@ -279,9 +303,7 @@ __global__ void __launch_bounds__(256) k_dropout_ln_bwd(
         o[e] += rs[k] * (g[e] * wf[e] - sums[2 * k] - xh[e] * sums[2 * k + 1]);
       }
       ox[k] = pack8(o);
-      const uint32_t keep = keep_bits(((size_t)(row0 + k) * C + col) >> 3, site, key, threshold);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = (keep >> e) & 1u ? o[e] * scale : 0.f;
+      drop8(o, draws(((size_t)(row0 + k) * C + col) >> 3), below, scale);
       od[k] = pack8(o);
       if constexpr (BIAS) {
         const bool ok = row0 + k < R;
@@ -317,34 +339,32 @@ __global__ void __launch_bounds__(256) k_dropout_ln_bwd(
 }
 
 // Column sums of the P partial rows of W = (2 or 3) C values, in a fixed order:
-// 16 lanes of 4 columns by 16 slices of the partial rows per block.
+// 8 lanes of 4 columns by 32 slices of the partial rows per block.
 __global__ void __launch_bounds__(256) k_dropout_ln_columns(const float* __restrict__ part, int P, int W, int C,
                                                             __nv_bfloat16* dw, __nv_bfloat16* db,
                                                             __nv_bfloat16* drb) {
-  __shared__ float4 red[16][16];
-  const int cg = threadIdx.x & 15, sl = threadIdx.x >> 4;
-  const int col = (blockIdx.x * 16 + cg) * 4;
+  __shared__ float4 red[32][8];
+  const int cg = threadIdx.x & 7, sl = threadIdx.x >> 3;
+  const int col = (blockIdx.x * 8 + cg) * 4;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   if (col < W) {
-#pragma unroll 4
-    for (int p = sl; p < P; p += 16) {
+#pragma unroll 8
+    for (int p = sl; p < P; p += 32) {
       const float4 v = *reinterpret_cast<const float4*>(part + (size_t)p * W + col);
       a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
     }
   }
   red[sl][cg] = a;
   __syncthreads();
-  if (sl == 0 && col < W) {
-    for (int j = 1; j < 16; ++j) {
-      const float4 v = red[j][cg];
-      a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+  if (threadIdx.x < 32) {  // one thread per column
+    const int c1 = blockIdx.x * 32 + threadIdx.x;
+    if (c1 < W) {
+      float t = 0.f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) t += reinterpret_cast<const float*>(red[j])[threadIdx.x];
+      const int which = c1 / C;
+      (which == 0 ? dw : which == 1 ? db : drb)[c1 % C] = __float2bfloat16_rn(t);
     }
-    const int which = col / C, c = col % C;  // C % 4 == 0: four columns are of one output
-    __nv_bfloat16* o = which == 0 ? dw : (which == 1 ? db : drb);
-    o[c] = __float2bfloat16_rn(a.x);
-    o[c + 1] = __float2bfloat16_rn(a.y);
-    o[c + 2] = __float2bfloat16_rn(a.z);
-    o[c + 3] = __float2bfloat16_rn(a.w);
   }
 }
 
@@ -353,7 +373,7 @@ __global__ void __launch_bounds__(256) k_dropout_ln_columns(const float* __restr
 // fits the GPU at once.
 int bwd_blocks(int R, int C) {
   const int threads = (C / 8 + 31) / 32 * 32;
-  const int per_sm = threads <= 96 ? 4 : (threads <= 128 ? 3 : 2);
+  const int per_sm = threads <= 128 ? 4 : 2;
   const int groups = (R + kBwdRows - 1) / kBwdRows;
   return groups < 148 * per_sm ? (groups < 1 ? 1 : groups) : 148 * per_sm;
 }
@@ -361,21 +381,23 @@ int bwd_blocks(int R, int C) {
 template <typename T>
 cudaError_t dropout_typed(const void* x, void* y, long long n, const int64_t* state, uint32_t site, uint32_t thr,
                           float scale, int64_t* snapshot, cudaStream_t s) {
-  const long long blocks = ((n + 7) / 8 + kDropThreads - 1) / kDropThreads;
-  const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
+  const long long blocks = (n + 7) / 8;
   const T* xi = reinterpret_cast<const T*>(x);
   T* yo = reinterpret_cast<T*>(y);
-  if ((uintptr_t)x % 16 == 0 && (uintptr_t)y % 16 == 0)
-    k_dropout<T, true><<<grid, kDropThreads, 0, s>>>(xi, yo, n, state, site, thr, scale, snapshot);
-  else
-    k_dropout<T, false><<<grid, kDropThreads, 0, s>>>(xi, yo, n, state, site, thr, scale, snapshot);
+  constexpr int U = sizeof(T) == 4 ? 2 : 4;
+  const bool many = blocks > 148LL * 2048;  // else one block per thread, for the shortest path
+  const long long per = (many ? U : 1) * kDropThreads, grid = (blocks + per - 1) / per;
+  if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const auto kernel = (uintptr_t)x % 16 || (uintptr_t)y % 16 ? (many ? k_dropout<T, false, U> : k_dropout<T, false, 1>)
+                                                             : (many ? k_dropout<T, true, U> : k_dropout<T, true, 1>);
+  kernel<<<(unsigned)grid, kDropThreads, 0, s>>>(xi, yo, n, state, site, thr, scale, snapshot);
   return cudaGetLastError();
 }
 }  // namespace
 
 cudaError_t dropout(const void* x, void* y, long long n, int dtype, const int64_t* state, uint32_t site,
                     uint32_t threshold, float scale, int64_t* snapshot, cudaStream_t s) {
-  if (n <= 0) return cudaErrorInvalidValue;
+  if (n <= 0 || threshold < 1 || threshold > 65536) return cudaErrorInvalidValue;
   if (dtype == 0) return dropout_typed<__nv_bfloat16>(x, y, n, state, site, threshold, scale, snapshot, s);
   if (dtype == 1) return dropout_typed<__half>(x, y, n, state, site, threshold, scale, snapshot, s);
   return dropout_typed<float>(x, y, n, state, site, threshold, scale, snapshot, s);
@@ -385,7 +407,7 @@ cudaError_t dropout_ln_fwd(const __nv_bfloat16* x, const __nv_bfloat16* r, const
                            __nv_bfloat16* sum_out, const __nv_bfloat16* w, const __nv_bfloat16* b, __nv_bfloat16* y,
                            float* mean, float* rstd, int R, int C, float eps, const int64_t* state, uint32_t site,
                            uint32_t threshold, float scale, int64_t* snapshot, cudaStream_t s) {
-  if (C % 8 || C > 2048 || R < 1) return cudaErrorInvalidValue;
+  if (C % 8 || C > 2048 || R < 1 || threshold < 1 || threshold > 65536) return cudaErrorInvalidValue;
   const int grid = (R + kRowWarps - 1) / kRowWarps;
 #define NEXAR_DROP_FWD(NP)                                                                                     \
   k_dropout_ln_fwd<NP><<<grid, kRowWarps * 32, 0, s>>>(x, r, rb, sum_out, w, b, y, mean, rstd, R, C, eps, state, \
@@ -406,7 +428,7 @@ cudaError_t dropout_ln_bwd(const __nv_bfloat16* dy, const __nv_bfloat16* s_in, c
                            const __nv_bfloat16* w, const __nv_bfloat16* dres, __nv_bfloat16* dx, __nv_bfloat16* dr,
                            __nv_bfloat16* dw, __nv_bfloat16* db, __nv_bfloat16* drb, float* scratch, int R, int C,
                            const int64_t* state, uint32_t site, uint32_t threshold, float scale, cudaStream_t s) {
-  if (C % 8 || C > 2048 || R < 1) return cudaErrorInvalidValue;
+  if (C % 8 || C > 2048 || R < 1 || threshold < 1 || threshold > 65536) return cudaErrorInvalidValue;
   const int grid = bwd_blocks(R, C), threads = (C / 8 + 31) / 32 * 32;
   if (drb)
     k_dropout_ln_bwd<true><<<grid, threads, 0, s>>>(dy, s_in, mean, rstd, w, dres, dx, dr, scratch, R, C, state, site,
@@ -417,7 +439,7 @@ cudaError_t dropout_ln_bwd(const __nv_bfloat16* dy, const __nv_bfloat16* s_in, c
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int W = (drb ? 3 : 2) * C;
-  k_dropout_ln_columns<<<(W + 63) / 64, 256, 0, s>>>(scratch, grid, W, C, dw, db, drb);
+  k_dropout_ln_columns<<<(W + 31) / 32, 256, 0, s>>>(scratch, grid, W, C, dw, db, drb);
   return cudaGetLastError();
 }
 

@@ -101,36 +101,6 @@ def _interleaved(layout: str) -> bool:
     return layout == "interleaved"
 
 
-def _rotate(xs, table, positions, start, heads, interleaved, inverse):
-    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
-        if table.requires_grad:
-            raise ValueError("the rotary table takes no gradient")
-        return _Rotary.apply(table, positions, start, heads, interleaved, inverse, *xs)
-    return tuple(_native.cuda().rotary(xs[0], xs[1] if len(xs) > 1 else None, table, positions, start, heads,
-                                       interleaved, inverse))
-
-
-class _Rotary(torch.autograd.Function):
-    """The turn is orthogonal up to the table's magnitude m: its adjoint is the
-    turn by the opposite angles (with the same m)."""
-
-    @staticmethod
-    def forward(ctx, table, positions, start, heads, interleaved, inverse, *xs):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(table, positions)
-        ctx.how = (start, heads, interleaved, inverse)
-        return tuple(_native.cuda().rotary(xs[0], xs[1] if len(xs) > 1 else None, table, positions, start, heads,
-                                           interleaved, inverse))
-
-    @staticmethod
-    def backward(ctx, *dys):
-        table, positions = ctx.saved_tensors
-        start, heads, interleaved, inverse = ctx.how
-        given = [d for d in dys if d is not None]
-        got = iter(_rotate(given, table, positions, start, heads, interleaved, not inverse) if given else ())
-        return (None,) * 6 + tuple(None if d is None else next(got) for d in dys)
-
-
 def rotary(x, table, positions=None, start: int = 0, heads: Optional[int] = None, layout: str = "half"):
     """Rotary positions of x [T, H, D] or [B, T, H, D] (bf16, fp16 or fp32, any strides): the first
     ``table.shape[1]`` elements of a head turn by their position's angles, the rest is copied.
@@ -142,12 +112,13 @@ def rotary(x, table, positions=None, start: int = 0, heads: Optional[int] = None
     (2i, 2i + 1) ("interleaved"). Returns a contiguous tensor; differentiable in x."""
     if heads is not None and heads < 0:
         raise ValueError(f"heads must not be negative, got {heads}")
-    return _rotate((x,), table, positions, start, -1 if heads is None else heads, _interleaved(layout), False)[0]
+    return _native.cuda().rotary(x, None, table, positions, start, -1 if heads is None else heads,
+                                 _interleaved(layout), False)[0]
 
 
 def rotary_qk(q, k, table, positions=None, start: int = 0, layout: str = "half"):
     """:func:`rotary` of queries [B, T, H, D] and keys [B, T, Hk, D] in one launch: returns both."""
-    return _rotate((q, k), table, positions, start, -1, _interleaved(layout), False)
+    return tuple(_native.cuda().rotary(q, k, table, positions, start, -1, _interleaved(layout), False))
 
 
 # ---------------------------------------------------------------- dropout
@@ -179,32 +150,12 @@ def _check_dropout(p: float, state) -> None:
         raise TypeError("dropout needs a DropoutState")
 
 
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, state, site, p):
-        y, used = _native.cuda().dropout(x, state, site, p, True)
-        ctx.save_for_backward(used)
-        ctx.how = (site, p)
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        (used,) = ctx.saved_tensors
-        return _drop(dy, used, *ctx.how), None, None, None
-
-
-def _drop(x, state, site, p):
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _Dropout.apply(x, state, site, p)
-    return _native.cuda().dropout(x, state, site, p, False)[0]
-
-
 def dropout(x, p: float, state: DropoutState, site: int = 0):
     """Zero each element of x (bf16, fp16 or fp32) with probability ``p`` (rounded to a multiple of
     2^-16) and scale the others by the inverse of the probability to be kept. No mask is stored: the
     backward draws it again from the (seed, step) that the forward used. Returns a contiguous tensor."""
     _check_dropout(p, state)
-    return _drop(x, state.tensor, site, p)
+    return _native.cuda().dropout(x, state.tensor, site, p)
 
 
 # ---------------------------------------------------------------- attention with a decay per head
@@ -212,52 +163,8 @@ def _decay_scale(scale, D):
     return D ** -0.5 if scale is None else float(scale)
 
 
-def _no_decay_grad(log_decay):
-    if log_decay.requires_grad:
-        raise ValueError("decay attention: the decays are fixed; log_decay takes no gradient (detach it)")
-
-
-class _DecayAttention(torch.autograd.Function):
-    """q, k, v [B, T, H, D], or (packed) one qkv [B, T, 3, H, D] with k = v = None."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, log_decay, state, lengths, scale, return_state):
-        ctx.set_materialize_grads(False)
-        ctx.packed = k is None
-        a = q.unbind(2) if ctx.packed else (q, k, v)
-        o, final = _native.cuda().decay_fwd(*a, log_decay, state, lengths, scale, return_state)
-        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
-        ctx.scale = scale
-        return o, final
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, do, dstate):
-        q, k, v, log_decay, state, lengths = ctx.saved_tensors
-        a = q.unbind(2) if ctx.packed else (q, k, v)
-        if ctx.packed:
-            grads = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            d = grads.unbind(2)
-        else:
-            d = grads = tuple(torch.empty(q.shape, dtype=q.dtype, device=q.device) for _ in range(3))
-        if do is None:
-            do = torch.zeros(a[0].shape, dtype=q.dtype, device=q.device)
-        if dstate is not None:
-            dstate = dstate.contiguous()
-        ds0 = _native.cuda().decay_bwd(*a, do, log_decay, state, dstate, lengths, ctx.scale, *d,
-                                       ctx.needs_input_grad[4])
-        if ctx.packed:
-            return grads, None, None, None, ds0, None, None, None
-        return (*grads, None, ds0, None, None, None)
-
-
 def _decay(q, k, v, log_decay, state, lengths, scale, return_state):
-    _no_decay_grad(log_decay)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
-        out = _DecayAttention.apply(q, k, v, log_decay, state, lengths, scale, return_state)
-    else:
-        out = _native.cuda().decay_fwd(*(q.unbind(2) if k is None else (q, k, v)), log_decay, state, lengths, scale,
-                                       return_state)
+    out = _native.cuda().decay_attention(q, k, v, log_decay, state, lengths, scale, return_state)
     return tuple(out) if return_state else out[0]
 
 
@@ -280,8 +187,6 @@ def decay_attention_qkv(qkv, log_decay, state=None, lengths=None, scale: Optiona
                         return_state: bool = False):
     """:func:`decay_attention` on a packed projection qkv [B, T, 3, H, D]; the gradient comes back
     packed, in one buffer."""
-    if qkv.dim() != 5 or qkv.shape[2] != 3:
-        raise ValueError(f"decay_attention_qkv takes qkv [B, T, 3, H, D], got {tuple(qkv.shape)}")
     return _decay(qkv, None, None, log_decay, state, lengths, _decay_scale(scale, qkv.shape[-1]), return_state)
 
 

@@ -266,7 +266,8 @@ class _ResidualLayerNorm(torch.autograd.Function):
 
 
 class _ResidualDropoutLayerNorm(torch.autograd.Function):
-    """s = x + dropout(r (+ rb)) ; y = LayerNorm(s), the mask drawn inside the kernels.
+    """s = x + dropout(r (+ rb)) ; y = LayerNorm(s), the mask drawn inside the kernels, for
+    parameters with gradient sinks (without them the extension's own graph node runs).
 
     The backward draws the same mask again from the (seed, step) that the
     forward noted, and returns the gradients of both summands, the LayerNorm's
@@ -311,10 +312,12 @@ def residual_layer_norm(x, r, w, b, eps: float = 1e-5, rbias=None, p: float = 0.
     if p or dropout is not None:
         from .decoder import _check_dropout
         _check_dropout(p, dropout)
-        if p:
+        if round(p * 65536):  # below 2^-17 nothing is dropped
             if r.numel() != x.numel():
                 raise ValueError(f"residual_layer_norm: x has {x.numel()} elements, r {r.numel()}")
-            return _ResidualDropoutLayerNorm.apply(x, r, w, b, rbias, eps, dropout.tensor, site, p)
+            if any(_sink(t) is not None for t in (w, b, rbias) if t is not None):
+                return _ResidualDropoutLayerNorm.apply(x, r, w, b, rbias, eps, dropout.tensor, site, p)
+            return tuple(_native.cuda().dropout_ln(x, r, rbias, w, b, eps, dropout.tensor, site, p))
     return _ResidualLayerNorm.apply(x, r, w, b, rbias, eps)
 
 

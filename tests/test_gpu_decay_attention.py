@@ -266,6 +266,17 @@ def test_step_marks_the_state_as_changed(cuda0):
         torch.autograd.grad(o, q, do)
 
 
+def test_second_derivatives_raise(cuda0):
+    from nexar_b200 import ops
+    q, k, v, do, s0, _, lam = _inputs(cuda0, 1, 10, 2, 64, 16)
+    q.requires_grad_(True)
+    first = torch.autograd.grad(ops.decay_attention(q, k, v, lam), q, do)[0]
+    (g,) = torch.autograd.grad(ops.decay_attention(q, k, v, lam), q, do, create_graph=True)
+    assert torch.equal(g.detach(), first)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        g.float().sum().backward()
+
+
 def test_empty_and_refusals(cuda0):
     from nexar_b200 import ops
     q, k, v, _, s0, _, lam = _inputs(cuda0, 2, 8, 2, 64, 15)
