@@ -19,20 +19,39 @@
 // k_decay_scan turns these into the state before each segment, and the main
 // kernel then runs all segments at once.
 //
+// Per chunk the scores (an eighth of the products) are formed with warp-level
+// MMAs, whose registers hold them where the decay and the mask are applied; they
+// go to shared memory as the operand P. Everything else runs on tcgen05, with the
+// value dimension along the 128 (D = 64: 64) TMEM lanes so that the state keeps
+// one layout from product to operand:
+//     O2 [dv, token] = X^T Q^T,   O1 [dv, token] = V^T P^T,   U [dv, dk] = V^T K'
+// (K': the chunk's keys decayed to its end). X lives in fp32 registers (a row of
+// X^T per thread) and goes back as an operand through TMEM (D = 128, over the
+// columns of U, which is done by then) or shared memory (D = 64).
+// Two blocks per SM: one block's products run while the other prepares.
+//
 // Roundings. Products are bf16 tensor-core products with fp32 sums. The decayed
 // keys that enter the state are split into three bf16 parts (24 bits, all of an
 // fp32 value), so the state is an fp32 state; scores and states that enter the
-// output are split into two parts (16 bits), well below the rounding of the bf16
-// output.
+// bf16 output are split into two parts (16 bits), well below the output's
+// rounding. U is formed apart and added to X once per chunk: the tensor cores cut
+// off what does not fit their accumulator, which on a state that grows over
+// thousands of tokens would add up.
+//
+// Every wait is bounded (2 s); one that gives up sets an error word of its GPU
+// (decay_error_flag), the block leaves together and frees its TMEM.
 #include "common.cuh"
 #include "decoder_api.h"
+#include "sm100.cuh"
 
 namespace nexar {
 
 namespace {
+using namespace sm100;
 constexpr int kChunk = 64;
+constexpr uint64_t kDecayWaitNs = 2000000000ull;
+__device__ unsigned int g_decay_error = 0;  // set once a wait has given up
 
-NEXAR_D uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 NEXAR_D void cp_async16(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? 16 : 0;  // zero-filled where there is no token
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
@@ -41,10 +60,6 @@ NEXAR_D void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); 
 template <int N> NEXAR_D void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 NEXAR_D void ldsm4(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-NEXAR_D void ldsm4t(uint32_t addr, uint32_t* r) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 NEXAR_D void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -59,30 +74,66 @@ NEXAR_D uint32_t bf2(float lo, float hi) {
 NEXAR_D float bf_lo(uint32_t v) { return __uint_as_float(v << 16); }
 NEXAR_D float bf_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
-// Byte offset of 16-byte group `g` of row `r` in a tile of D bf16 columns; the
-// group index is permuted by the row so that ldmatrix finds no bank conflicts.
-template <int D> NEXAR_D uint32_t tile_at(int r, int g) { return (uint32_t)(r * D * 2 + ((g ^ (r & 7)) << 4)); }
-
+// A tile of 64 rows x D bf16 is D / 64 boxes of 64 rows x 128 bytes in the
+// 128-byte-swizzled layout of the tcgen05 descriptors: 16-byte group g of row r.
+NEXAR_D uint32_t tile_at(int r, int g) { return (uint32_t)((g >> 3) * 8192 + r * 128 + (((g & 7) ^ (r & 7)) << 4)); }
 // Per-thread addresses of ldmatrix.x4 over a 16 x 16 block at (row, col): the
 // four 8 x 8 matrices are (rows 0-7, 8-15) x (cols 0-7, 8-15), rows first.
-template <int D> NEXAR_D uint32_t block_at(uint32_t tile, int row, int col, int lane) {
-  return tile + tile_at<D>(row + (lane & 15), (col >> 3) + (lane >> 4));
+NEXAR_D uint32_t block_at(uint32_t tile, int row, int col, int lane) {
+  return tile + tile_at(row + (lane & 15), (col >> 3) + (lane >> 4));
 }
 
-template <int D> struct Shape {
-  static constexpr int kWarps = D / 16;           // one warp per 16 rows of the state
-  static constexpr int kThreads = kWarps * 32;
-  static constexpr int kTile = kChunk * D * 2;    // bytes of one tile of q, k or v
-  static constexpr int kState = D * D * 2;        // bytes of one bf16 part of the state
-  static constexpr int kSmem = 6 * kTile + 2 * kState + 512;
-  static constexpr int kSmemStates = 4 * kTile + 512;  // k and v only, twice
+// MN-major operand: boxes of 64 contiguous MN elements x 64 K rows, 8 KB apart.
+NEXAR_D uint64_t desc_mn(uint32_t addr) { return umma_desc_sw128_mnmajor(addr); }
+// kind::f16 MMA whose A operand is read from tensor memory.
+NEXAR_D void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      :: "r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+NEXAR_D void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+NEXAR_D void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Bounded wait by polling: these waits sit on the chunk's critical path.
+NEXAR_D bool wait_phase(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = globaltimer_ns();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (globaltimer_ns() - t0 > kDecayWaitNs) return false;
+  }
+}
+
+template <int D, bool STATES> struct Shape {
+  static constexpr int kThreads = D == 64 ? 128 : 256;  // D = 128: two warps per TMEM lane quarter share its columns
+  static constexpr int kHalves = kThreads / 128;
+  static constexpr int kTile = kChunk * D * 2;     // bytes of one tile of q, k or v
+  static constexpr int kTiles = STATES ? 2 : 3;    // (q,) k, v
+  static constexpr int kKeys = kTiles * kTile;     // three parts of the decayed keys
+  static constexpr int kScores = kKeys + 3 * kTile;              // two parts of P, 8 KB each
+  static constexpr int kState = kScores + (STATES ? 0 : 16384);  // D = 64: two parts of X^T, 8 KB each
+  static constexpr int kMisc = kState + (STATES || D == 128 ? 0 : 16384);
+  static constexpr int kSmem = kMisc + 512;
+  // TMEM columns: U [0, D) (D = 128: also both parts of X^T), O1 [D, D + 64), O2 [D + 64, D + 128)
+  static constexpr uint32_t kCols = STATES ? D : 256;
 };
 
 template <int D, bool STATES>
-__global__ void __launch_bounds__(Shape<D>::kThreads, D == 64 ? (STATES ? 4 : 3) : (STATES ? 2 : 1))
+__global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
     k_decay_chunk(const __grid_constant__ DecayArgs a) {
-  using S = Shape<D>;
-  extern __shared__ __align__(128) unsigned char smem[];
+  using S = Shape<D, STATES>;
+  extern __shared__ __align__(1024) unsigned char smem[];
   const DecayRole& R = a.role[blockIdx.z];
   const int bh = blockIdx.x, seg = blockIdx.y;
   const int b = bh / a.H, h = bh % a.H;
@@ -93,24 +144,34 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, D == 64 ? (STATES ? 4 : 3)
   const int live = max(0, min(len, t_end) - t_begin);   // tokens of this segment that exist
   const int nchunks = (live + kChunk - 1) / kChunk;
 
-  constexpr int kTiles = STATES ? 2 : 3;
-  unsigned char* tiles = smem;                                   // [2][kTiles][kTile]
-  unsigned char* sx = smem + 2 * kTiles * S::kTile;              // [2 parts][D][D] bf16 (not for STATES)
-  float* pw = reinterpret_cast<float*>(smem + 2 * kTiles * S::kTile + (STATES ? 0 : 2 * S::kState));  // lam^0 .. lam^64
-  const uint32_t tiles_u = smem_addr(tiles), sx_u = smem_addr(sx);
+  float* pw = reinterpret_cast<float*>(smem + S::kMisc);        // lam^0 .. lam^64
+  uint64_t* done = reinterpret_cast<uint64_t*>(smem + S::kMisc + 320);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kMisc + 328);
+  const uint32_t base = smem_u32(smem);
 
+  if (tid == 0) {
+    mbar_init(done, 1);
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, S::kCols);
+    tmem_relinquish();
+  }
   const double g = (double)a.log_decay[h];
   for (int i = tid; i <= kChunk; i += S::kThreads) pw[i] = i ? (float)exp(g * i) : 1.f;
   // What the rounding of lam^64 leaves out: over hundreds of chunks that error would add up.
   const float full_rest = (float)(exp(g * kChunk) - (double)(float)exp(g * kChunk));
+  if constexpr (!STATES) {  // the blocks of P above the diagonal stay zero
+    for (int e = tid; e < 1024; e += S::kThreads)
+      reinterpret_cast<uint4*>(smem + S::kScores)[e] = make_uint4(0, 0, 0, 0);
+  }
 
   // Token index i sits at row i, or at len - 1 - i when the direction is reversed.
   auto prefetch = [&](int c) {
     const int i0 = t_begin + c * kChunk;
-    const uint32_t dst = tiles_u + (c & 1) * kTiles * S::kTile;
     constexpr int kGroups = D / 8;
 #pragma unroll
-    for (int w = 0; w < kTiles; ++w) {
+    for (int w = 0; w < S::kTiles; ++w) {
       const int which = STATES ? w + 1 : w;
       const __nv_bfloat16* p = which == 0 ? R.q + b * R.qb + h * R.qh
                                : which == 1 ? R.k + b * R.kb + h * R.kh : R.v + b * R.vb + h * R.vh;
@@ -121,106 +182,96 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, D == 64 ? (STATES ? 4 : 3)
         const int i = i0 + r;
         const bool ok = i < len;
         const long long t = ok ? (R.reverse ? len - 1 - i : i) : 0;
-        cp_async16(dst + w * S::kTile + tile_at<D>(r, gq), p + t * st + gq * 8, ok);
+        cp_async16(base + w * S::kTile + tile_at(r, gq), p + t * st + gq * 8, ok);
       }
     }
     cp_commit();
   };
+  if (nchunks > 0) prefetch(0);
 
-  // ---- state: warp w holds rows [16 w, 16 w + 16), all D columns, as accumulator fragments
-  float X[D / 8][4];
-  const int xr = warp * 16 + (lane >> 2), xc = (lane & 3) * 2;
+  // ---- state: this thread's row dv of X^T, columns dk0 .. dk0 + 63. With M = 64 the
+  // rows of an accumulator sit on the first 16 lanes of each quarter.
+  const int quarter = warp & 3, half = warp >> 2;
+  const bool row_ok = D == 128 || lane < 16;
+  const int dv = D == 128 ? quarter * 32 + lane : quarter * 16 + (lane & 15);
+  const int dk0 = half * 64;
+  float X[64];
   const float* x0 = nullptr;
   bool x0_t = false;
   if constexpr (!STATES) {
     if (a.nseg > 1) {
       const bool own = R.segments_from < 0;
-      const float* base = own ? R.segments : a.role[R.segments_from].segments;
-      x0 = base + ((size_t)bh * a.nseg + seg) * D * D;
+      x0 = (own ? R.segments : a.role[R.segments_from].segments) + ((size_t)bh * a.nseg + seg) * D * D;
       x0_t = !own;
     } else if (R.init) {
       x0 = R.init + (size_t)bh * D * D;
       x0_t = R.init_transposed;
     }
   }
-  if (nchunks > 0) prefetch(0);
-  if (x0) {
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = xr + (e >> 1) * 8, c = n * 8 + xc + (e & 1);
-        X[n][e] = x0_t ? x0[c * D + r] : x0[r * D + c];
-      }
-  } else {
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n) X[n][0] = X[n][1] = X[n][2] = X[n][3] = 0.f;
-  }
+  for (int n = 0; n < 64; ++n) X[n] = !x0 ? 0.f : x0_t ? x0[dv * D + dk0 + n] : x0[(dk0 + n) * D + dv];
   bool have = x0 != nullptr;  // a state that is known to be zero is not multiplied
-
-  auto publish = [&]() {  // bf16 parts of the state for the next chunk's X^T q
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const uint32_t hi = bf2(X[n][2 * p], X[n][2 * p + 1]);
-        const uint32_t lo = bf2(X[n][2 * p] - bf_lo(hi), X[n][2 * p + 1] - bf_hi(hi));
-        const uint32_t at = tile_at<D>(xr + 8 * p, n) + xc * 2;
-        *reinterpret_cast<uint32_t*>(sx + at) = hi;
-        *reinterpret_cast<uint32_t*>(sx + S::kState + at) = lo;
-      }
-  };
-  if constexpr (!STATES) {
-    if (have) publish();
-  }
   const bool want_final = STATES || (R.final_state != nullptr && a.nseg == 1);
   const int shift = R.reverse ? 0 : 1;  // exponents: i + shift and n - shift - j
 
-  for (int c = 0; c < nchunks; ++c) {
-    cp_wait<0>();
-    __syncthreads();  // chunk c and the published state are visible; the other buffer is free
-    if (c + 1 < nchunks) prefetch(c + 1);
-    const int n_tok = min(kChunk, live - c * kChunk);
-    const uint32_t buf = tiles_u + (c & 1) * kTiles * S::kTile;
-    const uint32_t tq = buf, tk = buf + (STATES ? 0 : S::kTile), tv = tk + S::kTile;
-    const bool update = want_final || c + 1 < nchunks;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tmem_slot;
+  const uint32_t lanes = tbase + ((uint32_t)(quarter * 32) << 16);
+  bool ok = true;
 
-    [[maybe_unused]] float O[8][4];
-    [[maybe_unused]] const int rb = warp & 3, ch = warp >> 2;  // 16 query rows, 64 output columns
-    [[maybe_unused]] const bool rows = rb * 16 < n_tok;
+  for (int c = 0; c < nchunks; ++c) {
+    const int n_tok = min(kChunk, live - c * kChunk);
+    const uint32_t tq = base, tk = base + (STATES ? 0 : S::kTile), tv = tk + S::kTile;
+    const bool update = want_final || c + 1 < nchunks;
+    cp_wait<0>();
+    // tiles are visible; everyone has read U and left the wait together or not at all
+    if (!__syncthreads_and(ok)) {
+      ok = false;
+      break;
+    }
+
     if constexpr (!STATES) {
+      if (have) {  // X^T as an operand: two bf16 parts
 #pragma unroll
-      for (int n = 0; n < 8; ++n) O[n][0] = O[n][1] = O[n][2] = O[n][3] = 0.f;
-      if (rows) {
+        for (int n = 0; n < 64; n += 32) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float x = X[n + 2 * e], y = X[n + 2 * e + 1];
+            hi[e] = bf2(x, y);
+            lo[e] = bf2(x - bf_lo(hi[e]), y - bf_hi(hi[e]));
+          }
+          if constexpr (D == 128) {
+            tmem_st_x16(lanes + half * 32 + n / 2, hi);
+            tmem_st_x16(lanes + 64 + half * 32 + n / 2, lo);
+          } else if (row_ok) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              unsigned char* at = smem + S::kState + tile_at(dv, n / 8 + q);
+              *reinterpret_cast<uint4*>(at) = make_uint4(hi[4 * q], hi[4 * q + 1], hi[4 * q + 2], hi[4 * q + 3]);
+              *reinterpret_cast<uint4*>(at + 8192) = make_uint4(lo[4 * q], lo[4 * q + 1], lo[4 * q + 2], lo[4 * q + 3]);
+            }
+          }
+        }
+        if constexpr (D == 128) tmem_st_wait();
+      }
+      // ---- scores: 16 query rows per warp, key blocks of 16 up to the diagonal (D = 128: every second one)
+      const int rb = warp & 3;
+      if (rb * 16 < n_tok) {
         uint32_t qf[D / 16][4];
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) ldsm4(block_at<D>(tq, rb * 16, k * 16, lane), qf[k]);
-        const int i_lo = rb * 16 + (lane >> 2);
-        if (have) {
-#pragma unroll
-          for (int part = 0; part < 2; ++part)
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-              for (int n = 0; n < 4; ++n) {
-                uint32_t f[4];
-                ldsm4t(block_at<D>(sx_u + part * S::kState, k * 16, ch * 64 + n * 16, lane), f);
-                mma16816(O[2 * n], qf[k], f[0], f[1]);
-                mma16816(O[2 * n + 1], qf[k], f[2], f[3]);
-              }
-          const float f0 = R.inter * pw[i_lo + shift], f1 = R.inter * pw[i_lo + 8 + shift];
-#pragma unroll
-          for (int n = 0; n < 8; ++n) O[n][0] *= f0, O[n][1] *= f0, O[n][2] *= f1, O[n][3] *= f1;
-        }
+        for (int k = 0; k < D / 16; ++k) ldsm4(block_at(tq, rb * 16, k * 16, lane), qf[k]);
+        const int i_lo = rb * 16 + (lane >> 2), jc = (lane & 3) * 2;
         // lam^15-jj of this thread's four key columns inside a block of 16
-        const int jc = (lane & 3) * 2;
         const float cf[4] = {pw[15 - jc], pw[14 - jc], pw[7 - jc], pw[6 - jc]};
-        for (int kb = 0; kb <= rb; ++kb) {
+        for (int kb = half; kb <= rb; kb += S::kHalves) {
           float P[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             uint32_t f[4];
-            ldsm4(block_at<D>(tk, kb * 16, k * 16, lane), f);
+            ldsm4(block_at(tk, kb * 16, k * 16, lane), f);
             mma16816(P[0], qf[k], f[0], f[2]);
             mma16816(P[1], qf[k], f[1], f[3]);
           }
@@ -240,125 +291,148 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, D == 64 ? (STATES ? 4 : 3)
                 P[n][e] = gap >= 0 ? P[n][e] * (R.intra * pw[gap]) : 0.f;
               }
           }
-          uint32_t ph[4], pl[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {  // A fragment: (row, row + 8) x (8 columns, next 8)
-            const float u = P[e >> 1][(e & 1) * 2], v = P[e >> 1][(e & 1) * 2 + 1];
-            ph[e] = bf2(u, v);
-            pl[e] = bf2(u - bf_lo(ph[e]), v - bf_hi(ph[e]));
-          }
+          for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            uint32_t f[4];
-            ldsm4t(block_at<D>(tv, kb * 16, ch * 64 + n * 16, lane), f);
-            mma16816(O[2 * n], ph, f[0], f[1]);
-            mma16816(O[2 * n + 1], ph, f[2], f[3]);
-            mma16816(O[2 * n], pl, f[0], f[1]);
-            mma16816(O[2 * n + 1], pl, f[2], f[3]);
-          }
+            for (int p = 0; p < 2; ++p) {
+              const float u = P[n][2 * p], v = P[n][2 * p + 1];
+              const uint32_t hi = bf2(u, v), lo = bf2(u - bf_lo(hi), v - bf_hi(hi));
+              unsigned char* at = smem + S::kScores + tile_at(i_lo + 8 * p, 2 * kb + n) + jc * 2;
+              *reinterpret_cast<uint32_t*>(at) = hi;
+              *reinterpret_cast<uint32_t*>(at + 8192) = lo;
+            }
         }
       }
     }
-
-    if (update) {
-      // A = k^T: rows are state rows, columns tokens (transposed 16 x 16 blocks of the key tile), decayed to the
-      // chunk's end and split into three parts
-      const float keep = pw[n_tok], rest = n_tok == kChunk ? full_rest : 0.f;
-      uint32_t kh[4][4], km[4][4], kl[4][4];
+    if (update) {  // ---- keys decayed to the chunk's end, in bf16 parts
+      constexpr int kGroups = D / 8;
 #pragma unroll
-      for (int tb = 0; tb < 4; ++tb) {
-        uint32_t kf[4];
-        ldsm4t(tk + tile_at<D>(tb * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * warp + ((lane >> 3) & 1)), kf);
-        const int j = tb * 16 + (lane & 3) * 2;
-        float w[4];
+      for (int u = 0; u < kChunk * kGroups / S::kThreads; ++u) {
+        const int e = tid + u * S::kThreads, r = e / kGroups, gq = e % kGroups;
+        const uint32_t at = tile_at(r, gq);
+        const uint4 raw = *reinterpret_cast<const uint4*>(smem + (tk - base) + at);
+        const uint32_t kw[4] = {raw.x, raw.y, raw.z, raw.w};
+        const float w = R.kv * pw[max(n_tok - shift - r, 0)];  // rows behind the last token are zero
+        uint32_t p0[4], p1[4], p2[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int p = n_tok - shift - (j + (e & 1) + (e >> 1) * 8);  // rows behind the last token are zero
-          w[e] = R.kv * pw[max(p, 0)];
+        for (int q = 0; q < 4; ++q) {
+          const float x = bf_lo(kw[q]) * w, y = bf_hi(kw[q]) * w;
+          p0[q] = bf2(x, y);
+          const float x1 = x - bf_lo(p0[q]), y1 = y - bf_hi(p0[q]);
+          p1[q] = bf2(x1, y1);
+          p2[q] = bf2(x1 - bf_lo(p1[q]), y1 - bf_hi(p1[q]));
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float u = bf_lo(kf[e]) * w[(e >> 1) * 2], v = bf_hi(kf[e]) * w[(e >> 1) * 2 + 1];
-          kh[tb][e] = bf2(u, v);
-          const float u1 = u - bf_lo(kh[tb][e]), v1 = v - bf_hi(kh[tb][e]);
-          km[tb][e] = bf2(u1, v1);
-          kl[tb][e] = bf2(u1 - bf_lo(km[tb][e]), v1 - bf_hi(km[tb][e]));
-        }
+        unsigned char* dst = smem + S::kKeys + at;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
+        *reinterpret_cast<uint4*>(dst + S::kTile) = make_uint4(p1[0], p1[1], p1[2], p1[3]);
+        *reinterpret_cast<uint4*>(dst + 2 * S::kTile) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
       }
-      // The chunk's own sum is formed apart and added once: the tensor cores cut off what does not fit their
-      // accumulator, which on a state that grows over thousands of tokens would add up.
+    }
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0) {
+      tc_fence_after();
+      // K steps of 16: 32 bytes along a K-major row (descriptor + 2; the next box of 64 is + 512), 16 rows of an
+      // MN-major box (+ 128), 8 columns of a TMEM operand.
+      if constexpr (!STATES) {
+        constexpr uint32_t id2 = umma_idesc_bf16_f32(D, 64), id1 = umma_idesc_bf16_f32(D, 64, true, false);
+        if (have) {
+          const uint64_t bq = umma_desc_sw128_kmajor(tq);
 #pragma unroll
-      for (int n = 0; n < D / 16; ++n) {
-        float U[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        uint32_t f[4][4];
+          for (int p = 1; p >= 0; --p)
 #pragma unroll
-        for (int tb = 0; tb < 4; ++tb) ldsm4t(block_at<D>(tv, tb * 16, n * 16, lane), f[tb]);
-#pragma unroll
-        for (int tb = 0; tb < 4; ++tb) {
-          mma16816(U[0], kl[tb], f[tb][0], f[tb][1]);
-          mma16816(U[1], kl[tb], f[tb][2], f[tb][3]);
+            for (int k = 0; k < D / 16; ++k) {
+              const uint64_t bk = bq + (k >> 2) * 512 + (k & 3) * 2;
+              const uint32_t acc = p == 0 || k > 0;
+              if constexpr (D == 128)
+                umma_ts(tbase + D + 64, tbase + p * 64 + k * 8, bk, id2, acc);
+              else
+                umma_f16(tbase + D + 64, umma_desc_sw128_kmajor(base + S::kState + p * 8192) + k * 2, bk, id2, acc);
+            }
         }
+        const uint64_t av = desc_mn(tv), bp = umma_desc_sw128_kmajor(base + S::kScores);
 #pragma unroll
-        for (int tb = 0; tb < 4; ++tb) {
-          mma16816(U[0], km[tb], f[tb][0], f[tb][1]);
-          mma16816(U[1], km[tb], f[tb][2], f[tb][3]);
-        }
+        for (int p = 1; p >= 0; --p)
 #pragma unroll
-        for (int tb = 0; tb < 4; ++tb) {
-          mma16816(U[0], kh[tb], f[tb][0], f[tb][1]);
-          mma16816(U[1], kh[tb], f[tb][2], f[tb][3]);
-        }
+          for (int k = 0; k < 4; ++k) umma_f16(tbase + D, av + 128 * k, bp + p * 512 + k * 2, id1, p == 0 || k > 0);
+      }
+      if (update) {  // behind the products that read X^T, whose columns U takes
+        constexpr uint32_t idu = umma_idesc_bf16_f32(D, D, true, true);
+        const uint64_t av = desc_mn(tv), bk = desc_mn(base + S::kKeys);
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int p = 2; p >= 0; --p)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            X[2 * n + m][e] = fmaf(X[2 * n + m][e], keep, fmaf(X[2 * n + m][e], rest, U[m][e]));
+          for (int k = 0; k < 4; ++k)
+            umma_f16(tbase, av + 128 * k, bk + p * (S::kTile >> 4) + 128 * k, idu, p < 2 || k > 0);
+      }
+      umma_commit(done);
+    }
+    __syncwarp();
+    if (!wait_phase(done, c & 1)) {
+      ok = false;
+      if (lane == 0) atomicExch(&g_decay_error, 1u);
+    }
+    tc_fence_after();
+    if (c + 1 < nchunks && ok) prefetch(c + 1);
+    if (update) {
+      const float keep = pw[n_tok], rest = n_tok == kChunk ? full_rest : 0.f;
+#pragma unroll
+      for (int n = 0; n < 64; n += 32) {
+        uint32_t u[32];
+        tmem_ld_32x32b_x32(lanes + dk0 + n, u);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) X[n + e] = fmaf(X[n + e], keep, fmaf(X[n + e], rest, __uint_as_float(u[e])));
       }
     }
     if constexpr (!STATES) {
-      __syncthreads();  // everyone has read the state's parts and the query tile
-      if (update && c + 1 < nchunks) publish();
-      have = true;
-      if (rows) {  // through the query tile, so that whole 16-byte groups are stored
-        unsigned char* o_tile = tiles + (c & 1) * kTiles * S::kTile;
-        const int r = rb * 16 + (lane >> 2);
+      // ---- o: a row of the value dimension per thread, 64 tokens (D = 128: 32 per half)
+      __nv_bfloat16* out = R.out + b * R.ob + h * R.oh + dv;
+      const int i0 = t_begin + c * kChunk;
+      constexpr int kTok = 64 / S::kHalves;
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          *reinterpret_cast<uint32_t*>(o_tile + tile_at<D>(r, ch * 8 + n) + xc * 2) = bf2(O[n][0], O[n][1]);
-          *reinterpret_cast<uint32_t*>(o_tile + tile_at<D>(r + 8, ch * 8 + n) + xc * 2) = bf2(O[n][2], O[n][3]);
-        }
-        __syncwarp();
-        __nv_bfloat16* out = R.out + b * R.ob + h * R.oh;
+      for (int n = 0; n < kTok; n += 16) {
+        const int t0 = half * kTok + n;
+        uint32_t o1[16], o2[16];
+        tmem_ld_32x32b_x16(lanes + D + t0, o1);
+        if (have) tmem_ld_32x32b_x16(lanes + D + 64 + t0, o2);
+        tmem_ld_wait();
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int rr = rb * 16 + u * 4 + (lane >> 3), gq = ch * 8 + (lane & 7);
-          if (rr < n_tok) {
-            const int i = t_begin + c * kChunk + rr;
-            const long long t = R.reverse ? len - 1 - i : i;
-            *reinterpret_cast<uint4*>(out + t * R.ot + gq * 8) =
-                *reinterpret_cast<const uint4*>(o_tile + tile_at<D>(rr, gq));
+        for (int e = 0; e < 16; ++e) {
+          const int i = t0 + e;
+          float o = __uint_as_float(o1[e]);
+          if (have) o = fmaf(R.inter * pw[i + shift], __uint_as_float(o2[e]), o);
+          if (row_ok && i < n_tok) {
+            const long long t = R.reverse ? len - 1 - (i0 + i) : i0 + i;
+            out[t * R.ot] = __float2bfloat16_rn(o);
           }
         }
       }
+      have = true;
     }
+    tc_fence_before();
   }
 
   if constexpr (!STATES) {
     // rows of the batch that hold no token (index >= length) give zeros
     __nv_bfloat16* out = R.out + b * R.ob + h * R.oh;
     constexpr int kGroups = D / 8;
-    for (int e = tid; e < (t_end - max(t_begin, min(len, t_end))) * kGroups; e += S::kThreads) {
-      const int i = max(t_begin, min(len, t_end)) + e / kGroups;
-      *reinterpret_cast<uint4*>(out + (long long)i * R.ot + (e % kGroups) * 8) = make_uint4(0, 0, 0, 0);
-    }
+    const int from = max(t_begin, min(len, t_end));
+    for (int e = tid; e < (t_end - from) * kGroups; e += S::kThreads)
+      *reinterpret_cast<uint4*>(out + (long long)(from + e / kGroups) * R.ot + (e % kGroups) * 8) = make_uint4(0, 0, 0, 0);
   }
-  if (want_final) {
+  if (want_final && row_ok) {
     float* dst = STATES ? R.segments + ((size_t)bh * a.nseg + seg) * D * D : R.final_state + (size_t)bh * D * D;
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-        *reinterpret_cast<float2*>(dst + (size_t)(xr + 8 * p) * D + n * 8 + xc) = make_float2(X[n][2 * p], X[n][2 * p + 1]);
+    for (int n = 0; n < 64; ++n) dst[(size_t)(dk0 + n) * D + dv] = X[n];
+  }
+  cp_wait<0>();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tbase, S::kCols);
   }
 }
 
@@ -447,38 +521,44 @@ template <int D> __global__ void __launch_bounds__(D * 2) k_decay_step(const Dec
   }
 }
 
-template <typename K> cudaError_t allow_smem(K kernel, int bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+template <int D, bool STATES>
+cudaError_t launch_chunks(const DecayArgs& a, int roles, cudaStream_t s) {
+  using S = Shape<D, STATES>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(k_decay_chunk<D, STATES>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (e != cudaSuccess) return e;
+  k_decay_chunk<D, STATES><<<dim3(a.B * a.H, a.nseg, roles), S::kThreads, S::kSmem, s>>>(a);
+  return cudaGetLastError();
 }
 
 template <int D> cudaError_t decay_typed(const DecayArgs& a, cudaStream_t s, int* launches) {
-  using S = Shape<D>;
   *launches = 0;
   if (a.nseg > 1) {
-    cudaError_t e = allow_smem(k_decay_chunk<D, true>, S::kSmemStates);
-    if (e != cudaSuccess) return e;
     // roles that read another role's segment states come last and need no states of their own
     int own = 0;
     while (own < a.nroles && a.role[own].segments_from < 0) ++own;
-    k_decay_chunk<D, true><<<dim3(a.B * a.H, a.nseg, own), S::kThreads, S::kSmemStates, s>>>(a);
+    const cudaError_t e = launch_chunks<D, true>(a, own, s);
+    if (e != cudaSuccess) return e;
     k_decay_scan<D><<<dim3(a.B * a.H, D * D / 1024, own), 256, 0, s>>>(a);
     *launches += 2;
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
-  cudaError_t e = allow_smem(k_decay_chunk<D, false>, S::kSmem);
-  if (e != cudaSuccess) return e;
-  k_decay_chunk<D, false><<<dim3(a.B * a.H, a.nseg, a.nroles), S::kThreads, S::kSmem, s>>>(a);
   *launches += 1;
-  return cudaGetLastError();
+  return launch_chunks<D, false>(a, a.nroles, s);
 }
 }  // namespace
 
+unsigned int decay_error_flag() {
+  unsigned int v = 0;
+  cudaMemcpyFromSymbol(&v, g_decay_error, sizeof(v));
+  return v;
+}
+
 int decay_segments(int B, int T, int H, int D, int roles) {
-  // Blocks resident at once: 3 per SM for D = 64, 1 for D = 128.
+  // Two blocks per SM are resident; without a split at least half of them should have work.
   const int chunks = (T + kChunk - 1) / kChunk;
-  const long long blocks = (long long)B * H * roles, want = 148LL * (D == 64 ? 3 : 1);
+  const long long blocks = (long long)B * H * roles, want = 148LL * 2;
   if (blocks * 2 > want || chunks < 4) return 1;
-  long long n = (want + blocks - 1) / blocks;
+  long long n = want / blocks;
   if (n > chunks / 2) n = chunks / 2;
   return (int)n;
 }

@@ -79,6 +79,7 @@ struct DecayArgs {
 };
 int decay_segments(int B, int T, int H, int D, int roles);  // number of token segments worked on side by side
 cudaError_t decay_attention(const DecayArgs& a, cudaStream_t s, int* launches);
+unsigned int decay_error_flag();  // current GPU: not 0 once a wait inside decay_attention has given up (synchronises)
 // One token: state = lam state + k v^T in place, o = scale * state^T q. q, k, v rows with strides, o contiguous.
 struct DecayStepArgs {
   const __nv_bfloat16 *q, *k, *v;

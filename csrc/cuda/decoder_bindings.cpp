@@ -635,6 +635,7 @@ void register_decoder_ops(py::module& m) {
   m.def("dropout_ln_bwd", &op_dropout_ln_bwd);
   m.def("decay_attention", &decay);
   m.def("decay_step", &op_decay_step);
+  m.def("decay_error_flag", &decay_error_flag);
 }
 
 }  // namespace nexar
