@@ -21,13 +21,14 @@
 //
 // Per chunk the scores (an eighth of the products) are formed with warp-level
 // MMAs, whose registers hold them where the decay and the mask are applied; they
-// go to shared memory as the operand P. Everything else runs on tcgen05, with the
-// value dimension along the 128 (D = 64: 64) TMEM lanes so that the state keeps
-// one layout from product to operand:
-//     O2 [dv, token] = X^T Q^T,   O1 [dv, token] = V^T P^T,   U [dv, dk] = V^T K'
-// (K': the chunk's keys decayed to its end). X lives in fp32 registers (a row of
-// X^T per thread) and goes back as an operand through TMEM (D = 128, over the
-// columns of U, which is done by then) or shared memory (D = 64).
+// go to shared memory as the operand P. Everything else runs on tcgen05 (K': the
+// chunk's keys decayed to its end):
+//     D = 64:   O2 [token, dv] = Q X,     O1 [token, dv] = P V,     U [dk, dv] = K'^T V
+//     D = 128:  O2 [dv, token] = X^T Q^T, O1 [dv, token] = V^T P^T, U [dv, dk] = V^T K'
+// With D = 64 the 64 rows of every accumulator are read as matrix fragments (16
+// lanes per warp), and X goes back as an operand through shared memory. With D =
+// 128 the value dimension fills the 128 lanes, X^T stays with its rows' threads
+// and goes back through TMEM, over the columns of U, which is done by then.
 // Two blocks per SM: one block's products run while the other prepares.
 //
 // Roundings. Products are bf16 tensor-core products with fp32 sums. The decayed
@@ -101,6 +102,18 @@ NEXAR_D void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// 16 lanes x 64 columns as matrix fragments: r[4 n + e] is row lane / 4 + 8 (e / 2), column 8 n + 2 (lane % 4) + e % 2.
+NEXAR_D void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
 NEXAR_D void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Bounded wait by polling: these waits sit on the chunk's critical path.
@@ -120,12 +133,13 @@ template <int D, bool STATES> struct Shape {
   static constexpr int kHalves = kThreads / 128;
   static constexpr int kTile = kChunk * D * 2;     // bytes of one tile of q, k or v
   static constexpr int kTiles = STATES ? 2 : 3;    // (q,) k, v
-  static constexpr int kKeys = kTiles * kTile;     // three parts of the decayed keys
+  static constexpr int kStages = D == 64 ? 2 : 1;  // chunks of tiles: two blocks of D = 128 leave no room for a second
+  static constexpr int kKeys = kStages * kTiles * kTile;         // three parts of the decayed keys; then the output
   static constexpr int kScores = kKeys + 3 * kTile;              // two parts of P, 8 KB each
-  static constexpr int kState = kScores + (STATES ? 0 : 16384);  // D = 64: two parts of X^T, 8 KB each
+  static constexpr int kState = kScores + (STATES ? 0 : 16384);  // D = 64: two parts of X, 8 KB each
   static constexpr int kMisc = kState + (STATES || D == 128 ? 0 : 16384);
   static constexpr int kSmem = kMisc + 512;
-  // TMEM columns: U [0, D) (D = 128: also both parts of X^T), O1 [D, D + 64), O2 [D + 64, D + 128)
+  // TMEM columns: U [0, D) (D = 128: also both parts of X^T), O1 and O2 of 64 columns behind it
   static constexpr uint32_t kCols = STATES ? D : 256;
 };
 
@@ -166,36 +180,53 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
       reinterpret_cast<uint4*>(smem + S::kScores)[e] = make_uint4(0, 0, 0, 0);
   }
 
-  // Token index i sits at row i, or at len - 1 - i when the direction is reversed.
-  auto prefetch = [&](int c) {
-    const int i0 = t_begin + c * kChunk;
-    constexpr int kGroups = D / 8;
+  // A thread moves 16-byte group g0 of rows r0, r0 + 16, ... of every tile. Token index i sits at row i, or at
+  // len - 1 - i when the direction is reversed.
+  constexpr int kGroups = D / 8;
+  const int r0 = tid / kGroups, g0 = tid % kGroups;
+  const uint32_t at0 = tile_at(r0, g0);  // + 2048 bytes for 16 rows more
+  const long long dir = R.reverse ? -1 : 1, first = (R.reverse ? len - 1 - t_begin : t_begin) + dir * r0;
+  const __nv_bfloat16* src[S::kTiles];
+  long long step[S::kTiles];  // 16 rows
+  {
+    const __nv_bfloat16* p[3] = {R.q + b * R.qb + h * R.qh, R.k + b * R.kb + h * R.kh, R.v + b * R.vb + h * R.vh};
+    const long long st[3] = {R.qt, R.kt, R.vt};
 #pragma unroll
     for (int w = 0; w < S::kTiles; ++w) {
       const int which = STATES ? w + 1 : w;
-      const __nv_bfloat16* p = which == 0 ? R.q + b * R.qb + h * R.qh
-                               : which == 1 ? R.k + b * R.kb + h * R.kh : R.v + b * R.vb + h * R.vh;
-      const long long st = which == 0 ? R.qt : which == 1 ? R.kt : R.vt;
+      src[w] = p[which] + first * st[which] + g0 * 8;
+      step[w] = dir * st[which] * 16;
+    }
+  }
+  auto prefetch = [&](int c) {  // chunks in order: moves the pointers on
+    const int left = live - c * kChunk - r0;
+    const uint32_t dst = base + (S::kStages == 2 ? (c & 1) * S::kTiles * S::kTile : 0) + at0;
 #pragma unroll
-      for (int u = 0; u < kChunk * kGroups / S::kThreads; ++u) {
-        const int e = tid + u * S::kThreads, r = e / kGroups, gq = e % kGroups;
-        const int i = i0 + r;
-        const bool ok = i < len;
-        const long long t = ok ? (R.reverse ? len - 1 - i : i) : 0;
-        cp_async16(base + w * S::kTile + tile_at(r, gq), p + t * st + gq * 8, ok);
+    for (int w = 0; w < S::kTiles; ++w) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bool ok = 16 * u < left;
+        cp_async16(dst + w * S::kTile + u * 2048, ok ? src[w] : R.k, ok);
+        src[w] += step[w];
       }
     }
     cp_commit();
   };
   if (nchunks > 0) prefetch(0);
 
-  // ---- state: this thread's row dv of X^T, columns dk0 .. dk0 + 63. With M = 64 the
-  // rows of an accumulator sit on the first 16 lanes of each quarter.
+  // ---- state. D = 64: fragments of X, rows dk = xr (+ 8), columns dv = 8 n + xc (+ 1). D = 128: row dv of X^T,
+  // columns dk0 .. dk0 + 63.
   const int quarter = warp & 3, half = warp >> 2;
-  const bool row_ok = D == 128 || lane < 16;
-  const int dv = D == 128 ? quarter * 32 + lane : quarter * 16 + (lane & 15);
-  const int dk0 = half * 64;
-  float X[64];
+  const int xr = warp * 16 + (lane >> 2), xc = (lane & 3) * 2;
+  const int dv = quarter * 32 + lane, dk0 = half * 64;
+  constexpr int kX = D == 64 ? 32 : 64;
+  float X[kX];
+  auto x_at = [&](int n) {  // element of [dk, dv] that X[n] holds
+    return D == 64 ? (xr + ((n >> 1) & 1) * 8) * D + (n >> 2) * 8 + xc + (n & 1) : (dk0 + n) * D + dv;
+  };
+  auto x_at_t = [&](int n) {  // the same element of the transposed state
+    return D == 64 ? ((n >> 2) * 8 + xc + (n & 1)) * D + xr + ((n >> 1) & 1) * 8 : dv * D + dk0 + n;
+  };
   const float* x0 = nullptr;
   bool x0_t = false;
   if constexpr (!STATES) {
@@ -209,7 +240,7 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
     }
   }
 #pragma unroll
-  for (int n = 0; n < 64; ++n) X[n] = !x0 ? 0.f : x0_t ? x0[dv * D + dk0 + n] : x0[(dk0 + n) * D + dv];
+  for (int n = 0; n < kX; ++n) X[n] = !x0 ? 0.f : x0[x0_t ? x_at_t(n) : x_at(n)];
   bool have = x0 != nullptr;  // a state that is known to be zero is not multiplied
   const bool want_final = STATES || (R.final_state != nullptr && a.nseg == 1);
   const int shift = R.reverse ? 0 : 1;  // exponents: i + shift and n - shift - j
@@ -219,43 +250,52 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
   tc_fence_after();
   const uint32_t tbase = *tmem_slot;
   const uint32_t lanes = tbase + ((uint32_t)(quarter * 32) << 16);
+  __nv_bfloat16* out = nullptr;  // this thread's group of the output, advanced like src
+  if constexpr (!STATES)
+    out = R.out + b * R.ob + h * R.oh + (D == 64 ? (first - dir * r0 + dir * (warp * 16 + (lane >> 3))) * R.ot + (lane & 7) * 8
+                                                 : first * R.ot + g0 * 8);
   bool ok = true;
 
   for (int c = 0; c < nchunks; ++c) {
     const int n_tok = min(kChunk, live - c * kChunk);
-    const uint32_t tq = base, tk = base + (STATES ? 0 : S::kTile), tv = tk + S::kTile;
+    const uint32_t stage = S::kStages == 2 ? (c & 1) * S::kTiles * S::kTile : 0;
+    const uint32_t tq = base + stage, tk = tq + (STATES ? 0 : S::kTile), tv = tk + S::kTile;
     const bool update = want_final || c + 1 < nchunks;
     cp_wait<0>();
-    // tiles are visible; everyone has read U and left the wait together or not at all
+    // tiles are visible; everyone has read U and the output, and all leave together if a wait gave up
     if (!__syncthreads_and(ok)) {
       ok = false;
       break;
     }
+    if constexpr (S::kStages == 2) {
+      if (c + 1 < nchunks) prefetch(c + 1);
+    }
 
     if constexpr (!STATES) {
-      if (have) {  // X^T as an operand: two bf16 parts
+      if (have) {  // the state as an operand: two bf16 parts
+        if constexpr (D == 64) {
 #pragma unroll
-        for (int n = 0; n < 64; n += 32) {
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float x = X[n + 2 * e], y = X[n + 2 * e + 1];
-            hi[e] = bf2(x, y);
-            lo[e] = bf2(x - bf_lo(hi[e]), y - bf_hi(hi[e]));
+          for (int n = 0; n < kX; n += 2) {
+            const uint32_t hi = bf2(X[n], X[n + 1]), lo = bf2(X[n] - bf_lo(hi), X[n + 1] - bf_hi(hi));
+            unsigned char* at = smem + S::kState + tile_at(xr + ((n >> 1) & 1) * 8, n >> 2) + xc * 2;
+            *reinterpret_cast<uint32_t*>(at) = hi;
+            *reinterpret_cast<uint32_t*>(at + 8192) = lo;
           }
-          if constexpr (D == 128) {
+        } else {
+#pragma unroll
+          for (int n = 0; n < kX; n += 32) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float x = X[n + 2 * e], y = X[n + 2 * e + 1];
+              hi[e] = bf2(x, y);
+              lo[e] = bf2(x - bf_lo(hi[e]), y - bf_hi(hi[e]));
+            }
             tmem_st_x16(lanes + half * 32 + n / 2, hi);
             tmem_st_x16(lanes + 64 + half * 32 + n / 2, lo);
-          } else if (row_ok) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              unsigned char* at = smem + S::kState + tile_at(dv, n / 8 + q);
-              *reinterpret_cast<uint4*>(at) = make_uint4(hi[4 * q], hi[4 * q + 1], hi[4 * q + 2], hi[4 * q + 3]);
-              *reinterpret_cast<uint4*>(at + 8192) = make_uint4(lo[4 * q], lo[4 * q + 1], lo[4 * q + 2], lo[4 * q + 3]);
-            }
           }
+          tmem_st_wait();
         }
-        if constexpr (D == 128) tmem_st_wait();
       }
       // ---- scores: 16 query rows per warp, key blocks of 16 up to the diagonal (D = 128: every second one)
       const int rb = warp & 3;
@@ -263,9 +303,9 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
         uint32_t qf[D / 16][4];
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) ldsm4(block_at(tq, rb * 16, k * 16, lane), qf[k]);
-        const int i_lo = rb * 16 + (lane >> 2), jc = (lane & 3) * 2;
+        const int i_lo = rb * 16 + (lane >> 2);
         // lam^15-jj of this thread's four key columns inside a block of 16
-        const float cf[4] = {pw[15 - jc], pw[14 - jc], pw[7 - jc], pw[6 - jc]};
+        const float cf[4] = {pw[15 - xc], pw[14 - xc], pw[7 - xc], pw[6 - xc]};
         for (int kb = half; kb <= rb; kb += S::kHalves) {
           float P[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -276,18 +316,18 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
             mma16816(P[1], qf[k], f[1], f[3]);
           }
           if (kb < rb) {
-            const float r0 = R.intra * pw[i_lo - kb * 16 - 15], r1 = R.intra * pw[i_lo + 8 - kb * 16 - 15];
+            const float f0 = R.intra * pw[i_lo - kb * 16 - 15], f1 = R.intra * pw[i_lo + 8 - kb * 16 - 15];
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-              P[n][0] *= r0 * cf[2 * n], P[n][1] *= r0 * cf[2 * n + 1];
-              P[n][2] *= r1 * cf[2 * n], P[n][3] *= r1 * cf[2 * n + 1];
+              P[n][0] *= f0 * cf[2 * n], P[n][1] *= f0 * cf[2 * n + 1];
+              P[n][2] *= f1 * cf[2 * n], P[n][3] *= f1 * cf[2 * n + 1];
             }
           } else {
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const int gap = (lane >> 2) + (e >> 1) * 8 - (n * 8 + jc + (e & 1));
+                const int gap = (lane >> 2) + (e >> 1) * 8 - (n * 8 + xc + (e & 1));
                 P[n][e] = gap >= 0 ? P[n][e] * (R.intra * pw[gap]) : 0.f;
               }
           }
@@ -297,7 +337,7 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
             for (int p = 0; p < 2; ++p) {
               const float u = P[n][2 * p], v = P[n][2 * p + 1];
               const uint32_t hi = bf2(u, v), lo = bf2(u - bf_lo(hi), v - bf_hi(hi));
-              unsigned char* at = smem + S::kScores + tile_at(i_lo + 8 * p, 2 * kb + n) + jc * 2;
+              unsigned char* at = smem + S::kScores + tile_at(i_lo + 8 * p, 2 * kb + n) + xc * 2;
               *reinterpret_cast<uint32_t*>(at) = hi;
               *reinterpret_cast<uint32_t*>(at + 8192) = lo;
             }
@@ -305,14 +345,11 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
       }
     }
     if (update) {  // ---- keys decayed to the chunk's end, in bf16 parts
-      constexpr int kGroups = D / 8;
 #pragma unroll
-      for (int u = 0; u < kChunk * kGroups / S::kThreads; ++u) {
-        const int e = tid + u * S::kThreads, r = e / kGroups, gq = e % kGroups;
-        const uint32_t at = tile_at(r, gq);
-        const uint4 raw = *reinterpret_cast<const uint4*>(smem + (tk - base) + at);
+      for (int u = 0; u < 4; ++u) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(smem + (tk - base) + at0 + u * 2048);
         const uint32_t kw[4] = {raw.x, raw.y, raw.z, raw.w};
-        const float w = R.kv * pw[max(n_tok - shift - r, 0)];  // rows behind the last token are zero
+        const float w = R.kv * pw[max(n_tok - shift - r0 - 16 * u, 0)];  // rows behind the last token are zero
         uint32_t p0[4], p1[4], p2[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -322,7 +359,7 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
           p1[q] = bf2(x1, y1);
           p2[q] = bf2(x1 - bf_lo(p1[q]), y1 - bf_hi(p1[q]));
         }
-        unsigned char* dst = smem + S::kKeys + at;
+        unsigned char* dst = smem + S::kKeys + at0 + u * 2048;
         *reinterpret_cast<uint4*>(dst) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
         *reinterpret_cast<uint4*>(dst + S::kTile) = make_uint4(p1[0], p1[1], p1[2], p1[3]);
         *reinterpret_cast<uint4*>(dst + 2 * S::kTile) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
@@ -334,37 +371,45 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
     if (tid == 0) {
       tc_fence_after();
       // K steps of 16: 32 bytes along a K-major row (descriptor + 2; the next box of 64 is + 512), 16 rows of an
-      // MN-major box (+ 128), 8 columns of a TMEM operand.
+      // MN-major box (+ 128), 8 columns of a TMEM operand. Small parts first.
+      const uint64_t mv = desc_mn(tv);
       if constexpr (!STATES) {
-        constexpr uint32_t id2 = umma_idesc_bf16_f32(D, 64), id1 = umma_idesc_bf16_f32(D, 64, true, false);
+        constexpr uint32_t id2 = umma_idesc_bf16_f32(D, 64, false, D == 64);
+        constexpr uint32_t id1 = umma_idesc_bf16_f32(D, 64, D == 128, D == 64);
+        const uint64_t kq = umma_desc_sw128_kmajor(tq), kp = umma_desc_sw128_kmajor(base + S::kScores);
         if (have) {
-          const uint64_t bq = umma_desc_sw128_kmajor(tq);
+          [[maybe_unused]] const uint64_t mx = desc_mn(base + S::kState);
 #pragma unroll
           for (int p = 1; p >= 0; --p)
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-              const uint64_t bk = bq + (k >> 2) * 512 + (k & 3) * 2;
               const uint32_t acc = p == 0 || k > 0;
-              if constexpr (D == 128)
-                umma_ts(tbase + D + 64, tbase + p * 64 + k * 8, bk, id2, acc);
+              if constexpr (D == 64)
+                umma_f16(tbase + D + 64, kq + k * 2, mx + p * 512 + 128 * k, id2, acc);
               else
-                umma_f16(tbase + D + 64, umma_desc_sw128_kmajor(base + S::kState + p * 8192) + k * 2, bk, id2, acc);
+                umma_ts(tbase + D + 64, tbase + p * 64 + k * 8, kq + (k >> 2) * 512 + (k & 3) * 2, id2, acc);
             }
         }
-        const uint64_t av = desc_mn(tv), bp = umma_desc_sw128_kmajor(base + S::kScores);
 #pragma unroll
         for (int p = 1; p >= 0; --p)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f16(tbase + D, av + 128 * k, bp + p * 512 + k * 2, id1, p == 0 || k > 0);
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (D == 64)
+              umma_f16(tbase + D, kp + p * 512 + k * 2, mv + 128 * k, id1, p == 0 || k > 0);
+            else
+              umma_f16(tbase + D, mv + 128 * k, kp + p * 512 + k * 2, id1, p == 0 || k > 0);
+          }
       }
       if (update) {  // behind the products that read X^T, whose columns U takes
         constexpr uint32_t idu = umma_idesc_bf16_f32(D, D, true, true);
-        const uint64_t av = desc_mn(tv), bk = desc_mn(base + S::kKeys);
+        const uint64_t mk = desc_mn(base + S::kKeys);
 #pragma unroll
         for (int p = 2; p >= 0; --p)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16(tbase, av + 128 * k, bk + p * (S::kTile >> 4) + 128 * k, idu, p < 2 || k > 0);
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t part = mk + p * (S::kTile >> 4) + 128 * k;
+            umma_f16(tbase, D == 64 ? part : mv + 128 * k, D == 64 ? mv + 128 * k : part, idu, p < 2 || k > 0);
+          }
       }
       umma_commit(done);
     }
@@ -374,41 +419,71 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
       if (lane == 0) atomicExch(&g_decay_error, 1u);
     }
     tc_fence_after();
-    if (c + 1 < nchunks && ok) prefetch(c + 1);
+    if constexpr (S::kStages == 1) {
+      if (c + 1 < nchunks && ok) prefetch(c + 1);
+    }
     if (update) {
       const float keep = pw[n_tok], rest = n_tok == kChunk ? full_rest : 0.f;
 #pragma unroll
-      for (int n = 0; n < 64; n += 32) {
+      for (int n = 0; n < kX; n += 32) {
         uint32_t u[32];
-        tmem_ld_32x32b_x32(lanes + dk0 + n, u);
+        if constexpr (D == 64) tmem_ld_frag(lanes, u);
+        else tmem_ld_32x32b_x32(lanes + dk0 + n, u);
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 32; ++e) X[n + e] = fmaf(X[n + e], keep, fmaf(X[n + e], rest, __uint_as_float(u[e])));
       }
     }
     if constexpr (!STATES) {
-      // ---- o: a row of the value dimension per thread, 64 tokens (D = 128: 32 per half)
-      __nv_bfloat16* out = R.out + b * R.ob + h * R.oh + dv;
-      const int i0 = t_begin + c * kChunk;
-      constexpr int kTok = 64 / S::kHalves;
-#pragma unroll
-      for (int n = 0; n < kTok; n += 16) {
-        const int t0 = half * kTok + n;
-        uint32_t o1[16], o2[16];
-        tmem_ld_32x32b_x16(lanes + D + t0, o1);
-        if (have) tmem_ld_32x32b_x16(lanes + D + 64 + t0, o2);
+      // ---- o = O1 + inter lam^(i + shift) O2, through the keys' space so that whole 16-byte groups are stored
+      unsigned char* o_tile = smem + S::kKeys;
+      if constexpr (D == 64) {
+        const float f0 = R.inter * pw[xr + shift], f1 = R.inter * pw[xr + 8 + shift];  // xr: here a token
+        uint32_t o1[32], o2[32];
+        tmem_ld_frag(lanes + D, o1);
+        if (have) tmem_ld_frag(lanes + D + 64, o2);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int i = t0 + e;
-          float o = __uint_as_float(o1[e]);
-          if (have) o = fmaf(R.inter * pw[i + shift], __uint_as_float(o2[e]), o);
-          if (row_ok && i < n_tok) {
-            const long long t = R.reverse ? len - 1 - (i0 + i) : i0 + i;
-            out[t * R.ot] = __float2bfloat16_rn(o);
+        for (int n = 0; n < 32; n += 2) {
+          float x = __uint_as_float(o1[n]), y = __uint_as_float(o1[n + 1]);
+          if (have) {
+            const float f = n & 2 ? f1 : f0;
+            x = fmaf(f, __uint_as_float(o2[n]), x), y = fmaf(f, __uint_as_float(o2[n + 1]), y);
+          }
+          *reinterpret_cast<uint32_t*>(o_tile + tile_at(xr + (n & 2) * 4, n >> 2) + xc * 2) = bf2(x, y);
+        }
+        __syncwarp();  // a warp stores the rows that it wrote
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int r = warp * 16 + u * 4 + (lane >> 3);
+          if (r < n_tok)
+            *reinterpret_cast<uint4*>(out + u * 4 * dir * R.ot) =
+                *reinterpret_cast<const uint4*>(o_tile + tile_at(r, lane & 7));
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < 32; n += 16) {
+          const int t0 = half * 32 + n;
+          uint32_t o1[16], o2[16];
+          tmem_ld_32x32b_x16(lanes + D + t0, o1);
+          if (have) tmem_ld_32x32b_x16(lanes + D + 64 + t0, o2);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float o = __uint_as_float(o1[e]);
+            if (have) o = fmaf(R.inter * pw[t0 + e + shift], __uint_as_float(o2[e]), o);
+            reinterpret_cast<__nv_bfloat16*>(o_tile)[(t0 + e) * D + dv] = __float2bfloat16_rn(o);
           }
         }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (r0 + 16 * u < n_tok)
+            *reinterpret_cast<uint4*>(out + u * 16 * dir * R.ot) =
+                *reinterpret_cast<const uint4*>(o_tile + (r0 + 16 * u) * D * 2 + g0 * 16);
+        }
       }
+      out += kChunk * dir * R.ot;
       have = true;
     }
     tc_fence_before();
@@ -416,16 +491,15 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
 
   if constexpr (!STATES) {
     // rows of the batch that hold no token (index >= length) give zeros
-    __nv_bfloat16* out = R.out + b * R.ob + h * R.oh;
-    constexpr int kGroups = D / 8;
+    __nv_bfloat16* rows = R.out + b * R.ob + h * R.oh;
     const int from = max(t_begin, min(len, t_end));
     for (int e = tid; e < (t_end - from) * kGroups; e += S::kThreads)
-      *reinterpret_cast<uint4*>(out + (long long)(from + e / kGroups) * R.ot + (e % kGroups) * 8) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(rows + (long long)(from + e / kGroups) * R.ot + (e % kGroups) * 8) = make_uint4(0, 0, 0, 0);
   }
-  if (want_final && row_ok) {
+  if (want_final) {
     float* dst = STATES ? R.segments + ((size_t)bh * a.nseg + seg) * D * D : R.final_state + (size_t)bh * D * D;
 #pragma unroll
-    for (int n = 0; n < 64; ++n) dst[(size_t)(dk0 + n) * D + dv] = X[n];
+    for (int n = 0; n < kX; ++n) dst[x_at(n)] = X[n];
   }
   cp_wait<0>();
   tc_fence_before();
