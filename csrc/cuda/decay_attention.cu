@@ -19,16 +19,17 @@
 // k_decay_scan turns these into the state before each segment, and the main
 // kernel then runs all segments at once.
 //
-// Per chunk the scores (an eighth of the products) are formed with warp-level
-// MMAs, whose registers hold them where the decay and the mask are applied; they
-// go to shared memory as the operand P. Everything else runs on tcgen05 (K': the
-// chunk's keys decayed to its end):
+// All products run on tcgen05 (K': the chunk's keys decayed to its end; P: the
+// decayed and masked scores):
+//     both:     S [token, token] = Q K^T
 //     D = 64:   O2 [token, dv] = Q X,     O1 [token, dv] = P V,     U [dk, dv] = K'^T V
 //     D = 128:  O2 [dv, token] = X^T Q^T, O1 [dv, token] = V^T P^T, U [dv, dk] = V^T K'
-// With D = 64 the 64 rows of every accumulator are read as matrix fragments (16
-// lanes per warp), and X goes back as an operand through shared memory. With D =
-// 128 the value dimension fills the 128 lanes, X^T stays with its rows' threads
-// and goes back through TMEM, over the columns of U, which is done by then.
+// S starts as soon as the rows are there and runs while the state and K' are
+// written as operands. With D = 64 the 64 rows of every accumulator are read as
+// matrix fragments (16 lanes per warp), and X goes back as an operand through
+// shared memory. With D = 128 the value dimension fills the 128 lanes, X^T stays
+// with its rows' threads and goes back through TMEM, over the columns of U, which
+// is done by then.
 // Two blocks per SM: one block's products run while the other prepares.
 //
 // Roundings. Products are bf16 tensor-core products with fp32 sums. The decayed
@@ -59,14 +60,16 @@ NEXAR_D void cp_async16(uint32_t dst, const void* src, bool valid) {
 }
 NEXAR_D void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> NEXAR_D void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-NEXAR_D void ldsm4(uint32_t addr, uint32_t* r) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+// Four 8 x 8 fragments stored transposed; lane l gives the address of row l % 8 of matrix l / 8.
+NEXAR_D void stsm4t(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};"
+               :: "r"(addr), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
 }
-NEXAR_D void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// Packed fp32 pairs: x = x * f + u.
+NEXAR_D void fma2(float& x0, float& x1, float f, float u0, float u1) {
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmov.b64 c, {%3, %4};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x0), "+f"(x1) : "f"(f), "f"(u0), "f"(u1));
 }
 NEXAR_D uint32_t bf2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -78,12 +81,6 @@ NEXAR_D float bf_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 // A tile of 64 rows x D bf16 is D / 64 boxes of 64 rows x 128 bytes in the
 // 128-byte-swizzled layout of the tcgen05 descriptors: 16-byte group g of row r.
 NEXAR_D uint32_t tile_at(int r, int g) { return (uint32_t)((g >> 3) * 8192 + r * 128 + (((g & 7) ^ (r & 7)) << 4)); }
-// Per-thread addresses of ldmatrix.x4 over a 16 x 16 block at (row, col): the
-// four 8 x 8 matrices are (rows 0-7, 8-15) x (cols 0-7, 8-15), rows first.
-NEXAR_D uint32_t block_at(uint32_t tile, int row, int col, int lane) {
-  return tile + tile_at(row + (lane & 15), (col >> 3) + (lane >> 4));
-}
-
 // MN-major operand: boxes of 64 contiguous MN elements x 64 K rows, 8 KB apart.
 NEXAR_D uint64_t desc_mn(uint32_t addr) { return umma_desc_sw128_mnmajor(addr); }
 // kind::f16 MMA whose A operand is read from tensor memory.
@@ -102,16 +99,13 @@ NEXAR_D void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-// 16 lanes x 64 columns as matrix fragments: r[4 n + e] is row lane / 4 + 8 (e / 2), column 8 n + 2 (lane % 4) + e % 2.
-NEXAR_D void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[32]) {
+// 16 lanes x 32 columns as matrix fragments: r[4 n + e] is row lane / 4 + 8 (e / 2), column 8 n + 2 (lane % 4) + e % 2.
+NEXAR_D void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
 NEXAR_D void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -129,17 +123,16 @@ NEXAR_D bool wait_phase(uint64_t* bar, uint32_t parity) {
 }
 
 template <int D, bool STATES> struct Shape {
-  static constexpr int kThreads = D == 64 ? 128 : 256;  // D = 128: two warps per TMEM lane quarter share its columns
-  static constexpr int kHalves = kThreads / 128;
+  static constexpr int kThreads = 256;             // two warps per TMEM lane quarter share its columns
   static constexpr int kTile = kChunk * D * 2;     // bytes of one tile of q, k or v
   static constexpr int kTiles = STATES ? 2 : 3;    // (q,) k, v
-  static constexpr int kStages = D == 64 ? 2 : 1;  // chunks of tiles: two blocks of D = 128 leave no room for a second
+  static constexpr int kStages = D == 64 || STATES ? 2 : 1;  // chunks of tiles: two main blocks of D = 128 leave no room for a second
   static constexpr int kKeys = kStages * kTiles * kTile;         // three parts of the decayed keys; then the output
   static constexpr int kScores = kKeys + 3 * kTile;              // two parts of P, 8 KB each
   static constexpr int kState = kScores + (STATES ? 0 : 16384);  // D = 64: two parts of X, 8 KB each
   static constexpr int kMisc = kState + (STATES || D == 128 ? 0 : 16384);
   static constexpr int kSmem = kMisc + 512;
-  // TMEM columns: U [0, D) (D = 128: also both parts of X^T), O1 and O2 of 64 columns behind it
+  // TMEM columns: U [0, D) (D = 128: also both parts of X^T), O1 (first S) and O2 of 64 columns behind it
   static constexpr uint32_t kCols = STATES ? D : 256;
 };
 
@@ -158,74 +151,69 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
   const int live = max(0, min(len, t_end) - t_begin);   // tokens of this segment that exist
   const int nchunks = (live + kChunk - 1) / kChunk;
 
-  float* pw = reinterpret_cast<float*>(smem + S::kMisc);        // lam^0 .. lam^64
+  float* pw = reinterpret_cast<float*>(smem + S::kMisc);  // lam^0 .. lam^64, then what the rounding of lam^64 leaves out:
+                                                          // over hundreds of chunks that error would add up
   uint64_t* done = reinterpret_cast<uint64_t*>(smem + S::kMisc + 320);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kMisc + 328);
+  uint64_t* s_done = done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kMisc + 336);
   const uint32_t base = smem_u32(smem);
 
-  if (tid == 0) {
-    mbar_init(done, 1);
-    mbar_fence_init();
-  }
-  if (warp == 0) {
-    tmem_alloc(tmem_slot, S::kCols);
-    tmem_relinquish();
-  }
-  const double g = (double)a.log_decay[h];
-  for (int i = tid; i <= kChunk; i += S::kThreads) pw[i] = i ? (float)exp(g * i) : 1.f;
-  // What the rounding of lam^64 leaves out: over hundreds of chunks that error would add up.
-  const float full_rest = (float)(exp(g * kChunk) - (double)(float)exp(g * kChunk));
-  if constexpr (!STATES) {  // the blocks of P above the diagonal stay zero
-    for (int e = tid; e < 1024; e += S::kThreads)
-      reinterpret_cast<uint4*>(smem + S::kScores)[e] = make_uint4(0, 0, 0, 0);
-  }
-
-  // A thread moves 16-byte group g0 of rows r0, r0 + 16, ... of every tile. Token index i sits at row i, or at
+  // A thread moves 16-byte group g0 of rows r0, r0 + kRows, ... of every tile. Token index i sits at row i, or at
   // len - 1 - i when the direction is reversed.
-  constexpr int kGroups = D / 8;
+  constexpr int kGroups = D / 8, kRows = S::kThreads / kGroups, kPasses = kChunk / kRows;
   const int r0 = tid / kGroups, g0 = tid % kGroups;
-  const uint32_t at0 = tile_at(r0, g0);  // + 2048 bytes for 16 rows more
-  const long long dir = R.reverse ? -1 : 1, first = (R.reverse ? len - 1 - t_begin : t_begin) + dir * r0;
-  const __nv_bfloat16* src[S::kTiles];
-  long long step[S::kTiles];  // 16 rows
-  {
-    const __nv_bfloat16* p[3] = {R.q + b * R.qb + h * R.qh, R.k + b * R.kb + h * R.kh, R.v + b * R.vb + h * R.vh};
-    const long long st[3] = {R.qt, R.kt, R.vt};
-#pragma unroll
-    for (int w = 0; w < S::kTiles; ++w) {
-      const int which = STATES ? w + 1 : w;
-      src[w] = p[which] + first * st[which] + g0 * 8;
-      step[w] = dir * st[which] * 16;
-    }
-  }
-  auto prefetch = [&](int c) {  // chunks in order: moves the pointers on
+  const uint32_t at0 = tile_at(r0, g0);  // + 128 kRows bytes for kRows rows more
+  const int dir = R.reverse ? -1 : 1, origin = R.reverse ? len - 1 : 0;
+  auto prefetch = [&](int c) {
     const int left = live - c * kChunk - r0;
+    const long long t = origin + dir * (t_begin + c * kChunk + r0);
     const uint32_t dst = base + (S::kStages == 2 ? (c & 1) * S::kTiles * S::kTile : 0) + at0;
 #pragma unroll
     for (int w = 0; w < S::kTiles; ++w) {
+      const int which = STATES ? w + 1 : w;
+      const long long st = which == 0 ? R.qt : which == 1 ? R.kt : R.vt;
+      const __nv_bfloat16* src = (which == 0 ? R.q + b * R.qb + h * R.qh
+                                  : which == 1 ? R.k + b * R.kb + h * R.kh : R.v + b * R.vb + h * R.vh) + t * st + g0 * 8;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const bool ok = 16 * u < left;
-        cp_async16(dst + w * S::kTile + u * 2048, ok ? src[w] : R.k, ok);
-        src[w] += step[w];
+      for (int u = 0; u < kPasses; ++u) {
+        const bool there = kRows * u < left;
+        cp_async16(dst + w * S::kTile + u * kRows * 128, there ? src + u * (dir * kRows * st) : R.k, there);
       }
     }
     cp_commit();
   };
   if (nchunks > 0) prefetch(0);
 
-  // ---- state. D = 64: fragments of X, rows dk = xr (+ 8), columns dv = 8 n + xc (+ 1). D = 128: row dv of X^T,
-  // columns dk0 .. dk0 + 63.
+  if (tid == 0) {
+    mbar_init(done, 1);
+    mbar_init(s_done, 1);
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, S::kCols);
+    tmem_relinquish();
+  }
+  if (tid <= kChunk + 1) {
+    const double g = (double)a.log_decay[h], p = tid == 0 ? 1.0 : exp(g * min(tid, kChunk));
+    pw[tid] = tid <= kChunk ? (float)p : (float)(p - (double)(float)p);
+  }
+  if constexpr (!STATES) {  // the blocks of P above the diagonal stay zero
+    for (int e = tid; e < 1024; e += S::kThreads)
+      reinterpret_cast<uint4*>(smem + S::kScores)[e] = make_uint4(0, 0, 0, 0);
+  }
+
+  // ---- state. D = 64: fragments of X, rows dk = xr (+ 8), columns dv = 32 half + 8 n + xc (+ 1). D = 128: row dv of
+  // X^T, columns 64 half .. 64 half + 63.
   const int quarter = warp & 3, half = warp >> 2;
-  const int xr = warp * 16 + (lane >> 2), xc = (lane & 3) * 2;
+  const int xr = quarter * 16 + (lane >> 2), xc = (lane & 3) * 2;
   const int dv = quarter * 32 + lane, dk0 = half * 64;
-  constexpr int kX = D == 64 ? 32 : 64;
+  constexpr int kX = D == 64 ? 16 : 64;
   float X[kX];
   auto x_at = [&](int n) {  // element of [dk, dv] that X[n] holds
-    return D == 64 ? (xr + ((n >> 1) & 1) * 8) * D + (n >> 2) * 8 + xc + (n & 1) : (dk0 + n) * D + dv;
+    return D == 64 ? (xr + ((n >> 1) & 1) * 8) * D + half * 32 + (n >> 2) * 8 + xc + (n & 1) : (dk0 + n) * D + dv;
   };
   auto x_at_t = [&](int n) {  // the same element of the transposed state
-    return D == 64 ? ((n >> 2) * 8 + xc + (n & 1)) * D + xr + ((n >> 1) & 1) * 8 : dv * D + dk0 + n;
+    return D == 64 ? (half * 32 + (n >> 2) * 8 + xc + (n & 1)) * D + xr + ((n >> 1) & 1) * 8 : dv * D + dk0 + n;
   };
   const float* x0 = nullptr;
   bool x0_t = false;
@@ -250,10 +238,6 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
   tc_fence_after();
   const uint32_t tbase = *tmem_slot;
   const uint32_t lanes = tbase + ((uint32_t)(quarter * 32) << 16);
-  __nv_bfloat16* out = nullptr;  // this thread's group of the output, advanced like src
-  if constexpr (!STATES)
-    out = R.out + b * R.ob + h * R.oh + (D == 64 ? (first - dir * r0 + dir * (warp * 16 + (lane >> 3))) * R.ot + (lane & 7) * 8
-                                                 : first * R.ot + g0 * 8);
   bool ok = true;
 
   for (int c = 0; c < nchunks; ++c) {
@@ -262,22 +246,58 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
     const uint32_t tq = base + stage, tk = tq + (STATES ? 0 : S::kTile), tv = tk + S::kTile;
     const bool update = want_final || c + 1 < nchunks;
     cp_wait<0>();
+    fence_proxy_async_smem();
     // tiles are visible; everyone has read U and the output, and all leave together if a wait gave up
     if (!__syncthreads_and(ok)) {
       ok = false;
       break;
     }
+    // K steps of 16 in the descriptors: 32 bytes along a K-major row (+ 2; the next box of 64 is + 512), 16 rows of
+    // an MN-major box (+ 128), 8 columns of a TMEM operand.
+    if constexpr (!STATES) {
+      if (tid == 0) {
+        tc_fence_after();
+        const uint64_t kq = umma_desc_sw128_kmajor(tq), kk = umma_desc_sw128_kmajor(tk);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t o = (k >> 2) * 512 + (k & 3) * 2;
+          umma_f16(tbase + D, kq + o, kk + o, umma_idesc_bf16_f32(64, 64), k > 0);
+        }
+        umma_commit(s_done);
+      }
+      __syncwarp();
+    }
     if constexpr (S::kStages == 2) {
       if (c + 1 < nchunks) prefetch(c + 1);
     }
-
+    if (update) {  // ---- keys decayed to the chunk's end, in bf16 parts
+#pragma unroll
+      for (int u = 0; u < kPasses; ++u) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(smem + (tk - base) + at0 + u * kRows * 128);
+        const uint32_t kw[4] = {raw.x, raw.y, raw.z, raw.w};
+        const float w = R.kv * pw[max(n_tok - shift - r0 - kRows * u, 0)];  // rows behind the last token are zero
+        uint32_t p0[4], p1[4], p2[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float x = bf_lo(kw[q]) * w, y = bf_hi(kw[q]) * w;
+          p0[q] = bf2(x, y);
+          const float x1 = x - bf_lo(p0[q]), y1 = y - bf_hi(p0[q]);
+          p1[q] = bf2(x1, y1);
+          p2[q] = bf2(x1 - bf_lo(p1[q]), y1 - bf_hi(p1[q]));
+        }
+        unsigned char* dst = smem + S::kKeys + at0 + u * kRows * 128;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
+        *reinterpret_cast<uint4*>(dst + S::kTile) = make_uint4(p1[0], p1[1], p1[2], p1[3]);
+        *reinterpret_cast<uint4*>(dst + 2 * S::kTile) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
+      }
+    }
     if constexpr (!STATES) {
-      if (have) {  // the state as an operand: two bf16 parts
+      if (have) {  // ---- the state as an operand: two bf16 parts
         if constexpr (D == 64) {
 #pragma unroll
           for (int n = 0; n < kX; n += 2) {
             const uint32_t hi = bf2(X[n], X[n + 1]), lo = bf2(X[n] - bf_lo(hi), X[n + 1] - bf_hi(hi));
-            unsigned char* at = smem + S::kState + tile_at(xr + ((n >> 1) & 1) * 8, n >> 2) + xc * 2;
+            unsigned char* at = smem + S::kState + tile_at(xr + (n & 2) * 4, half * 4 + (n >> 2)) + xc * 2;
             *reinterpret_cast<uint32_t*>(at) = hi;
             *reinterpret_cast<uint32_t*>(at + 8192) = lo;
           }
@@ -297,26 +317,29 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
           tmem_st_wait();
         }
       }
-      // ---- scores: 16 query rows per warp, key blocks of 16 up to the diagonal (D = 128: every second one)
-      const int rb = warp & 3;
-      if (rb * 16 < n_tok) {
-        uint32_t qf[D / 16][4];
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) ldsm4(block_at(tq, rb * 16, k * 16, lane), qf[k]);
-        const int i_lo = rb * 16 + (lane >> 2);
+      // ---- P: 16 query rows and 32 key columns per warp, up to the diagonal
+      if (!wait_phase(s_done, c & 1)) {
+        ok = false;
+        if (lane == 0) atomicExch(&g_decay_error, 1u);
+      }
+      tc_fence_after();
+      if (half * 2 <= quarter && quarter * 16 < n_tok) {
+        uint32_t sc[16];
+        tmem_ld_frag(lanes + D + half * 32, sc);
         // lam^15-jj of this thread's four key columns inside a block of 16
         const float cf[4] = {pw[15 - xc], pw[14 - xc], pw[7 - xc], pw[6 - xc]};
-        for (int kb = half; kb <= rb; kb += S::kHalves) {
-          float P[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        tmem_ld_wait();
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            uint32_t f[4];
-            ldsm4(block_at(tk, kb * 16, k * 16, lane), f);
-            mma16816(P[0], qf[k], f[0], f[2]);
-            mma16816(P[1], qf[k], f[1], f[3]);
-          }
-          if (kb < rb) {
-            const float f0 = R.intra * pw[i_lo - kb * 16 - 15], f1 = R.intra * pw[i_lo + 8 - kb * 16 - 15];
+        for (int m = 0; m < 2; ++m) {
+          const int kb = half * 2 + m;
+          if (kb > quarter) continue;
+          float P[2][4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) P[n][e] = __uint_as_float(sc[m * 8 + n * 4 + e]);
+          if (kb < quarter) {
+            const float f0 = R.intra * pw[xr - kb * 16 - 15], f1 = R.intra * pw[xr + 8 - kb * 16 - 15];
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
               P[n][0] *= f0 * cf[2 * n], P[n][1] *= f0 * cf[2 * n + 1];
@@ -328,7 +351,7 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int gap = (lane >> 2) + (e >> 1) * 8 - (n * 8 + xc + (e & 1));
-                P[n][e] = gap >= 0 ? P[n][e] * (R.intra * pw[gap]) : 0.f;
+                P[n][e] = gap >= 0 ? P[n][e] * (R.intra * pw[max(gap, 0)]) : 0.f;
               }
           }
 #pragma unroll
@@ -337,41 +360,18 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
             for (int p = 0; p < 2; ++p) {
               const float u = P[n][2 * p], v = P[n][2 * p + 1];
               const uint32_t hi = bf2(u, v), lo = bf2(u - bf_lo(hi), v - bf_hi(hi));
-              unsigned char* at = smem + S::kScores + tile_at(i_lo + 8 * p, 2 * kb + n) + xc * 2;
+              unsigned char* at = smem + S::kScores + tile_at(xr + 8 * p, 2 * kb + n) + xc * 2;
               *reinterpret_cast<uint32_t*>(at) = hi;
               *reinterpret_cast<uint32_t*>(at + 8192) = lo;
             }
         }
       }
     }
-    if (update) {  // ---- keys decayed to the chunk's end, in bf16 parts
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(smem + (tk - base) + at0 + u * 2048);
-        const uint32_t kw[4] = {raw.x, raw.y, raw.z, raw.w};
-        const float w = R.kv * pw[max(n_tok - shift - r0 - 16 * u, 0)];  // rows behind the last token are zero
-        uint32_t p0[4], p1[4], p2[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float x = bf_lo(kw[q]) * w, y = bf_hi(kw[q]) * w;
-          p0[q] = bf2(x, y);
-          const float x1 = x - bf_lo(p0[q]), y1 = y - bf_hi(p0[q]);
-          p1[q] = bf2(x1, y1);
-          p2[q] = bf2(x1 - bf_lo(p1[q]), y1 - bf_hi(p1[q]));
-        }
-        unsigned char* dst = smem + S::kKeys + at0 + u * 2048;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
-        *reinterpret_cast<uint4*>(dst + S::kTile) = make_uint4(p1[0], p1[1], p1[2], p1[3]);
-        *reinterpret_cast<uint4*>(dst + 2 * S::kTile) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
-      }
-    }
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
-    if (tid == 0) {
+    if (tid == 0) {  // small parts first
       tc_fence_after();
-      // K steps of 16: 32 bytes along a K-major row (descriptor + 2; the next box of 64 is + 512), 16 rows of an
-      // MN-major box (+ 128), 8 columns of a TMEM operand. Small parts first.
       const uint64_t mv = desc_mn(tv);
       if constexpr (!STATES) {
         constexpr uint32_t id2 = umma_idesc_bf16_f32(D, 64, false, D == 64);
@@ -423,67 +423,85 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
       if (c + 1 < nchunks && ok) prefetch(c + 1);
     }
     if (update) {
-      const float keep = pw[n_tok], rest = n_tok == kChunk ? full_rest : 0.f;
+      const float keep = pw[n_tok], rest = n_tok == kChunk ? pw[kChunk + 1] : 0.f;
 #pragma unroll
-      for (int n = 0; n < kX; n += 32) {
-        uint32_t u[32];
-        if constexpr (D == 64) tmem_ld_frag(lanes, u);
-        else tmem_ld_32x32b_x32(lanes + dk0 + n, u);
+      for (int n = 0; n < kX; n += 16) {
+        uint32_t u[16];
+        if constexpr (D == 64) tmem_ld_frag(lanes + half * 32, u);
+        else tmem_ld_32x32b_x16(lanes + dk0 + n, u);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) X[n + e] = fmaf(X[n + e], keep, fmaf(X[n + e], rest, __uint_as_float(u[e])));
+        for (int e = 0; e < 16; e += 2) {
+          float r0_ = X[n + e], r1_ = X[n + e + 1];
+          fma2(r0_, r1_, rest, __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
+          fma2(X[n + e], X[n + e + 1], keep, r0_, r1_);
+        }
       }
     }
     if constexpr (!STATES) {
       // ---- o = O1 + inter lam^(i + shift) O2, through the keys' space so that whole 16-byte groups are stored
       unsigned char* o_tile = smem + S::kKeys;
+      const long long row = origin + dir * (t_begin + c * kChunk);
+      __nv_bfloat16* out = R.out + b * R.ob + h * R.oh;
       if constexpr (D == 64) {
         const float f0 = R.inter * pw[xr + shift], f1 = R.inter * pw[xr + 8 + shift];  // xr: here a token
-        uint32_t o1[32], o2[32];
-        tmem_ld_frag(lanes + D, o1);
-        if (have) tmem_ld_frag(lanes + D + 64, o2);
+        uint32_t o1[16], o2[16];
+        tmem_ld_frag(lanes + D + half * 32, o1);
+        if (have) tmem_ld_frag(lanes + D + 64 + half * 32, o2);
         tmem_ld_wait();
 #pragma unroll
-        for (int n = 0; n < 32; n += 2) {
+        for (int n = 0; n < 16; n += 2) {
           float x = __uint_as_float(o1[n]), y = __uint_as_float(o1[n + 1]);
           if (have) {
             const float f = n & 2 ? f1 : f0;
             x = fmaf(f, __uint_as_float(o2[n]), x), y = fmaf(f, __uint_as_float(o2[n + 1]), y);
           }
-          *reinterpret_cast<uint32_t*>(o_tile + tile_at(xr + (n & 2) * 4, n >> 2) + xc * 2) = bf2(x, y);
+          *reinterpret_cast<uint32_t*>(o_tile + tile_at(xr + (n & 2) * 4, half * 4 + (n >> 2)) + xc * 2) = bf2(x, y);
         }
-        __syncwarp();  // a warp stores the rows that it wrote
+        __syncwarp();  // a warp stores what it wrote: 16 rows of 64 bytes
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int r = warp * 16 + u * 4 + (lane >> 3);
+        for (int u = 0; u < 2; ++u) {
+          const int r = quarter * 16 + u * 8 + (lane >> 2), g = half * 4 + (lane & 3);
           if (r < n_tok)
-            *reinterpret_cast<uint4*>(out + u * 4 * dir * R.ot) =
-                *reinterpret_cast<const uint4*>(o_tile + tile_at(r, lane & 7));
+            *reinterpret_cast<uint4*>(out + (row + dir * r) * R.ot + g * 8) =
+                *reinterpret_cast<const uint4*>(o_tile + tile_at(r, g));
         }
       } else {
+        // fragments of 16 value rows x 8 tokens, stored transposed
+        float f[8];
 #pragma unroll
-        for (int n = 0; n < 32; n += 16) {
-          const int t0 = half * 32 + n;
-          uint32_t o1[16], o2[16];
-          tmem_ld_32x32b_x16(lanes + D + t0, o1);
-          if (have) tmem_ld_32x32b_x16(lanes + D + 64 + t0, o2);
+        for (int n = 0; n < 8; ++n) f[n] = have ? R.inter * pw[half * 32 + (n >> 1) * 8 + xc + (n & 1) + shift] : 0.f;
+#pragma unroll
+        for (int hl = 0; hl < 2; ++hl) {
+          const uint32_t from = lanes + ((uint32_t)(hl * 16) << 16) + D + half * 32;
+          uint32_t o1[16], o2[16], w[8];
+          tmem_ld_frag(from, o1);
+          if (have) tmem_ld_frag(from + 64, o2);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float o = __uint_as_float(o1[e]);
-            if (have) o = fmaf(R.inter * pw[t0 + e + shift], __uint_as_float(o2[e]), o);
-            reinterpret_cast<__nv_bfloat16*>(o_tile)[(t0 + e) * D + dv] = __float2bfloat16_rn(o);
+          for (int n = 0; n < 16; n += 2) {
+            float x = __uint_as_float(o1[n]), y = __uint_as_float(o1[n + 1]);
+            if (have) {
+              x = fmaf(f[(n >> 2) * 2], __uint_as_float(o2[n]), x);
+              y = fmaf(f[(n >> 2) * 2 + 1], __uint_as_float(o2[n + 1]), y);
+            }
+            w[n >> 1] = bf2(x, y);
+          }
+#pragma unroll
+          for (int n = 0; n < 4; n += 2) {
+            const int t = half * 32 + (n + (lane >> 4)) * 8 + (lane & 7), g = quarter * 4 + hl * 2 + ((lane >> 3) & 1);
+            stsm4t(smem_u32(o_tile) + tile_at(t, g), w[2 * n], w[2 * n + 1], w[2 * n + 2], w[2 * n + 3]);
           }
         }
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (r0 + 16 * u < n_tok)
-            *reinterpret_cast<uint4*>(out + u * 16 * dir * R.ot) =
-                *reinterpret_cast<const uint4*>(o_tile + (r0 + 16 * u) * D * 2 + g0 * 16);
+        for (int u = 0; u < kPasses; ++u) {
+          const int r = r0 + kRows * u;
+          if (r < n_tok)
+            *reinterpret_cast<uint4*>(out + (row + dir * r) * R.ot + g0 * 8) =
+                *reinterpret_cast<const uint4*>(o_tile + at0 + u * kRows * 128);
         }
       }
-      out += kChunk * dir * R.ot;
       have = true;
     }
     tc_fence_before();
@@ -518,7 +536,14 @@ template <int D> __global__ void __launch_bounds__(256) k_decay_scan(const __gri
   const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H;
   const int e = blockIdx.y * 256 + threadIdx.x;  // < D * D / 4
   const int len = a.lengths ? max(0, min(a.lengths[b], a.T)) : a.T;
-  const double g = (double)a.log_decay[h];
+  // whole segments, then one with the last tokens, then empty ones
+  __shared__ float decay[3];
+  const int whole = len / a.seg_tokens, rest = len - whole * a.seg_tokens;
+  if (threadIdx.x < 2) {
+    const double f = exp((double)a.log_decay[h] * (threadIdx.x ? rest : a.seg_tokens));
+    decay[threadIdx.x] = threadIdx.x && !rest ? 1.f : (float)f;
+    if (threadIdx.x == 0) decay[2] = (float)(f - (double)(float)f);
+  }
   float4* p = reinterpret_cast<float4*>(R.segments + (size_t)bh * a.nseg * D * D) + e;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   if (R.init) {
@@ -530,18 +555,24 @@ template <int D> __global__ void __launch_bounds__(256) k_decay_scan(const __gri
       x = reinterpret_cast<const float4*>(q)[e];
     }
   }
-  // whole segments, then one with the last tokens, then empty ones
-  const int whole = len / a.seg_tokens, rest = len - whole * a.seg_tokens;
-  const double whole_decay = exp(g * a.seg_tokens);
-  const float full = (float)whole_decay, full_rest = (float)(whole_decay - (double)full);
-  const float part = rest ? (float)exp(g * rest) : 1.f;
-#pragma unroll 4
-  for (int s = 0; s < a.nseg; ++s) {
-    const float f = s < whole ? full : (s == whole ? part : 1.f), r = s < whole ? full_rest : 0.f;
-    const float4 u = p[(size_t)s * (D * D / 4)];
-    p[(size_t)s * (D * D / 4)] = x;
-    x.x = fmaf(f, x.x, fmaf(r, x.x, u.x)), x.y = fmaf(f, x.y, fmaf(r, x.y, u.y));
-    x.z = fmaf(f, x.z, fmaf(r, x.z, u.z)), x.w = fmaf(f, x.w, fmaf(r, x.w, u.w));
+  __syncthreads();
+  const float full = decay[0], part = decay[1], full_rest = decay[2];
+  constexpr int kBatch = 8;  // segments whose loads are in flight together
+  for (int s0 = 0; s0 < a.nseg; s0 += kBatch) {
+    float4 u[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (s0 + k < a.nseg) u[k] = p[(size_t)(s0 + k) * (D * D / 4)];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int s = s0 + k;
+      if (s < a.nseg) {
+        const float f = s < whole ? full : (s == whole ? part : 1.f), r = s < whole ? full_rest : 0.f;
+        p[(size_t)s * (D * D / 4)] = x;
+        x.x = fmaf(f, x.x, fmaf(r, x.x, u[k].x)), x.y = fmaf(f, x.y, fmaf(r, x.y, u[k].y));
+        x.z = fmaf(f, x.z, fmaf(r, x.z, u[k].z)), x.w = fmaf(f, x.w, fmaf(r, x.w, u[k].w));
+      }
+    }
   }
   if (R.final_state) reinterpret_cast<float4*>(R.final_state + (size_t)bh * D * D)[e] = x;
 }
@@ -627,14 +658,21 @@ unsigned int decay_error_flag() {
   return v;
 }
 
+// Two blocks per SM are resident. Whole sequences take `chunks` steps of a block,
+// n segments ceil(chunks / n) of the main kernel and of the state-only one, and two
+// more launches. In units of a main step with two blocks on the SM (3.3 us for D =
+// 64, 4.5 us for D = 128): a step of a block that has the SM to itself 0.75, a
+// state-only step 0.65, the two launches 2.5 (measured at B H = 96, T = 1024, D =
+// 64: 38 us whole, 42 us in 3 segments; at 16 heads of 128 and T = 16385, 18
+// segments take 152 us).
 int decay_segments(int B, int T, int H, int D, int roles) {
-  // Two blocks per SM are resident; without a split at least half of them should have work.
   const int chunks = (T + kChunk - 1) / kChunk;
-  const long long blocks = (long long)B * H * roles, want = 148LL * 2;
-  if (blocks * 2 > want || chunks < 4) return 1;
-  long long n = want / blocks;
-  if (n > chunks / 2) n = chunks / 2;
-  return (int)n;
+  const long long blocks = (long long)B * H * roles, slots = 148LL * 2;
+  const auto steps = [&](long long n) { return (double)((chunks + n - 1) / n); };
+  if (blocks * 2 > slots) return 1;
+  const long long n = slots / blocks < chunks ? slots / blocks : chunks;
+  const double whole = chunks * (blocks <= 148 ? 0.75 : 1.0), split = steps(n) * 1.65 + 2.5;
+  return split < whole ? (int)n : 1;
 }
 
 cudaError_t decay_attention(const DecayArgs& a, cudaStream_t s, int* launches) {
