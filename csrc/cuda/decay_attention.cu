@@ -19,18 +19,22 @@
 // k_decay_scan turns these into the state before each segment, and the main
 // kernel then runs all segments at once.
 //
-// All products run on tcgen05 (K': the chunk's keys decayed to its end; P: the
-// decayed and masked scores):
-//     both:     S [token, token] = Q K^T
-//     D = 64:   O2 [token, dv] = Q X,     O1 [token, dv] = P V,     U [dk, dv] = K'^T V
-//     D = 128:  O2 [dv, token] = X^T Q^T, O1 [dv, token] = V^T P^T, U [dv, dk] = V^T K'
-// S starts as soon as the rows are there and runs while the state and K' are
-// written as operands. With D = 64 the 64 rows of every accumulator are read as
-// matrix fragments (16 lanes per warp), and X goes back as an operand through
-// shared memory. With D = 128 the value dimension fills the 128 lanes, X^T stays
-// with its rows' threads and goes back through TMEM, over the columns of U, which
-// is done by then.
-// Two blocks per SM: one block's products run while the other prepares.
+// Rows come by TMA in their order; a reversed role numbers them from the end.
+// All products run on tcgen05 in two groups (K': the chunk's keys decayed to its
+// end; P: the decayed and masked scores):
+//     D = 64:   S [token, token] = Q K^T, O [token, dv] = Q X;
+//               then O = lam^(i+1) O + P V, U [dk, dv] = K'^T V
+//     D = 128:  S [token, token] = Q K^T;
+//               then O2 [dv, token] = X^T Q^T, O1 [dv, token] = V^T P^T, U [dv, dk] = V^T K'
+// The first group runs while K' is written; two (D = 128) or three (D = 64) blocks
+// per SM fill each other's gaps during the second. The warp that has no scores above
+// the mask issues the products and the loads. With D = 64 the 64 rows of every
+// accumulator are read as matrix fragments (16 lanes per warp), X goes back as an
+// operand through shared memory, in the place that P takes later, S lies over U, and
+// Q X is scaled in place so that P V adds to it: 128 TMEM columns and 64 KB a block.
+// With D = 128 the value dimension fills the 128 lanes, X^T stays with its rows'
+// threads and goes back through TMEM, over the columns of U, which is done by then;
+// o = lam^(i+1) O2 + O1 at the end.
 //
 // Roundings. Products are bf16 tensor-core products with fp32 sums. The decayed
 // keys that enter the state are split into three bf16 parts (24 bits, all of an
@@ -44,6 +48,7 @@
 // (decay_error_flag), the block leaves together and frees its TMEM.
 #include "common.cuh"
 #include "decoder_api.h"
+#include "gemm_api.h"
 #include "sm100.cuh"
 
 namespace nexar {
@@ -54,12 +59,13 @@ constexpr int kChunk = 64;
 constexpr uint64_t kDecayWaitNs = 2000000000ull;
 __device__ unsigned int g_decay_error = 0;  // set once a wait has given up
 
-NEXAR_D void cp_async16(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 16 : 0;  // zero-filled where there is no token
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+// Box of 64 tokens x 64 columns (x = 0 or 64) of head h and sequence b.
+NEXAR_D void tma_load_rows(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int h, int t, int b) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(h), "r"(t), "r"(b)
+      : "memory");
 }
-NEXAR_D void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> NEXAR_D void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // Four 8 x 8 fragments stored transposed; lane l gives the address of row l % 8 of matrix l / 8.
 NEXAR_D void stsm4t(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};"
@@ -108,37 +114,57 @@ NEXAR_D void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
+NEXAR_D void tmem_st_frag(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 NEXAR_D void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Bounded wait by polling: these waits sit on the chunk's critical path.
-NEXAR_D bool wait_phase(uint64_t* bar, uint32_t parity) {
+// Bounded wait of a whole warp: one lane polls, then every lane sees the completed
+// phase itself (a phase that is usually complete costs one test).
+NEXAR_D bool wait_phase(uint64_t* bar, uint32_t parity, int lane) {
   if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = globaltimer_ns();
-  while (true) {
+  int ok = 1;
+  if (lane == 0) {
+    const unsigned long long t0 = globaltimer_ns();
+    bool got = false;
+    while (!got && ok) {
 #pragma unroll 1
-    for (int i = 0; i < 256; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
-    if (globaltimer_ns() - t0 > kDecayWaitNs) return false;
+      for (int i = 0; i < 64 && !got; ++i) got = mbar_try_wait(bar, parity);
+      if (!got && globaltimer_ns() - t0 > kDecayWaitNs) ok = 0;
+    }
   }
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  if (ok) mbar_try_wait(bar, parity);
+  return ok != 0;
 }
+
+struct DecayMaps {
+  CUtensorMap in[4];
+};
 
 template <int D, bool STATES> struct Shape {
   static constexpr int kThreads = 256;             // two warps per TMEM lane quarter share its columns
+  static constexpr int kBlocks = D == 64 ? 3 : 2;  // resident per SM
   static constexpr int kTile = kChunk * D * 2;     // bytes of one tile of q, k or v
   static constexpr int kTiles = STATES ? 2 : 3;    // (q,) k, v
-  static constexpr int kStages = D == 64 || STATES ? 2 : 1;  // chunks of tiles: two main blocks of D = 128 leave no room for a second
-  static constexpr int kKeys = kStages * kTiles * kTile;         // three parts of the decayed keys; then the output
-  static constexpr int kScores = kKeys + 3 * kTile;              // two parts of P, 8 KB each
-  static constexpr int kState = kScores + (STATES ? 0 : 16384);  // D = 64: two parts of X, 8 KB each
-  static constexpr int kMisc = kState + (STATES || D == 128 ? 0 : 16384);
+  static constexpr int kStages = STATES ? 2 : 1;   // chunks of tiles: the main blocks leave no room for a second
+  static constexpr int kKeys = kStages * kTiles * kTile;  // three parts of the decayed keys; then the output
+  static constexpr int kScores = kKeys + 3 * kTile;       // two parts of P (D = 64: first of X), 8 KB each
+  static constexpr int kMisc = kScores + (STATES ? 0 : 16384);
   static constexpr int kSmem = kMisc + 512;
-  // TMEM columns: U [0, D) (D = 128: also both parts of X^T), O1 (first S) and O2 of 64 columns behind it
-  static constexpr uint32_t kCols = STATES ? D : 256;
+  // TMEM columns. U at 0 (D = 64: first S; D = 128: first both parts of X^T); D = 64: O at 64;
+  // D = 128: O1 (first S) at 128, O2 at 192.
+  static constexpr uint32_t kCols = STATES ? D : 2 * D;
 };
 
 template <int D, bool STATES>
-__global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
-    k_decay_chunk(const __grid_constant__ DecayArgs a) {
+__global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::kBlocks)
+    k_decay_chunk(const __grid_constant__ DecayArgs a, const __grid_constant__ DecayMaps maps) {
   using S = Shape<D, STATES>;
   extern __shared__ __align__(1024) unsigned char smem[];
   const DecayRole& R = a.role[blockIdx.z];
@@ -150,44 +176,39 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
   const int t_end = min(a.T, t_begin + a.seg_tokens);   // index i, counted from the first token of the direction
   const int live = max(0, min(len, t_end) - t_begin);   // tokens of this segment that exist
   const int nchunks = (live + kChunk - 1) / kChunk;
+  const bool rev = R.reverse != 0;
 
   float* pw = reinterpret_cast<float*>(smem + S::kMisc);  // lam^0 .. lam^64, then what the rounding of lam^64 leaves out:
                                                           // over hundreds of chunks that error would add up
-  uint64_t* done = reinterpret_cast<uint64_t*>(smem + S::kMisc + 320);
-  uint64_t* s_done = done + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kMisc + 336);
+  uint64_t* done = reinterpret_cast<uint64_t*>(smem + S::kMisc + 320);  // second group of products
+  uint64_t* s_done = done + 1;                                          // first group
+  uint64_t* full = done + 2;                                            // [stage] tiles
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kMisc + 352);
   const uint32_t base = smem_u32(smem);
 
-  // A thread moves 16-byte group g0 of rows r0, r0 + kRows, ... of every tile. Token index i sits at row i, or at
-  // len - 1 - i when the direction is reversed.
-  constexpr int kGroups = D / 8, kRows = S::kThreads / kGroups, kPasses = kChunk / kRows;
-  const int r0 = tid / kGroups, g0 = tid % kGroups;
-  const uint32_t at0 = tile_at(r0, g0);  // + 128 kRows bytes for kRows rows more
-  const int dir = R.reverse ? -1 : 1, origin = R.reverse ? len - 1 : 0;
-  auto prefetch = [&](int c) {
-    const int left = live - c * kChunk - r0;
-    const long long t = origin + dir * (t_begin + c * kChunk + r0);
-    const uint32_t dst = base + (S::kStages == 2 ? (c & 1) * S::kTiles * S::kTile : 0) + at0;
-#pragma unroll
-    for (int w = 0; w < S::kTiles; ++w) {
+  // Row r of chunk c's tiles is token first_row(c) + r: index 64 c + r of the segment, or (reversed) 64 c + 63 - r.
+  const auto first_row = [&](int c) { return rev ? len - t_begin - (c + 1) * kChunk : t_begin + c * kChunk; };
+  // The loads of chunk c's tiles from w0 to w1 (of q, k, v; STATES: k, v), by one thread; rows outside the tensor are
+  // filled with zeros. The first call of a chunk announces all its bytes.
+  const auto load = [&](int c, int w0, int w1) {
+    const int s = S::kStages == 2 ? c & 1 : 0, t0 = first_row(c);
+    const uint32_t dst = base + s * S::kTiles * S::kTile;
+    if (w0 == 0) mbar_arrive_expect_tx(full + s, S::kTiles * S::kTile);
+    for (int w = w0; w < w1; ++w) {
       const int which = STATES ? w + 1 : w;
-      const long long st = which == 0 ? R.qt : which == 1 ? R.kt : R.vt;
-      const __nv_bfloat16* src = (which == 0 ? R.q + b * R.qb + h * R.qh
-                                  : which == 1 ? R.k + b * R.kb + h * R.kh : R.v + b * R.vb + h * R.vh) + t * st + g0 * 8;
+      const CUtensorMap* m = &maps.in[which == 0 ? R.q : which == 1 ? R.k : R.v];
 #pragma unroll
-      for (int u = 0; u < kPasses; ++u) {
-        const bool there = kRows * u < left;
-        cp_async16(dst + w * S::kTile + u * kRows * 128, there ? src + u * (dir * kRows * st) : R.k, there);
-      }
+      for (int x = 0; x < D; x += 64) tma_load_rows(dst + w * S::kTile + (x >> 6) * 8192, m, full + s, x, h, t0, b);
     }
-    cp_commit();
   };
-  if (nchunks > 0) prefetch(0);
-
   if (tid == 0) {
     mbar_init(done, 1);
     mbar_init(s_done, 1);
+    mbar_init(full, 1);
+    mbar_init(full + 1, 1);
     mbar_fence_init();
+    if (nchunks > 0) load(0, 0, S::kTiles);
+    if (S::kStages == 2 && nchunks > 1) load(1, 0, S::kTiles);
   }
   if (warp == 0) {
     tmem_alloc(tmem_slot, S::kCols);
@@ -196,10 +217,6 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
   if (tid <= kChunk + 1) {
     const double g = (double)a.log_decay[h], p = tid == 0 ? 1.0 : exp(g * min(tid, kChunk));
     pw[tid] = tid <= kChunk ? (float)p : (float)(p - (double)(float)p);
-  }
-  if constexpr (!STATES) {  // the blocks of P above the diagonal stay zero
-    for (int e = tid; e < 1024; e += S::kThreads)
-      reinterpret_cast<uint4*>(smem + S::kScores)[e] = make_uint4(0, 0, 0, 0);
   }
 
   // ---- state. D = 64: fragments of X, rows dk = xr (+ 8), columns dv = 32 half + 8 n + xc (+ 1). D = 128: row dv of
@@ -231,55 +248,84 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
   for (int n = 0; n < kX; ++n) X[n] = !x0 ? 0.f : x0[x0_t ? x_at_t(n) : x_at(n)];
   bool have = x0 != nullptr;  // a state that is known to be zero is not multiplied
   const bool want_final = STATES || (R.final_state != nullptr && a.nseg == 1);
-  const int shift = R.reverse ? 0 : 1;  // exponents: i + shift and n - shift - j
+  const int shift = rev ? 0 : 1;  // exponents: i + shift and n - shift - j
 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = *tmem_slot;
   const uint32_t lanes = tbase + ((uint32_t)(quarter * 32) << 16);
+  constexpr int kGroups = D / 8, kRows = S::kThreads / kGroups, kPasses = kChunk / kRows;
+  const int r0 = tid / kGroups, g0 = tid % kGroups;  // 16-byte group g0 of rows r0, r0 + kRows, ... of a tile
+  const uint32_t at0 = tile_at(r0, g0);              // + 128 kRows bytes for kRows rows more
   bool ok = true;
+  int seen = 0;  // chunks whose loads were waited for
+  const bool ctl = warp == (rev ? 3 : 4) && lane == 0;  // issues products and loads: no scores of this warp are kept
+  const auto give_up = [&]() {
+    ok = false;
+    if (lane == 0) atomicExch(&g_decay_error, 1u);
+  };
 
   for (int c = 0; c < nchunks; ++c) {
     const int n_tok = min(kChunk, live - c * kChunk);
+    const int lo = rev ? kChunk - n_tok : 0, hi = rev ? kChunk : n_tok;  // rows [lo, hi) are tokens of this chunk
     const uint32_t stage = S::kStages == 2 ? (c & 1) * S::kTiles * S::kTile : 0;
     const uint32_t tq = base + stage, tk = tq + (STATES ? 0 : S::kTile), tv = tk + S::kTile;
     const bool update = want_final || c + 1 < nchunks;
-    cp_wait<0>();
-    fence_proxy_async_smem();
-    // tiles are visible; everyone has read U and the output, and all leave together if a wait gave up
+    if constexpr (!STATES && D == 64) {
+      if (have) {  // ---- the state as an operand: two bf16 parts
+#pragma unroll
+        for (int n = 0; n < kX; n += 2) {
+          const uint32_t hi_ = bf2(X[n], X[n + 1]), lo_ = bf2(X[n] - bf_lo(hi_), X[n + 1] - bf_hi(hi_));
+          unsigned char* at = smem + S::kScores + tile_at(xr + (n & 2) * 4, half * 4 + (n >> 2)) + xc * 2;
+          *reinterpret_cast<uint32_t*>(at) = hi_;
+          *reinterpret_cast<uint32_t*>(at + 8192) = lo_;
+        }
+        fence_proxy_async_smem();
+      }
+    }
+    // The state is written (D = 64); everyone has read U and the output. All leave together if a wait gave up.
     if (!__syncthreads_and(ok)) {
       ok = false;
       break;
     }
+    if (!wait_phase(full + (S::kStages == 2 ? c & 1 : 0), (S::kStages == 2 ? c >> 1 : c) & 1, lane)) give_up();
+    else seen = c + 1;
     // K steps of 16 in the descriptors: 32 bytes along a K-major row (+ 2; the next box of 64 is + 512), 16 rows of
-    // an MN-major box (+ 128), 8 columns of a TMEM operand.
+    // an MN-major box (+ 128), 8 columns of a TMEM operand. Small parts first.
     if constexpr (!STATES) {
-      if (tid == 0) {
+      if (ctl) {
         tc_fence_after();
         const uint64_t kq = umma_desc_sw128_kmajor(tq), kk = umma_desc_sw128_kmajor(tk);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t o = (k >> 2) * 512 + (k & 3) * 2;
-          umma_f16(tbase + D, kq + o, kk + o, umma_idesc_bf16_f32(64, 64), k > 0);
+          umma_f16(tbase + (D == 64 ? 0 : 128), kq + o, kk + o, umma_idesc_bf16_f32(64, 64), k > 0);
+        }
+        if (D == 64 && have) {
+          const uint64_t mx = desc_mn(base + S::kScores);
+#pragma unroll
+          for (int p = 1; p >= 0; --p)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_f16(tbase + 64, kq + k * 2, mx + p * 512 + 128 * k, umma_idesc_bf16_f32(64, 64, false, true), p == 0 || k > 0);
         }
         umma_commit(s_done);
       }
       __syncwarp();
     }
-    if constexpr (S::kStages == 2) {
-      if (c + 1 < nchunks) prefetch(c + 1);
-    }
     if (update) {  // ---- keys decayed to the chunk's end, in bf16 parts
 #pragma unroll
       for (int u = 0; u < kPasses; ++u) {
+        const int r = r0 + kRows * u;
         const uint4 raw = *reinterpret_cast<const uint4*>(smem + (tk - base) + at0 + u * kRows * 128);
         const uint32_t kw[4] = {raw.x, raw.y, raw.z, raw.w};
-        const float w = R.kv * pw[max(n_tok - shift - r0 - kRows * u, 0)];  // rows behind the last token are zero
+        const bool there = r >= lo && r < hi;
+        const float w = R.kv * pw[there ? (rev ? n_tok - 63 + r : n_tok - 1 - r) : 0];
         uint32_t p0[4], p1[4], p2[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float x = bf_lo(kw[q]) * w, y = bf_hi(kw[q]) * w;
+          const float x = there ? bf_lo(kw[q]) * w : 0.f, y = there ? bf_hi(kw[q]) * w : 0.f;
           p0[q] = bf2(x, y);
           const float x1 = x - bf_lo(p0[q]), y1 = y - bf_hi(p0[q]);
           p1[q] = bf2(x1, y1);
@@ -291,137 +337,134 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
         *reinterpret_cast<uint4*>(dst + 2 * S::kTile) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
       }
     }
-    if constexpr (!STATES) {
-      if (have) {  // ---- the state as an operand: two bf16 parts
-        if constexpr (D == 64) {
+    if (n_tok < kChunk && a.lengths) {  // rows of v behind the last token may hold anything: P and K' are zero there
 #pragma unroll
-          for (int n = 0; n < kX; n += 2) {
-            const uint32_t hi = bf2(X[n], X[n + 1]), lo = bf2(X[n] - bf_lo(hi), X[n + 1] - bf_hi(hi));
-            unsigned char* at = smem + S::kState + tile_at(xr + (n & 2) * 4, half * 4 + (n >> 2)) + xc * 2;
-            *reinterpret_cast<uint32_t*>(at) = hi;
-            *reinterpret_cast<uint32_t*>(at + 8192) = lo;
+      for (int u = 0; u < kPasses; ++u) {
+        const int r = r0 + kRows * u;
+        if (r < lo || r >= hi)
+          *reinterpret_cast<uint4*>(smem + (tv - base) + at0 + u * kRows * 128) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    if constexpr (!STATES && D == 128) {
+      if (have) {  // ---- the state as an operand: two bf16 parts
+#pragma unroll
+        for (int n = 0; n < kX; n += 32) {
+          uint32_t hi_[16], lo_[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float x = X[n + 2 * e], y = X[n + 2 * e + 1];
+            hi_[e] = bf2(x, y);
+            lo_[e] = bf2(x - bf_lo(hi_[e]), y - bf_hi(hi_[e]));
+          }
+          tmem_st_x16(lanes + half * 32 + n / 2, hi_);
+          tmem_st_x16(lanes + 64 + half * 32 + n / 2, lo_);
+        }
+        tmem_st_wait();
+      }
+    }
+    if constexpr (!STATES) {
+      // ---- P: 16 query rows and 32 key columns per warp, up to the diagonal
+      if (!wait_phase(s_done, c & 1, lane)) give_up();
+      tc_fence_after();
+      uint32_t sc[16], o[16];
+      const bool some = rev ? half * 2 + 1 >= quarter : half * 2 <= quarter, scaled = D == 64 && have;
+      if (some) tmem_ld_frag(lanes + (D == 64 ? 0 : 128) + half * 32, sc);
+      if (scaled) tmem_ld_frag(lanes + 64 + half * 32, o);
+      tmem_ld_wait();
+      if (scaled) {  // Q X -> inter lam^(i + shift) Q X, in place
+        const float f0 = R.inter * pw[rev ? 63 - xr : xr + 1], f1 = R.inter * pw[rev ? 55 - xr : xr + 9];
+#pragma unroll
+        for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * (n & 2 ? f1 : f0));
+        tmem_st_frag(lanes + 64 + half * 32, o);
+      }
+      // the part of the power that belongs to this thread's four key columns inside a block of 16
+      const int c0 = rev ? xc : 15 - xc, cs = rev ? 1 : -1;
+      const float cf[4] = {pw[c0], pw[c0 + cs], pw[c0 + 8 * cs], pw[c0 + 9 * cs]};
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const int kb = half * 2 + m;
+        float P[2][4];
+        if (kb == quarter) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int ahead = (lane >> 2) + (e >> 1) * 8 - (n * 8 + xc + (e & 1)), gap = rev ? -ahead : ahead;
+              P[n][e] = gap >= 0 ? __uint_as_float(sc[m * 8 + n * 4 + e]) * (R.intra * pw[max(gap, 0)]) : 0.f;
+            }
+        } else if ((kb < quarter) != rev) {
+          const int e0 = rev ? kb * 16 - xr : xr - kb * 16 - 15;
+          const float f0 = R.intra * pw[e0], f1 = R.intra * pw[rev ? e0 - 8 : e0 + 8];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const uint32_t* v = sc + m * 8 + n * 4;
+            P[n][0] = __uint_as_float(v[0]) * (f0 * cf[2 * n]), P[n][1] = __uint_as_float(v[1]) * (f0 * cf[2 * n + 1]);
+            P[n][2] = __uint_as_float(v[2]) * (f1 * cf[2 * n]), P[n][3] = __uint_as_float(v[3]) * (f1 * cf[2 * n + 1]);
           }
         } else {
 #pragma unroll
-          for (int n = 0; n < kX; n += 32) {
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float x = X[n + 2 * e], y = X[n + 2 * e + 1];
-              hi[e] = bf2(x, y);
-              lo[e] = bf2(x - bf_lo(hi[e]), y - bf_hi(hi[e]));
-            }
-            tmem_st_x16(lanes + half * 32 + n / 2, hi);
-            tmem_st_x16(lanes + 64 + half * 32 + n / 2, lo);
-          }
-          tmem_st_wait();
+          for (int n = 0; n < 2; ++n) P[n][0] = P[n][1] = P[n][2] = P[n][3] = 0.f;
         }
-      }
-      // ---- P: 16 query rows and 32 key columns per warp, up to the diagonal
-      if (!wait_phase(s_done, c & 1)) {
-        ok = false;
-        if (lane == 0) atomicExch(&g_decay_error, 1u);
-      }
-      tc_fence_after();
-      if (half * 2 <= quarter && quarter * 16 < n_tok) {
-        uint32_t sc[16];
-        tmem_ld_frag(lanes + D + half * 32, sc);
-        // lam^15-jj of this thread's four key columns inside a block of 16
-        const float cf[4] = {pw[15 - xc], pw[14 - xc], pw[7 - xc], pw[6 - xc]};
-        tmem_ld_wait();
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const int kb = half * 2 + m;
-          if (kb > quarter) continue;
-          float P[2][4];
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) P[n][e] = __uint_as_float(sc[m * 8 + n * 4 + e]);
-          if (kb < quarter) {
-            const float f0 = R.intra * pw[xr - kb * 16 - 15], f1 = R.intra * pw[xr + 8 - kb * 16 - 15];
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              P[n][0] *= f0 * cf[2 * n], P[n][1] *= f0 * cf[2 * n + 1];
-              P[n][2] *= f1 * cf[2 * n], P[n][3] *= f1 * cf[2 * n + 1];
-            }
-          } else {
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int gap = (lane >> 2) + (e >> 1) * 8 - (n * 8 + xc + (e & 1));
-                P[n][e] = gap >= 0 ? P[n][e] * (R.intra * pw[max(gap, 0)]) : 0.f;
-              }
+          for (int p = 0; p < 2; ++p) {
+            const float u = P[n][2 * p], v = P[n][2 * p + 1];
+            const uint32_t hi_ = bf2(u, v), lo_ = bf2(u - bf_lo(hi_), v - bf_hi(hi_));
+            unsigned char* at = smem + S::kScores + tile_at(xr + 8 * p, 2 * kb + n) + xc * 2;
+            *reinterpret_cast<uint32_t*>(at) = hi_;
+            *reinterpret_cast<uint32_t*>(at + 8192) = lo_;
           }
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-              const float u = P[n][2 * p], v = P[n][2 * p + 1];
-              const uint32_t hi = bf2(u, v), lo = bf2(u - bf_lo(hi), v - bf_hi(hi));
-              unsigned char* at = smem + S::kScores + tile_at(xr + 8 * p, 2 * kb + n) + xc * 2;
-              *reinterpret_cast<uint32_t*>(at) = hi;
-              *reinterpret_cast<uint32_t*>(at + 8192) = lo;
-            }
-        }
       }
+      if (D == 64) tmem_st_wait();
     }
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
-    if (tid == 0) {  // small parts first
+    const bool more = c + S::kStages < nchunks;
+    if (ctl) {
       tc_fence_after();
       const uint64_t mv = desc_mn(tv);
       if constexpr (!STATES) {
-        constexpr uint32_t id2 = umma_idesc_bf16_f32(D, 64, false, D == 64);
-        constexpr uint32_t id1 = umma_idesc_bf16_f32(D, 64, D == 128, D == 64);
-        const uint64_t kq = umma_desc_sw128_kmajor(tq), kp = umma_desc_sw128_kmajor(base + S::kScores);
-        if (have) {
-          [[maybe_unused]] const uint64_t mx = desc_mn(base + S::kState);
+        if (D == 128 && have) {
+          const uint64_t kq = umma_desc_sw128_kmajor(tq);
 #pragma unroll
           for (int p = 1; p >= 0; --p)
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint32_t acc = p == 0 || k > 0;
-              if constexpr (D == 64)
-                umma_f16(tbase + D + 64, kq + k * 2, mx + p * 512 + 128 * k, id2, acc);
-              else
-                umma_ts(tbase + D + 64, tbase + p * 64 + k * 8, kq + (k >> 2) * 512 + (k & 3) * 2, id2, acc);
-            }
+            for (int k = 0; k < D / 16; ++k)
+              umma_ts(tbase + 192, tbase + p * 64 + k * 8, kq + (k >> 2) * 512 + (k & 3) * 2, umma_idesc_bf16_f32(D, 64),
+                      p == 0 || k > 0);
         }
+        const uint64_t kp = umma_desc_sw128_kmajor(base + S::kScores);
 #pragma unroll
         for (int p = 1; p >= 0; --p)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
+            const uint32_t acc = p == 0 || k > 0;
             if constexpr (D == 64)
-              umma_f16(tbase + D, kp + p * 512 + k * 2, mv + 128 * k, id1, p == 0 || k > 0);
+              umma_f16(tbase + 64, kp + p * 512 + k * 2, mv + 128 * k, umma_idesc_bf16_f32(64, 64, false, true), acc || have);
             else
-              umma_f16(tbase + D, mv + 128 * k, kp + p * 512 + k * 2, id1, p == 0 || k > 0);
+              umma_f16(tbase + 128, mv + 128 * k, kp + p * 512 + k * 2, umma_idesc_bf16_f32(D, 64, true, false), acc);
           }
       }
-      if (update) {  // behind the products that read X^T, whose columns U takes
-        constexpr uint32_t idu = umma_idesc_bf16_f32(D, D, true, true);
+      if (update) {  // D = 128: behind the products that read X^T, whose columns U takes
         const uint64_t mk = desc_mn(base + S::kKeys);
 #pragma unroll
         for (int p = 2; p >= 0; --p)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint64_t part = mk + p * (S::kTile >> 4) + 128 * k;
-            umma_f16(tbase, D == 64 ? part : mv + 128 * k, D == 64 ? mv + 128 * k : part, idu, p < 2 || k > 0);
+            umma_f16(tbase, D == 64 ? part : mv + 128 * k, D == 64 ? mv + 128 * k : part,
+                     umma_idesc_bf16_f32(D, D, true, true), p < 2 || k > 0);
           }
       }
       umma_commit(done);
+      if (!STATES && D == 64 && more) load(c + 1, 0, 2);  // nothing reads q and k any more
     }
     __syncwarp();
-    if (!wait_phase(done, c & 1)) {
-      ok = false;
-      if (lane == 0) atomicExch(&g_decay_error, 1u);
-    }
+    if (!wait_phase(done, c & 1, lane)) give_up();
     tc_fence_after();
-    if constexpr (S::kStages == 1) {
-      if (c + 1 < nchunks && ok) prefetch(c + 1);
-    }
+    if (ctl && more) load(c + S::kStages, !STATES && D == 64 ? 2 : 0, S::kTiles);
     if (update) {
       const float keep = pw[n_tok], rest = n_tok == kChunk ? pw[kChunk + 1] : 0.f;
 #pragma unroll
@@ -432,48 +475,42 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
-          float r0_ = X[n + e], r1_ = X[n + e + 1];
-          fma2(r0_, r1_, rest, __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
-          fma2(X[n + e], X[n + e + 1], keep, r0_, r1_);
+          float s0 = X[n + e], s1 = X[n + e + 1];
+          fma2(s0, s1, rest, __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
+          fma2(X[n + e], X[n + e + 1], keep, s0, s1);
         }
       }
     }
     if constexpr (!STATES) {
-      // ---- o = O1 + inter lam^(i + shift) O2, through the keys' space so that whole 16-byte groups are stored
+      // ---- the output, through the keys' space so that whole 16-byte groups are stored
       unsigned char* o_tile = smem + S::kKeys;
-      const long long row = origin + dir * (t_begin + c * kChunk);
-      __nv_bfloat16* out = R.out + b * R.ob + h * R.oh;
+      __nv_bfloat16* out = R.out + b * R.ob + h * R.oh + (long long)first_row(c) * R.ot;
       if constexpr (D == 64) {
-        const float f0 = R.inter * pw[xr + shift], f1 = R.inter * pw[xr + 8 + shift];  // xr: here a token
-        uint32_t o1[16], o2[16];
-        tmem_ld_frag(lanes + D + half * 32, o1);
-        if (have) tmem_ld_frag(lanes + D + 64 + half * 32, o2);
+        uint32_t o[16];
+        tmem_ld_frag(lanes + 64 + half * 32, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int n = 0; n < 16; n += 2) {
-          float x = __uint_as_float(o1[n]), y = __uint_as_float(o1[n + 1]);
-          if (have) {
-            const float f = n & 2 ? f1 : f0;
-            x = fmaf(f, __uint_as_float(o2[n]), x), y = fmaf(f, __uint_as_float(o2[n + 1]), y);
-          }
-          *reinterpret_cast<uint32_t*>(o_tile + tile_at(xr + (n & 2) * 4, half * 4 + (n >> 2)) + xc * 2) = bf2(x, y);
-        }
+        for (int n = 0; n < 16; n += 2)
+          *reinterpret_cast<uint32_t*>(o_tile + tile_at(xr + (n & 2) * 4, half * 4 + (n >> 2)) + xc * 2) =
+              bf2(__uint_as_float(o[n]), __uint_as_float(o[n + 1]));
         __syncwarp();  // a warp stores what it wrote: 16 rows of 64 bytes
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int r = quarter * 16 + u * 8 + (lane >> 2), g = half * 4 + (lane & 3);
-          if (r < n_tok)
-            *reinterpret_cast<uint4*>(out + (row + dir * r) * R.ot + g * 8) =
-                *reinterpret_cast<const uint4*>(o_tile + tile_at(r, g));
+          if (r >= lo && r < hi)
+            *reinterpret_cast<uint4*>(out + r * R.ot + g * 8) = *reinterpret_cast<const uint4*>(o_tile + tile_at(r, g));
         }
       } else {
         // fragments of 16 value rows x 8 tokens, stored transposed
         float f[8];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) f[n] = have ? R.inter * pw[half * 32 + (n >> 1) * 8 + xc + (n & 1) + shift] : 0.f;
+        for (int n = 0; n < 8; ++n) {
+          const int r = half * 32 + (n >> 1) * 8 + xc + (n & 1);
+          f[n] = have ? R.inter * pw[rev ? 63 - r : r + 1] : 0.f;
+        }
 #pragma unroll
         for (int hl = 0; hl < 2; ++hl) {
-          const uint32_t from = lanes + ((uint32_t)(hl * 16) << 16) + D + half * 32;
+          const uint32_t from = lanes + ((uint32_t)(hl * 16) << 16) + 128 + half * 32;
           uint32_t o1[16], o2[16], w[8];
           tmem_ld_frag(from, o1);
           if (have) tmem_ld_frag(from + 64, o2);
@@ -493,12 +530,13 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
             stsm4t(smem_u32(o_tile) + tile_at(t, g), w[2 * n], w[2 * n + 1], w[2 * n + 2], w[2 * n + 3]);
           }
         }
+        tc_fence_before();
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < kPasses; ++u) {
           const int r = r0 + kRows * u;
-          if (r < n_tok)
-            *reinterpret_cast<uint4*>(out + (row + dir * r) * R.ot + g0 * 8) =
+          if (r >= lo && r < hi)
+            *reinterpret_cast<uint4*>(out + r * R.ot + g0 * 8) =
                 *reinterpret_cast<const uint4*>(o_tile + at0 + u * kRows * 128);
         }
       }
@@ -519,7 +557,8 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, 2)
 #pragma unroll
     for (int n = 0; n < kX; ++n) dst[x_at(n)] = X[n];
   }
-  cp_wait<0>();
+  for (int c = seen; c < min(nchunks, seen + S::kStages); ++c)  // no load may still be landing when the block exits
+    wait_phase(full + (S::kStages == 2 ? c & 1 : 0), (S::kStages == 2 ? c >> 1 : c) & 1, lane);
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
@@ -627,28 +666,34 @@ template <int D> __global__ void __launch_bounds__(D * 2) k_decay_step(const Dec
 }
 
 template <int D, bool STATES>
-cudaError_t launch_chunks(const DecayArgs& a, int roles, cudaStream_t s) {
+cudaError_t launch_chunks(const DecayArgs& a, const DecayMaps& maps, int roles, cudaStream_t s) {
   using S = Shape<D, STATES>;
   const cudaError_t e =
       cudaFuncSetAttribute(k_decay_chunk<D, STATES>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
-  k_decay_chunk<D, STATES><<<dim3(a.B * a.H, a.nseg, roles), S::kThreads, S::kSmem, s>>>(a);
+  k_decay_chunk<D, STATES><<<dim3(a.B * a.H, a.nseg, roles), S::kThreads, S::kSmem, s>>>(a, maps);
   return cudaGetLastError();
 }
 
 template <int D> cudaError_t decay_typed(const DecayArgs& a, cudaStream_t s, int* launches) {
   *launches = 0;
+  DecayMaps maps;
+  for (int i = 0; i < a.nin; ++i) {
+    const DecayInput& t = a.in[i];
+    const cudaError_t e = make_tmap_bf16_heads(&maps.in[i], t.p, a.B, a.T, a.H, D, t.sb, t.st, t.sh);
+    if (e != cudaSuccess) return e;
+  }
   if (a.nseg > 1) {
     // roles that read another role's segment states come last and need no states of their own
     int own = 0;
     while (own < a.nroles && a.role[own].segments_from < 0) ++own;
-    const cudaError_t e = launch_chunks<D, true>(a, own, s);
+    const cudaError_t e = launch_chunks<D, true>(a, maps, own, s);
     if (e != cudaSuccess) return e;
     k_decay_scan<D><<<dim3(a.B * a.H, D * D / 1024, own), 256, 0, s>>>(a);
     *launches += 2;
   }
   *launches += 1;
-  return launch_chunks<D, false>(a, a.nroles, s);
+  return launch_chunks<D, false>(a, maps, a.nroles, s);
 }
 }  // namespace
 
@@ -676,7 +721,7 @@ int decay_segments(int B, int T, int H, int D, int roles) {
 }
 
 cudaError_t decay_attention(const DecayArgs& a, cudaStream_t s, int* launches) {
-  if (a.nroles < 1 || a.nroles > 3 || a.B < 1 || a.H < 1 || a.T < 1 || (long long)a.B * a.H > 0x7fffffffLL || a.nseg > 65535 || a.nseg < 1 ||
+  if (a.nroles < 1 || a.nroles > 3 || a.nin < 1 || a.nin > 4 || a.B < 1 || a.H < 1 || a.T < 1 || (long long)a.B * a.H > 0x7fffffffLL || a.nseg > 65535 || a.nseg < 1 ||
       (long long)a.nseg * a.seg_tokens < a.T || (a.nseg > 1 && a.seg_tokens % kChunk))
     return cudaErrorInvalidValue;
   if (a.D == 64) return decay_typed<64>(a, s, launches);
