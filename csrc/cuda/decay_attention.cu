@@ -19,7 +19,6 @@
 // k_decay_scan turns these into the state before each segment, and the main
 // kernel then runs all segments at once.
 //
-// Rows come by TMA in their order; a reversed role numbers them from the end.
 // All products run on tcgen05 in two groups (K': the chunk's keys decayed to its
 // end; P: the decayed and masked scores):
 //     D = 64:   S [token, token] = Q K^T, O [token, dv] = Q X;
@@ -27,14 +26,15 @@
 //     D = 128:  S [token, token] = Q K^T;
 //               then O2 [dv, token] = X^T Q^T, O1 [dv, token] = V^T P^T, U [dv, dk] = V^T K'
 // The first group runs while K' is written; two (D = 128) or three (D = 64) blocks
-// per SM fill each other's gaps during the second. The warp that has no scores above
-// the mask issues the products and the loads. With D = 64 the 64 rows of every
+// per SM fill each other's gaps during the second. With D = 64 the 64 rows of every
 // accumulator are read as matrix fragments (16 lanes per warp), X goes back as an
 // operand through shared memory, in the place that P takes later, S lies over U, and
 // Q X is scaled in place so that P V adds to it: 128 TMEM columns and 64 KB a block.
 // With D = 128 the value dimension fills the 128 lanes, X^T stays with its rows'
 // threads and goes back through TMEM, over the columns of U, which is done by then;
-// o = lam^(i+1) O2 + O1 at the end.
+// o = lam^(i+1) O2 + O1 at the end. Rows come by cp.async, each thread its 16-byte
+// groups (a reversed role simply reads its rows from the end): tensor-map loads of
+// the same tiles measured 17 to 25 % slower here, with D = 128.
 //
 // Roundings. Products are bf16 tensor-core products with fp32 sums. The decayed
 // keys that enter the state are split into three bf16 parts (24 bits, all of an
@@ -48,7 +48,6 @@
 // (decay_error_flag), the block leaves together and frees its TMEM.
 #include "common.cuh"
 #include "decoder_api.h"
-#include "gemm_api.h"
 #include "sm100.cuh"
 
 namespace nexar {
@@ -59,13 +58,12 @@ constexpr int kChunk = 64;
 constexpr uint64_t kDecayWaitNs = 2000000000ull;
 __device__ unsigned int g_decay_error = 0;  // set once a wait has given up
 
-// Box of 64 tokens x 64 columns (x = 0 or 64) of head h and sequence b.
-NEXAR_D void tma_load_rows(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int h, int t, int b) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(h), "r"(t), "r"(b)
-      : "memory");
+NEXAR_D void cp_async16(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;  // zero-filled where there is no token
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
+NEXAR_D void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> NEXAR_D void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // Four 8 x 8 fragments stored transposed; lane l gives the address of row l % 8 of matrix l / 8.
 NEXAR_D void stsm4t(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};"
@@ -89,13 +87,31 @@ NEXAR_D float bf_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 NEXAR_D uint32_t tile_at(int r, int g) { return (uint32_t)((g >> 3) * 8192 + r * 128 + (((g & 7) ^ (r & 7)) << 4)); }
 // MN-major operand: boxes of 64 contiguous MN elements x 64 K rows, 8 KB apart.
 NEXAR_D uint64_t desc_mn(uint32_t addr) { return umma_desc_sw128_mnmajor(addr); }
-// kind::f16 MMA whose A operand is read from tensor memory.
-NEXAR_D void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// tcgen05.mma and commit by the elected lane of a converged warp (always the same one). With the election inside,
+// the operands stay in uniform registers: 32 products of 64 x 64 x 16 take 1120 cycles instead of the 1570 that one
+// lane in a branch of its own needs, and the first four 375 instead of 660.
+NEXAR_D void warp_mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+NEXAR_D void warp_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       :: "r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+NEXAR_D void warp_commit(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      :: "r"(smem_u32(bar)) : "memory");
 }
 NEXAR_D void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
@@ -124,28 +140,17 @@ NEXAR_D void tmem_st_frag(uint32_t taddr, const uint32_t (&r)[16]) {
 }
 NEXAR_D void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Bounded wait of a whole warp: one lane polls, then every lane sees the completed
-// phase itself (a phase that is usually complete costs one test).
-NEXAR_D bool wait_phase(uint64_t* bar, uint32_t parity, int lane) {
+// Bounded wait by polling: these waits sit on the chunk's critical path.
+NEXAR_D bool wait_phase(uint64_t* bar, uint32_t parity) {
   if (mbar_try_wait(bar, parity)) return true;
-  int ok = 1;
-  if (lane == 0) {
-    const unsigned long long t0 = globaltimer_ns();
-    bool got = false;
-    while (!got && ok) {
+  const unsigned long long t0 = globaltimer_ns();
+  while (true) {
 #pragma unroll 1
-      for (int i = 0; i < 64 && !got; ++i) got = mbar_try_wait(bar, parity);
-      if (!got && globaltimer_ns() - t0 > kDecayWaitNs) ok = 0;
-    }
+    for (int i = 0; i < 256; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (globaltimer_ns() - t0 > kDecayWaitNs) return false;
   }
-  ok = __shfl_sync(0xffffffffu, ok, 0);
-  if (ok) mbar_try_wait(bar, parity);
-  return ok != 0;
 }
-
-struct DecayMaps {
-  CUtensorMap in[4];
-};
 
 template <int D, bool STATES> struct Shape {
   static constexpr int kThreads = 256;             // two warps per TMEM lane quarter share its columns
@@ -164,7 +169,7 @@ template <int D, bool STATES> struct Shape {
 
 template <int D, bool STATES>
 __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::kBlocks)
-    k_decay_chunk(const __grid_constant__ DecayArgs a, const __grid_constant__ DecayMaps maps) {
+    k_decay_chunk(const __grid_constant__ DecayArgs a) {
   using S = Shape<D, STATES>;
   extern __shared__ __align__(1024) unsigned char smem[];
   const DecayRole& R = a.role[blockIdx.z];
@@ -176,39 +181,45 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
   const int t_end = min(a.T, t_begin + a.seg_tokens);   // index i, counted from the first token of the direction
   const int live = max(0, min(len, t_end) - t_begin);   // tokens of this segment that exist
   const int nchunks = (live + kChunk - 1) / kChunk;
-  const bool rev = R.reverse != 0;
 
   float* pw = reinterpret_cast<float*>(smem + S::kMisc);  // lam^0 .. lam^64, then what the rounding of lam^64 leaves out:
                                                           // over hundreds of chunks that error would add up
-  uint64_t* done = reinterpret_cast<uint64_t*>(smem + S::kMisc + 320);  // second group of products
-  uint64_t* s_done = done + 1;                                          // first group
-  uint64_t* full = done + 2;                                            // [stage] tiles
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kMisc + 352);
+  uint64_t* done = reinterpret_cast<uint64_t*>(smem + S::kMisc + 320);
+  uint64_t* s_done = done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kMisc + 336);
   const uint32_t base = smem_u32(smem);
 
-  // Row r of chunk c's tiles is token first_row(c) + r: index 64 c + r of the segment, or (reversed) 64 c + 63 - r.
-  const auto first_row = [&](int c) { return rev ? len - t_begin - (c + 1) * kChunk : t_begin + c * kChunk; };
-  // The loads of chunk c's tiles from w0 to w1 (of q, k, v; STATES: k, v), by one thread; rows outside the tensor are
-  // filled with zeros. The first call of a chunk announces all its bytes.
-  const auto load = [&](int c, int w0, int w1) {
-    const int s = S::kStages == 2 ? c & 1 : 0, t0 = first_row(c);
-    const uint32_t dst = base + s * S::kTiles * S::kTile;
-    if (w0 == 0) mbar_arrive_expect_tx(full + s, S::kTiles * S::kTile);
-    for (int w = w0; w < w1; ++w) {
-      const int which = STATES ? w + 1 : w;
-      const CUtensorMap* m = &maps.in[which == 0 ? R.q : which == 1 ? R.k : R.v];
+  // A thread moves 16-byte group g0 of rows r0, r0 + kRows, ... of every tile. Token index i sits at row i, or at
+  // len - 1 - i when the direction is reversed.
+  constexpr int kGroups = D / 8, kRows = S::kThreads / kGroups, kPasses = kChunk / kRows;
+  const int r0 = tid / kGroups, g0 = tid % kGroups;
+  const uint32_t at0 = tile_at(r0, g0);  // + 128 kRows bytes for kRows rows more
+  const int dir = R.reverse ? -1 : 1, origin = R.reverse ? len - 1 : 0;
+  auto prefetch = [&](int c, int w0 = 0, int w1 = S::kTiles) {  // tiles w0 .. w1 - 1 (of q, k, v; STATES: k, v)
+    const int left = live - c * kChunk - r0;
+    const long long t = origin + dir * (t_begin + c * kChunk + r0);
+    const uint32_t dst = base + (S::kStages == 2 ? (c & 1) * S::kTiles * S::kTile : 0) + at0;
 #pragma unroll
-      for (int x = 0; x < D; x += 64) tma_load_rows(dst + w * S::kTile + (x >> 6) * 8192, m, full + s, x, h, t0, b);
+    for (int w = 0; w < S::kTiles; ++w) {
+      if (w < w0 || w >= w1) continue;
+      const int which = STATES ? w + 1 : w;
+      const long long st = which == 0 ? R.qt : which == 1 ? R.kt : R.vt;
+      const __nv_bfloat16* src = (which == 0 ? R.q + b * R.qb + h * R.qh
+                                  : which == 1 ? R.k + b * R.kb + h * R.kh : R.v + b * R.vb + h * R.vh) + t * st + g0 * 8;
+#pragma unroll
+      for (int u = 0; u < kPasses; ++u) {
+        const bool there = kRows * u < left;
+        cp_async16(dst + w * S::kTile + u * kRows * 128, there ? src + u * (dir * kRows * st) : R.k, there);
+      }
     }
+    cp_commit();
   };
+  if (nchunks > 0) prefetch(0);
+
   if (tid == 0) {
     mbar_init(done, 1);
     mbar_init(s_done, 1);
-    mbar_init(full, 1);
-    mbar_init(full + 1, 1);
     mbar_fence_init();
-    if (nchunks > 0) load(0, 0, S::kTiles);
-    if (S::kStages == 2 && nchunks > 1) load(1, 0, S::kTiles);
   }
   if (warp == 0) {
     tmem_alloc(tmem_slot, S::kCols);
@@ -217,6 +228,10 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
   if (tid <= kChunk + 1) {
     const double g = (double)a.log_decay[h], p = tid == 0 ? 1.0 : exp(g * min(tid, kChunk));
     pw[tid] = tid <= kChunk ? (float)p : (float)(p - (double)(float)p);
+  }
+  if constexpr (!STATES && D == 128) {  // the blocks of P above the diagonal stay zero
+    for (int e = tid; e < 1024; e += S::kThreads)
+      reinterpret_cast<uint4*>(smem + S::kScores)[e] = make_uint4(0, 0, 0, 0);
   }
 
   // ---- state. D = 64: fragments of X, rows dk = xr (+ 8), columns dv = 32 half + 8 n + xc (+ 1). D = 128: row dv of
@@ -248,27 +263,17 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
   for (int n = 0; n < kX; ++n) X[n] = !x0 ? 0.f : x0[x0_t ? x_at_t(n) : x_at(n)];
   bool have = x0 != nullptr;  // a state that is known to be zero is not multiplied
   const bool want_final = STATES || (R.final_state != nullptr && a.nseg == 1);
-  const int shift = rev ? 0 : 1;  // exponents: i + shift and n - shift - j
+  const int shift = R.reverse ? 0 : 1;  // exponents: i + shift and n - shift - j
 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tbase = *tmem_slot;
+  const uint32_t tbase = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const uint32_t lanes = tbase + ((uint32_t)(quarter * 32) << 16);
-  constexpr int kGroups = D / 8, kRows = S::kThreads / kGroups, kPasses = kChunk / kRows;
-  const int r0 = tid / kGroups, g0 = tid % kGroups;  // 16-byte group g0 of rows r0, r0 + kRows, ... of a tile
-  const uint32_t at0 = tile_at(r0, g0);              // + 128 kRows bytes for kRows rows more
   bool ok = true;
-  int seen = 0;  // chunks whose loads were waited for
-  const bool ctl = warp == (rev ? 3 : 4) && lane == 0;  // issues products and loads: no scores of this warp are kept
-  const auto give_up = [&]() {
-    ok = false;
-    if (lane == 0) atomicExch(&g_decay_error, 1u);
-  };
 
   for (int c = 0; c < nchunks; ++c) {
     const int n_tok = min(kChunk, live - c * kChunk);
-    const int lo = rev ? kChunk - n_tok : 0, hi = rev ? kChunk : n_tok;  // rows [lo, hi) are tokens of this chunk
     const uint32_t stage = S::kStages == 2 ? (c & 1) * S::kTiles * S::kTile : 0;
     const uint32_t tq = base + stage, tk = tq + (STATES ? 0 : S::kTile), tv = tk + S::kTile;
     const bool update = want_final || c + 1 < nchunks;
@@ -276,31 +281,30 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
       if (have) {  // ---- the state as an operand: two bf16 parts
 #pragma unroll
         for (int n = 0; n < kX; n += 2) {
-          const uint32_t hi_ = bf2(X[n], X[n + 1]), lo_ = bf2(X[n] - bf_lo(hi_), X[n + 1] - bf_hi(hi_));
+          const uint32_t hi = bf2(X[n], X[n + 1]), lo = bf2(X[n] - bf_lo(hi), X[n + 1] - bf_hi(hi));
           unsigned char* at = smem + S::kScores + tile_at(xr + (n & 2) * 4, half * 4 + (n >> 2)) + xc * 2;
-          *reinterpret_cast<uint32_t*>(at) = hi_;
-          *reinterpret_cast<uint32_t*>(at + 8192) = lo_;
+          *reinterpret_cast<uint32_t*>(at) = hi;
+          *reinterpret_cast<uint32_t*>(at + 8192) = lo;
         }
-        fence_proxy_async_smem();
       }
     }
-    // The state is written (D = 64); everyone has read U and the output. All leave together if a wait gave up.
+    cp_wait<0>();
+    fence_proxy_async_smem();
+    // tiles (D = 64: and the state) are visible; everyone has read U and the output, and all leave together if a wait gave up
     if (!__syncthreads_and(ok)) {
       ok = false;
       break;
     }
-    if (!wait_phase(full + (S::kStages == 2 ? c & 1 : 0), (S::kStages == 2 ? c >> 1 : c) & 1, lane)) give_up();
-    else seen = c + 1;
     // K steps of 16 in the descriptors: 32 bytes along a K-major row (+ 2; the next box of 64 is + 512), 16 rows of
-    // an MN-major box (+ 128), 8 columns of a TMEM operand. Small parts first.
+    // an MN-major box (+ 128), 8 columns of a TMEM operand.
     if constexpr (!STATES) {
-      if (ctl) {
+      if (__shfl_sync(0xffffffffu, warp, 0) == 4) {
         tc_fence_after();
         const uint64_t kq = umma_desc_sw128_kmajor(tq), kk = umma_desc_sw128_kmajor(tk);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t o = (k >> 2) * 512 + (k & 3) * 2;
-          umma_f16(tbase + (D == 64 ? 0 : 128), kq + o, kk + o, umma_idesc_bf16_f32(64, 64), k > 0);
+          warp_mma(tbase + (D == 64 ? 0 : D), kq + o, kk + o, umma_idesc_bf16_f32(64, 64), k > 0);
         }
         if (D == 64 && have) {
           const uint64_t mx = desc_mn(base + S::kScores);
@@ -308,24 +312,25 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
           for (int p = 1; p >= 0; --p)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_f16(tbase + 64, kq + k * 2, mx + p * 512 + 128 * k, umma_idesc_bf16_f32(64, 64, false, true), p == 0 || k > 0);
+              warp_mma(tbase + 64, kq + k * 2, mx + p * 512 + 128 * k, umma_idesc_bf16_f32(64, 64, false, true), p == 0 || k > 0);
         }
-        umma_commit(s_done);
+        warp_commit(s_done);
       }
       __syncwarp();
+    }
+    if constexpr (S::kStages == 2) {
+      if (c + 1 < nchunks) prefetch(c + 1);
     }
     if (update) {  // ---- keys decayed to the chunk's end, in bf16 parts
 #pragma unroll
       for (int u = 0; u < kPasses; ++u) {
-        const int r = r0 + kRows * u;
         const uint4 raw = *reinterpret_cast<const uint4*>(smem + (tk - base) + at0 + u * kRows * 128);
         const uint32_t kw[4] = {raw.x, raw.y, raw.z, raw.w};
-        const bool there = r >= lo && r < hi;
-        const float w = R.kv * pw[there ? (rev ? n_tok - 63 + r : n_tok - 1 - r) : 0];
+        const float w = R.kv * pw[max(n_tok - shift - r0 - kRows * u, 0)];  // rows behind the last token are zero
         uint32_t p0[4], p1[4], p2[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float x = there ? bf_lo(kw[q]) * w : 0.f, y = there ? bf_hi(kw[q]) * w : 0.f;
+          const float x = bf_lo(kw[q]) * w, y = bf_hi(kw[q]) * w;
           p0[q] = bf2(x, y);
           const float x1 = x - bf_lo(p0[q]), y1 = y - bf_hi(p0[q]);
           p1[q] = bf2(x1, y1);
@@ -337,134 +342,146 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
         *reinterpret_cast<uint4*>(dst + 2 * S::kTile) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
       }
     }
-    if (n_tok < kChunk && a.lengths) {  // rows of v behind the last token may hold anything: P and K' are zero there
-#pragma unroll
-      for (int u = 0; u < kPasses; ++u) {
-        const int r = r0 + kRows * u;
-        if (r < lo || r >= hi)
-          *reinterpret_cast<uint4*>(smem + (tv - base) + at0 + u * kRows * 128) = make_uint4(0, 0, 0, 0);
-      }
-    }
-    if constexpr (!STATES && D == 128) {
-      if (have) {  // ---- the state as an operand: two bf16 parts
-#pragma unroll
-        for (int n = 0; n < kX; n += 32) {
-          uint32_t hi_[16], lo_[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float x = X[n + 2 * e], y = X[n + 2 * e + 1];
-            hi_[e] = bf2(x, y);
-            lo_[e] = bf2(x - bf_lo(hi_[e]), y - bf_hi(hi_[e]));
-          }
-          tmem_st_x16(lanes + half * 32 + n / 2, hi_);
-          tmem_st_x16(lanes + 64 + half * 32 + n / 2, lo_);
-        }
-        tmem_st_wait();
-      }
-    }
     if constexpr (!STATES) {
+      if (D == 128 && have) {  // ---- the state as an operand: two bf16 parts
+        if constexpr (D == 128) {
+#pragma unroll
+          for (int n = 0; n < kX; n += 32) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float x = X[n + 2 * e], y = X[n + 2 * e + 1];
+              hi[e] = bf2(x, y);
+              lo[e] = bf2(x - bf_lo(hi[e]), y - bf_hi(hi[e]));
+            }
+            tmem_st_x16(lanes + half * 32 + n / 2, hi);
+            tmem_st_x16(lanes + 64 + half * 32 + n / 2, lo);
+          }
+          tmem_st_wait();
+        }
+      }
       // ---- P: 16 query rows and 32 key columns per warp, up to the diagonal
-      if (!wait_phase(s_done, c & 1, lane)) give_up();
+      if (!wait_phase(s_done, c & 1)) {
+        ok = false;
+        if (lane == 0) atomicExch(&g_decay_error, 1u);
+      }
       tc_fence_after();
-      uint32_t sc[16], o[16];
-      const bool some = rev ? half * 2 + 1 >= quarter : half * 2 <= quarter, scaled = D == 64 && have;
-      if (some) tmem_ld_frag(lanes + (D == 64 ? 0 : 128) + half * 32, sc);
-      if (scaled) tmem_ld_frag(lanes + 64 + half * 32, o);
-      tmem_ld_wait();
-      if (scaled) {  // Q X -> inter lam^(i + shift) Q X, in place
-        const float f0 = R.inter * pw[rev ? 63 - xr : xr + 1], f1 = R.inter * pw[rev ? 55 - xr : xr + 9];
+      if (D == 64 && have) {  // Q X -> inter lam^(i + shift) Q X, in place
+        uint32_t o[16];
+        tmem_ld_frag(lanes + 64 + half * 32, o);
+        const float f0 = R.inter * pw[xr + shift], f1 = R.inter * pw[xr + 8 + shift];  // xr: here a token
+        tmem_ld_wait();
 #pragma unroll
         for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * (n & 2 ? f1 : f0));
         tmem_st_frag(lanes + 64 + half * 32, o);
       }
-      // the part of the power that belongs to this thread's four key columns inside a block of 16
-      const int c0 = rev ? xc : 15 - xc, cs = rev ? 1 : -1;
-      const float cf[4] = {pw[c0], pw[c0 + cs], pw[c0 + 8 * cs], pw[c0 + 9 * cs]};
+      if (D == 64) {  // above the diagonal, where the state's parts were
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const int kb = half * 2 + m;
-        float P[2][4];
-        if (kb == quarter) {
+        for (int m = 0; m < 2; ++m)
+          if (half * 2 + m > quarter) {
+            unsigned char* at = smem + S::kScores + tile_at(quarter * 16 + (lane & 15), 4 * half + 2 * m + (lane >> 4));
+            *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(at + 8192) = make_uint4(0, 0, 0, 0);
+          }
+      }
+      if (half * 2 <= quarter && quarter * 16 < n_tok) {
+        uint32_t sc[16];
+        tmem_ld_frag(lanes + (D == 64 ? 0 : D) + half * 32, sc);
+        // lam^15-jj of this thread's four key columns inside a block of 16
+        const float cf[4] = {pw[15 - xc], pw[14 - xc], pw[7 - xc], pw[6 - xc]};
+        tmem_ld_wait();
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const int kb = half * 2 + m;
+          if (kb > quarter) continue;
+          float P[2][4];
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int ahead = (lane >> 2) + (e >> 1) * 8 - (n * 8 + xc + (e & 1)), gap = rev ? -ahead : ahead;
-              P[n][e] = gap >= 0 ? __uint_as_float(sc[m * 8 + n * 4 + e]) * (R.intra * pw[max(gap, 0)]) : 0.f;
+            for (int e = 0; e < 4; ++e) P[n][e] = __uint_as_float(sc[m * 8 + n * 4 + e]);
+          if (kb < quarter) {
+            const float f0 = R.intra * pw[xr - kb * 16 - 15], f1 = R.intra * pw[xr + 8 - kb * 16 - 15];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              P[n][0] *= f0 * cf[2 * n], P[n][1] *= f0 * cf[2 * n + 1];
+              P[n][2] *= f1 * cf[2 * n], P[n][3] *= f1 * cf[2 * n + 1];
             }
-        } else if ((kb < quarter) != rev) {
-          const int e0 = rev ? kb * 16 - xr : xr - kb * 16 - 15;
-          const float f0 = R.intra * pw[e0], f1 = R.intra * pw[rev ? e0 - 8 : e0 + 8];
+          } else {
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const uint32_t* v = sc + m * 8 + n * 4;
-            P[n][0] = __uint_as_float(v[0]) * (f0 * cf[2 * n]), P[n][1] = __uint_as_float(v[1]) * (f0 * cf[2 * n + 1]);
-            P[n][2] = __uint_as_float(v[2]) * (f1 * cf[2 * n]), P[n][3] = __uint_as_float(v[3]) * (f1 * cf[2 * n + 1]);
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int gap = (lane >> 2) + (e >> 1) * 8 - (n * 8 + xc + (e & 1));
+                P[n][e] = gap >= 0 ? P[n][e] * (R.intra * pw[max(gap, 0)]) : 0.f;
+              }
           }
-        } else {
 #pragma unroll
-          for (int n = 0; n < 2; ++n) P[n][0] = P[n][1] = P[n][2] = P[n][3] = 0.f;
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              const float u = P[n][2 * p], v = P[n][2 * p + 1];
+              const uint32_t hi = bf2(u, v), lo = bf2(u - bf_lo(hi), v - bf_hi(hi));
+              unsigned char* at = smem + S::kScores + tile_at(xr + 8 * p, 2 * kb + n) + xc * 2;
+              *reinterpret_cast<uint32_t*>(at) = hi;
+              *reinterpret_cast<uint32_t*>(at + 8192) = lo;
+            }
         }
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            const float u = P[n][2 * p], v = P[n][2 * p + 1];
-            const uint32_t hi_ = bf2(u, v), lo_ = bf2(u - bf_lo(hi_), v - bf_hi(hi_));
-            unsigned char* at = smem + S::kScores + tile_at(xr + 8 * p, 2 * kb + n) + xc * 2;
-            *reinterpret_cast<uint32_t*>(at) = hi_;
-            *reinterpret_cast<uint32_t*>(at + 8192) = lo_;
-          }
       }
-      if (D == 64) tmem_st_wait();
     }
+    if (!STATES && D == 64) tmem_st_wait();
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
-    const bool more = c + S::kStages < nchunks;
-    if (ctl) {
+    if (__shfl_sync(0xffffffffu, warp, 0) == 4) {  // small parts first
       tc_fence_after();
       const uint64_t mv = desc_mn(tv);
       if constexpr (!STATES) {
+        constexpr uint32_t id1 = umma_idesc_bf16_f32(D, 64, D == 128, D == 64);
+        const uint64_t kp = umma_desc_sw128_kmajor(base + S::kScores);
         if (D == 128 && have) {
           const uint64_t kq = umma_desc_sw128_kmajor(tq);
 #pragma unroll
           for (int p = 1; p >= 0; --p)
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
-              umma_ts(tbase + 192, tbase + p * 64 + k * 8, kq + (k >> 2) * 512 + (k & 3) * 2, umma_idesc_bf16_f32(D, 64),
-                      p == 0 || k > 0);
+              warp_mma_ts(tbase + D + 64, tbase + p * 64 + k * 8, kq + (k >> 2) * 512 + (k & 3) * 2,
+                          umma_idesc_bf16_f32(D, 64), p == 0 || k > 0);
         }
-        const uint64_t kp = umma_desc_sw128_kmajor(base + S::kScores);
 #pragma unroll
         for (int p = 1; p >= 0; --p)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t acc = p == 0 || k > 0;
             if constexpr (D == 64)
-              umma_f16(tbase + 64, kp + p * 512 + k * 2, mv + 128 * k, umma_idesc_bf16_f32(64, 64, false, true), acc || have);
+              warp_mma(tbase + 64, kp + p * 512 + k * 2, mv + 128 * k, id1, p == 0 || k > 0 || have);
             else
-              umma_f16(tbase + 128, mv + 128 * k, kp + p * 512 + k * 2, umma_idesc_bf16_f32(D, 64, true, false), acc);
+              warp_mma(tbase + D, mv + 128 * k, kp + p * 512 + k * 2, id1, p == 0 || k > 0);
           }
       }
-      if (update) {  // D = 128: behind the products that read X^T, whose columns U takes
+      if (update) {  // behind the products that read X^T, whose columns U takes
+        constexpr uint32_t idu = umma_idesc_bf16_f32(D, D, true, true);
         const uint64_t mk = desc_mn(base + S::kKeys);
 #pragma unroll
         for (int p = 2; p >= 0; --p)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint64_t part = mk + p * (S::kTile >> 4) + 128 * k;
-            umma_f16(tbase, D == 64 ? part : mv + 128 * k, D == 64 ? mv + 128 * k : part,
-                     umma_idesc_bf16_f32(D, D, true, true), p < 2 || k > 0);
+            warp_mma(tbase, D == 64 ? part : mv + 128 * k, D == 64 ? mv + 128 * k : part, idu, p < 2 || k > 0);
           }
       }
-      umma_commit(done);
-      if (!STATES && D == 64 && more) load(c + 1, 0, 2);  // nothing reads q and k any more
+      warp_commit(done);
     }
     __syncwarp();
-    if (!wait_phase(done, c & 1, lane)) give_up();
+    if constexpr (!STATES && D == 64) {
+      if (c + 1 < nchunks) prefetch(c + 1, 0, 2);  // nothing reads q and k any more
+    }
+    if (!wait_phase(done, c & 1)) {
+      ok = false;
+      if (lane == 0) atomicExch(&g_decay_error, 1u);
+    }
     tc_fence_after();
-    if (ctl && more) load(c + S::kStages, !STATES && D == 64 ? 2 : 0, S::kTiles);
+    if constexpr (S::kStages == 1) {
+      if (c + 1 < nchunks && ok) prefetch(c + 1, D == 64 ? 2 : 0, 3);
+    }
     if (update) {
       const float keep = pw[n_tok], rest = n_tok == kChunk ? pw[kChunk + 1] : 0.f;
 #pragma unroll
@@ -475,16 +492,17 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
-          float s0 = X[n + e], s1 = X[n + e + 1];
-          fma2(s0, s1, rest, __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
-          fma2(X[n + e], X[n + e + 1], keep, s0, s1);
+          float r0_ = X[n + e], r1_ = X[n + e + 1];
+          fma2(r0_, r1_, rest, __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
+          fma2(X[n + e], X[n + e + 1], keep, r0_, r1_);
         }
       }
     }
     if constexpr (!STATES) {
       // ---- the output, through the keys' space so that whole 16-byte groups are stored
       unsigned char* o_tile = smem + S::kKeys;
-      __nv_bfloat16* out = R.out + b * R.ob + h * R.oh + (long long)first_row(c) * R.ot;
+      const long long row = origin + dir * (t_begin + c * kChunk);
+      __nv_bfloat16* out = R.out + b * R.ob + h * R.oh;
       if constexpr (D == 64) {
         uint32_t o[16];
         tmem_ld_frag(lanes + 64 + half * 32, o);
@@ -497,20 +515,18 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int r = quarter * 16 + u * 8 + (lane >> 2), g = half * 4 + (lane & 3);
-          if (r >= lo && r < hi)
-            *reinterpret_cast<uint4*>(out + r * R.ot + g * 8) = *reinterpret_cast<const uint4*>(o_tile + tile_at(r, g));
+          if (r < n_tok)
+            *reinterpret_cast<uint4*>(out + (row + dir * r) * R.ot + g * 8) =
+                *reinterpret_cast<const uint4*>(o_tile + tile_at(r, g));
         }
       } else {
         // fragments of 16 value rows x 8 tokens, stored transposed
         float f[8];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const int r = half * 32 + (n >> 1) * 8 + xc + (n & 1);
-          f[n] = have ? R.inter * pw[rev ? 63 - r : r + 1] : 0.f;
-        }
+        for (int n = 0; n < 8; ++n) f[n] = have ? R.inter * pw[half * 32 + (n >> 1) * 8 + xc + (n & 1) + shift] : 0.f;
 #pragma unroll
         for (int hl = 0; hl < 2; ++hl) {
-          const uint32_t from = lanes + ((uint32_t)(hl * 16) << 16) + 128 + half * 32;
+          const uint32_t from = lanes + ((uint32_t)(hl * 16) << 16) + D + half * 32;
           uint32_t o1[16], o2[16], w[8];
           tmem_ld_frag(from, o1);
           if (have) tmem_ld_frag(from + 64, o2);
@@ -530,13 +546,12 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
             stsm4t(smem_u32(o_tile) + tile_at(t, g), w[2 * n], w[2 * n + 1], w[2 * n + 2], w[2 * n + 3]);
           }
         }
-        tc_fence_before();
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < kPasses; ++u) {
           const int r = r0 + kRows * u;
-          if (r >= lo && r < hi)
-            *reinterpret_cast<uint4*>(out + r * R.ot + g0 * 8) =
+          if (r < n_tok)
+            *reinterpret_cast<uint4*>(out + (row + dir * r) * R.ot + g0 * 8) =
                 *reinterpret_cast<const uint4*>(o_tile + at0 + u * kRows * 128);
         }
       }
@@ -557,8 +572,7 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
 #pragma unroll
     for (int n = 0; n < kX; ++n) dst[x_at(n)] = X[n];
   }
-  for (int c = seen; c < min(nchunks, seen + S::kStages); ++c)  // no load may still be landing when the block exits
-    wait_phase(full + (S::kStages == 2 ? c & 1 : 0), (S::kStages == 2 ? c >> 1 : c) & 1, lane);
+  cp_wait<0>();
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
@@ -666,34 +680,28 @@ template <int D> __global__ void __launch_bounds__(D * 2) k_decay_step(const Dec
 }
 
 template <int D, bool STATES>
-cudaError_t launch_chunks(const DecayArgs& a, const DecayMaps& maps, int roles, cudaStream_t s) {
+cudaError_t launch_chunks(const DecayArgs& a, int roles, cudaStream_t s) {
   using S = Shape<D, STATES>;
   const cudaError_t e =
       cudaFuncSetAttribute(k_decay_chunk<D, STATES>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
-  k_decay_chunk<D, STATES><<<dim3(a.B * a.H, a.nseg, roles), S::kThreads, S::kSmem, s>>>(a, maps);
+  k_decay_chunk<D, STATES><<<dim3(a.B * a.H, a.nseg, roles), S::kThreads, S::kSmem, s>>>(a);
   return cudaGetLastError();
 }
 
 template <int D> cudaError_t decay_typed(const DecayArgs& a, cudaStream_t s, int* launches) {
   *launches = 0;
-  DecayMaps maps;
-  for (int i = 0; i < a.nin; ++i) {
-    const DecayInput& t = a.in[i];
-    const cudaError_t e = make_tmap_bf16_heads(&maps.in[i], t.p, a.B, a.T, a.H, D, t.sb, t.st, t.sh);
-    if (e != cudaSuccess) return e;
-  }
   if (a.nseg > 1) {
     // roles that read another role's segment states come last and need no states of their own
     int own = 0;
     while (own < a.nroles && a.role[own].segments_from < 0) ++own;
-    const cudaError_t e = launch_chunks<D, true>(a, maps, own, s);
+    const cudaError_t e = launch_chunks<D, true>(a, own, s);
     if (e != cudaSuccess) return e;
     k_decay_scan<D><<<dim3(a.B * a.H, D * D / 1024, own), 256, 0, s>>>(a);
     *launches += 2;
   }
   *launches += 1;
-  return launch_chunks<D, false>(a, maps, a.nroles, s);
+  return launch_chunks<D, false>(a, a.nroles, s);
 }
 }  // namespace
 
@@ -703,25 +711,25 @@ unsigned int decay_error_flag() {
   return v;
 }
 
-// Two blocks per SM are resident. Whole sequences take `chunks` steps of a block,
-// n segments ceil(chunks / n) of the main kernel and of the state-only one, and two
-// more launches. In units of a main step with two blocks on the SM (3.3 us for D =
-// 64, 4.5 us for D = 128): a step of a block that has the SM to itself 0.75, a
-// state-only step 0.65, the two launches 2.5 (measured at B H = 96, T = 1024, D =
-// 64: 38 us whole, 42 us in 3 segments; at 16 heads of 128 and T = 16385, 18
-// segments take 152 us).
+// Whole sequences take `chunks` steps of a block that has its SM to itself (2.9 us
+// each for D = 64, 5.4 us for D = 128). n segments that fill every resident block
+// take ceil(chunks / n) steps of the main kernel beside its neighbours and of the
+// state-only one, 2.9 (D = 64) or 1.85 (D = 128) of those together, and the two
+// launches more 4.5 or 2.5. Measured whole / split, us: 12 heads of 64, T = 4096:
+// 184 / 33; 96 heads, T = 1024: 50 / 47; 60 heads, T = 1000: 49 / 37; 16 heads of
+// 128, T = 16385: 1386 / 165; 64 heads, T = 1024: 87 / 62; 128 heads: 93 / 102.
 int decay_segments(int B, int T, int H, int D, int roles) {
   const int chunks = (T + kChunk - 1) / kChunk;
-  const long long blocks = (long long)B * H * roles, slots = 148LL * 2;
-  const auto steps = [&](long long n) { return (double)((chunks + n - 1) / n); };
-  if (blocks * 2 > slots) return 1;
+  const long long blocks = (long long)B * H * roles, slots = 148LL * (D == 64 ? 3 : 2);
+  if (blocks > 148) return 1;
   const long long n = slots / blocks < chunks ? slots / blocks : chunks;
-  const double whole = chunks * (blocks <= 148 ? 0.75 : 1.0), split = steps(n) * 1.65 + 2.5;
-  return split < whole ? (int)n : 1;
+  const double steps = (double)((chunks + n - 1) / n);
+  const double split = D == 64 ? steps * 2.9 + 4.5 : steps * 1.85 + 2.5;
+  return split < chunks ? (int)n : 1;
 }
 
 cudaError_t decay_attention(const DecayArgs& a, cudaStream_t s, int* launches) {
-  if (a.nroles < 1 || a.nroles > 3 || a.nin < 1 || a.nin > 4 || a.B < 1 || a.H < 1 || a.T < 1 || (long long)a.B * a.H > 0x7fffffffLL || a.nseg > 65535 || a.nseg < 1 ||
+  if (a.nroles < 1 || a.nroles > 3 || a.B < 1 || a.H < 1 || a.T < 1 || (long long)a.B * a.H > 0x7fffffffLL || a.nseg > 65535 || a.nseg < 1 ||
       (long long)a.nseg * a.seg_tokens < a.T || (a.nseg > 1 && a.seg_tokens % kChunk))
     return cudaErrorInvalidValue;
   if (a.D == 64) return decay_typed<64>(a, s, launches);

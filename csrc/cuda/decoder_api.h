@@ -55,18 +55,13 @@ cudaError_t dropout_ln_bwd(const __nv_bfloat16* dy, const __nv_bfloat16* s_in, c
                            const int64_t* state, uint32_t site, uint32_t threshold, float scale, cudaStream_t s);
 
 // ---------------------------------------------------------------- decay attention
-// A [B, T, H, D] bf16 input: strides in elements, multiples of 8 and not 0, base 16-byte aligned.
-struct DecayInput {
-  const __nv_bfloat16* p;
-  long long sb, st, sh;
-};
 // One use of the chunked recurrence (see decay_attention.cu): out_i = intra *
 // sum_{j <= i} lam^(i-j) (q_i . k_j) v_j + inter * lam^(i+a) X q_i, tokens
 // taken from the first (reverse = 0) or the last (reverse = 1).
 struct DecayRole {
-  int q, k, v;              // which inputs
+  const __nv_bfloat16 *q, *k, *v;
   __nv_bfloat16* out;
-  long long ob, ot, oh;     // its strides
+  long long qb, qt, qh, kb, kt, kh, vb, vt, vh, ob, ot, oh;  // strides in elements
   int reverse;
   float intra, inter, kv;   // factors of the scores, of the state's part and of the state's update
   const float* init;        // [B, H, D, D] state before the first token, or null
@@ -76,8 +71,6 @@ struct DecayRole {
   int segments_from;        // index of the role whose segment states this one reads, transposed (-1: its own)
 };
 struct DecayArgs {
-  DecayInput in[4];
-  int nin;
   DecayRole role[3];
   int nroles;
   const float* log_decay;   // [H]

@@ -246,11 +246,10 @@ std::vector<at::Tensor> op_dropout_ln_bwd(const at::Tensor& dy, const at::Tensor
 }
 
 // ---------------------------------------------------------------- decay attention
-// A [B, T, H, D] view that a tensor map can describe (rows in 16-byte groups, no repeated rows), or a contiguous copy.
+// A [B, T, H, D] view whose rows the kernels can read in 16-byte groups, or a contiguous copy of it.
 at::Tensor row_view(const at::Tensor& t) {
   bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  for (int64_t i = 0; i + 1 < t.dim(); ++i)
-    ok = ok && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0 && t.stride(i) < (1LL << 38)));
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
   return ok ? t : t.contiguous();
 }
 void need_decay_input(const at::Tensor& t, const at::Tensor& q, const char* name) {
@@ -286,10 +285,9 @@ const int* decay_lengths(const OptTensor& lengths, const at::Tensor& q) {
               "nexar_b200: decay attention: lengths must be a contiguous int32 tensor of one value per sequence");
   return lengths->data_ptr<int>();
 }
-int add_in(DecayArgs& a, const at::Tensor& t) {  // the stride of a dimension of one element is free
-  const auto stride = [&](int i) { return t.size(i) > 1 ? (long long)t.stride(i) : (long long)t.size(-1); };
-  a.in[a.nin] = DecayInput{cbf(t), stride(0), stride(1), stride(2)};
-  return a.nin++;
+void set_in(const at::Tensor& t, const __nv_bfloat16*& p, long long& b, long long& tt, long long& h) {
+  p = cbf(t);
+  b = t.stride(0), tt = t.stride(1), h = t.stride(2);
 }
 void set_out(const at::Tensor& t, DecayRole& r) {
   r.out = mbf(t);
@@ -338,7 +336,9 @@ std::tuple<at::Tensor, OptTensor> op_decay_fwd(const at::Tensor& q_in, const at:
   DecayArgs a{};
   a.nroles = 1;
   DecayRole& r = a.role[0];
-  r.q = add_in(a, q), r.k = add_in(a, k), r.v = add_in(a, v);
+  set_in(q, r.q, r.qb, r.qt, r.qh);
+  set_in(k, r.k, r.kb, r.kt, r.kh);
+  set_in(v, r.v, r.vb, r.vt, r.vh);
   set_out(o, r);
   r.intra = r.inter = (float)scale;
   r.kv = 1.f;
@@ -378,23 +378,28 @@ OptTensor op_decay_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at:
   a.nroles = 3;
   const float sc = (float)scale;
   const float* ds = dstate ? dstate->data_ptr<float>() : nullptr;
-  const int iq = add_in(a, q), ik = add_in(a, k), iv = add_in(a, v), io = add_in(a, dO);
   DecayRole& rv = a.role[0];  // dv: state dS [q dim, do dim], last token to first
-  rv.q = ik, rv.k = iq, rv.v = io;
+  set_in(k, rv.q, rv.qb, rv.qt, rv.qh);
+  set_in(q, rv.k, rv.kb, rv.kt, rv.kh);
+  set_in(dO, rv.v, rv.vb, rv.vt, rv.vh);
   set_out(dv, rv);
   rv.reverse = 1, rv.intra = sc, rv.inter = 1.f, rv.kv = sc;
   rv.init = ds;
   rv.final_state = ds0 ? ds0->data_ptr<float>() : nullptr;
   rv.segments_from = -1;
   DecayRole& rq = a.role[1];  // dq: state S transposed, first token to last
-  rq.q = io, rq.k = iv, rq.v = ik;
+  set_in(dO, rq.q, rq.qb, rq.qt, rq.qh);
+  set_in(v, rq.k, rq.kb, rq.kt, rq.kh);
+  set_in(k, rq.v, rq.vb, rq.vt, rq.vh);
   set_out(dq, rq);
   rq.intra = rq.inter = sc, rq.kv = 1.f;
   rq.init = state ? state->data_ptr<float>() : nullptr;
   rq.init_transposed = 1;
   rq.segments_from = -1;
   DecayRole& rk = a.role[2];  // dk: dS transposed, last token to first
-  rk.q = iv, rk.k = io, rk.v = iq;
+  set_in(v, rk.q, rk.qb, rk.qt, rk.qh);
+  set_in(dO, rk.k, rk.kb, rk.kt, rk.kh);
+  set_in(q, rk.v, rk.vb, rk.vt, rk.vh);
   set_out(dk, rk);
   rk.reverse = 1, rk.intra = sc, rk.inter = 1.f, rk.kv = sc;
   rk.init = ds;

@@ -107,23 +107,6 @@ cudaError_t make_tmap_f32_3d(CUtensorMap* map, void* base, long long splits, lon
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-// 4-D bf16 tensor map over [B, T, H, D] with any outer strides (elements), box
-// 64 tokens x 64 columns of one head and sequence, 128-byte swizzle.
-cudaError_t make_tmap_bf16_heads(CUtensorMap* map, const void* base, long long B, long long T, long long H, long long D,
-                                 long long sb, long long st, long long sh) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return cudaErrorNotSupported;
-  if ((reinterpret_cast<uintptr_t>(base) & 15u) || sb % 8 || st % 8 || sh % 8) return cudaErrorInvalidValue;
-  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T, (cuuint64_t)B};
-  cuuint64_t strides[3] = {(cuuint64_t)sh * 2, (cuuint64_t)st * 2, (cuuint64_t)sb * 2};
-  cuuint32_t box[4] = {64, 1, 64, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
-}
-
 namespace {
 // out = act(sum_s part[s] + bias) (+ residual) (+ out if accumulate), fixed
 // summation order over the splits; 4 columns per thread.

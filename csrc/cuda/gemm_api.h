@@ -42,8 +42,6 @@ cudaError_t make_tmap_bf16(CUtensorMap* map, const void* base, long long rows, l
                            int box_rows, int box_cols);
 cudaError_t make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, int esize, const void* base, long long rows,
                          long long cols, long long ld, int box_rows, int box_cols);
-cudaError_t make_tmap_bf16_heads(CUtensorMap* map, const void* base, long long B, long long T, long long H, long long D,
-                                 long long sb, long long st, long long sh);
 
 // ---- fp8 (e4m3) block-scaled GEMM: C[M,N] = epi( sum_kb sa[m,kb] sb[n/128,kb] (A_kb . B_kb^T) )
 // A [M, K] e4m3 with 1x128 scales sa [M, ceil(K/128)] (fp32, row-major);
