@@ -56,10 +56,10 @@ cudaError_t xent_fwd_bwd(const __nv_bfloat16* logits, const int64_t* targets, fl
                          __nv_bfloat16* dlogits, int R, int V, int Vp, float grad_scale,
                          cudaStream_t s);
 
-// Token + position embedding: out[r] = wte[tok[r]] + wpe[r % T].
+// Token + position embedding: out[r] = wte[tok[r]] + wpe[r % T] (wpe null: the token's row alone).
 cudaError_t embed_fwd(const int64_t* tok, const __nv_bfloat16* wte, const __nv_bfloat16* wpe,
                       __nv_bfloat16* out, int R, int T, int C, cudaStream_t s);
-// dwte[tok[r]] += dout[r] (atomic); dwpe[t] = sum_b dout[b*T + t] (overwrites).
+// dwte[tok[r]] += dout[r] (atomic); dwpe[t] = sum_b dout[b*T + t] (overwrites; null: none).
 cudaError_t embed_bwd(const int64_t* tok, const __nv_bfloat16* dout, __nv_bfloat16* dwte,
                       __nv_bfloat16* dwpe, int B, int T, int C, cudaStream_t s);
 

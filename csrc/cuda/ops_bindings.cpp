@@ -147,28 +147,29 @@ void op_xent(const at::Tensor& logits, const at::Tensor& targets, const at::Tens
   count_launch(1);
 }
 
-void op_embed_fwd(const at::Tensor& tok, const at::Tensor& wte, const at::Tensor& wpe, const at::Tensor& out,
-                  int64_t T) {
+void op_embed_fwd(const at::Tensor& tok, const at::Tensor& wte, const c10::optional<at::Tensor>& wpe,
+                  const at::Tensor& out, int64_t T) {
   TORCH_CHECK(tok.scalar_type() == at::kLong && tok.is_contiguous(), "embed: tokens must be int64");
   need_bf16(wte, "wte");
-  need_bf16(wpe, "wpe");
+  if (wpe) need_bf16(*wpe, "wpe");
   need_bf16(out, "out");
   const int C = wte.size(-1);
   c10::cuda::CUDAGuard g(wte.get_device());
-  chk(embed_fwd(tok.data_ptr<int64_t>(), bf(wte), bf(wpe), bf(out), tok.numel(), (int)T, C, stream_of(wte)),
+  chk(embed_fwd(tok.data_ptr<int64_t>(), bf(wte), bfc(wpe), bf(out), tok.numel(), (int)T, C, stream_of(wte)),
       "embed_fwd");
   count_launch(1);
 }
-void op_embed_bwd(const at::Tensor& tok, const at::Tensor& dout, const at::Tensor& dwte, const at::Tensor& dwpe,
-                  int64_t B, int64_t T) {
+void op_embed_bwd(const at::Tensor& tok, const at::Tensor& dout, const at::Tensor& dwte,
+                  const c10::optional<at::Tensor>& dwpe, int64_t B, int64_t T) {
   need_bf16(dout, "dout");
   need_bf16(dwte, "dwte");
-  need_bf16(dwpe, "dwpe");
+  if (dwpe) need_bf16(*dwpe, "dwpe");
   const int C = dout.size(-1);
   c10::cuda::CUDAGuard g(dout.get_device());
-  chk(embed_bwd(tok.data_ptr<int64_t>(), bf(dout), bf(dwte), bf(dwpe), (int)B, (int)T, C, stream_of(dout)),
+  chk(embed_bwd(tok.data_ptr<int64_t>(), bf(dout), bf(dwte), dwpe ? bf(*dwpe) : nullptr, (int)B, (int)T, C,
+                stream_of(dout)),
       "embed_bwd");
-  count_launch(2);
+  count_launch(dwpe ? 2 : 1);
 }
 
 int64_t op_grad_norm_blocks(int64_t n) { return grad_norm_blocks(n); }

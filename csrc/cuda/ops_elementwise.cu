@@ -122,9 +122,11 @@ __global__ void __launch_bounds__(kEwThreads) k_embed_fwd(const int64_t* __restr
     const long long t = tok[r];
     float a[8], b[8];
     ld8f(wte + t * C + c, a);
-    ld8f(wpe + (r % T) * C + c, b);
+    if (wpe) {
+      ld8f(wpe + (r % T) * C + c, b);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) a[e] += b[e];
+      for (int e = 0; e < 8; ++e) a[e] += b[e];
+    }
     st8f(out + r * C + c, a);
   }
 }
@@ -206,7 +208,7 @@ cudaError_t embed_bwd(const int64_t* tok, const __nv_bfloat16* dout, __nv_bfloat
   if (C % 8) return cudaErrorInvalidValue;
   const int R = B * T;
   k_embed_bwd_wte<<<ew_grid((long long)R * C / 2), kEwThreads, 0, s>>>(tok, dout, dwte, R, C);
-  k_embed_bwd_wpe<<<ew_grid((long long)T * C / 8), kEwThreads, 0, s>>>(dout, dwpe, B, T, C);
+  if (dwpe) k_embed_bwd_wpe<<<ew_grid((long long)T * C / 8), kEwThreads, 0, s>>>(dout, dwpe, B, T, C);
   return cudaGetLastError();
 }
 

@@ -15,6 +15,15 @@ head is the tied embedding GEMM followed by the fused softmax-cross-entropy
 kernel that writes its gradient in place of the logits. Weight gradients
 are stored straight into the flat gradient buffer (no zero-fill, no
 per-parameter accumulation).
+
+Options of the configuration, all off by default: ``positions="rotary"`` turns
+queries and keys (``ops.rotary`` on the packed projection) instead of adding a
+learned position embedding; ``dropout`` drops elements of the embedding and of
+both residual branches with the counter-based generator (no stored masks; the
+residual ones run inside the LayerNorm kernels); ``mixer="decay"`` replaces the
+softmax attention with ``ops.decay_attention_qkv`` (a fixed decay per head, 1 -
+2^-(5 + head)) and normalises each head's output (LayerNorm over the head, shared
+by the heads of a layer).
 """
 from __future__ import annotations
 
@@ -39,6 +48,9 @@ class GPT2Config:
     padded_vocab: int = 50304
     block_size: int = 1024
     ln_eps: float = 1e-5
+    dropout: float = 0.0
+    positions: str = "learned"   # or "rotary"
+    mixer: str = "attention"     # or "decay"
 
     @staticmethod
     def small() -> "GPT2Config":
@@ -52,12 +64,18 @@ class GPT2Config:
 def param_specs(cfg: GPT2Config) -> List[Tuple[str, Tuple[int, ...], bool]]:
     """(name, shape, weight_decay) in forward-use order."""
     C, Vp = cfg.n_embd, cfg.padded_vocab
-    specs = [("wte", (Vp, C), True), ("wpe", (cfg.block_size, C), True)]
+    specs = [("wte", (Vp, C), True)]
+    if cfg.positions == "learned":
+        specs.append(("wpe", (cfg.block_size, C), True))
     for l in range(cfg.n_layer):
         p = f"h{l}."
         specs += [
             (p + "ln1.w", (C,), False), (p + "ln1.b", (C,), False),
             (p + "attn.w", (3 * C, C), True), (p + "attn.b", (3 * C,), False),
+        ]
+        if cfg.mixer == "decay":
+            specs += [(p + "head_norm.w", (C // cfg.n_head,), False), (p + "head_norm.b", (C // cfg.n_head,), False)]
+        specs += [
             (p + "proj.w", (C, C), True), (p + "proj.b", (C,), False),
             (p + "ln2.w", (C,), False), (p + "ln2.b", (C,), False),
             (p + "fc.w", (4 * C, C), True), (p + "fc.b", (4 * C,), False),
@@ -71,6 +89,15 @@ class GPT2(torch.nn.Module):
     def __init__(self, cfg: GPT2Config, device, grad_alloc=None, seed: int = 0,
                  own_attention: Optional[bool] = None):
         super().__init__()
+        if cfg.positions not in ("learned", "rotary"):
+            raise ValueError(f"unknown positions {cfg.positions!r} (learned, rotary)")
+        if cfg.mixer not in ("attention", "decay"):
+            raise ValueError(f"unknown mixer {cfg.mixer!r} (attention, decay)")
+        if not 0.0 <= cfg.dropout < 1.0:
+            raise ValueError(f"dropout must be in [0, 1), got {cfg.dropout}")
+        hd = cfg.n_embd // cfg.n_head
+        if cfg.mixer == "decay" and hd not in (64, 128):
+            raise ValueError(f"the decay mixer takes heads of 64 or 128, got {hd}")
         self.cfg = cfg
         if own_attention is None:
             own_attention = os.environ.get("NEXAR_ATTENTION", "sdpa") == "nexar"
@@ -80,6 +107,12 @@ class GPT2(torch.nn.Module):
         self.p: Dict[str, torch.nn.Parameter] = self.flat.params()
         for i, (name, par) in enumerate(self.p.items()):
             self.register_parameter(name.replace(".", "_"), par)
+        self.rotary_table = ops.rotary_table(cfg.block_size, hd, device=device) if cfg.positions == "rotary" else None
+        self.log_decay = None
+        if cfg.mixer == "decay":
+            decay = [math.log1p(-(2.0 ** -(5 + h))) for h in range(cfg.n_head)]
+            self.log_decay = torch.tensor(decay, dtype=torch.float32, device=device)
+        self.dropout_state = ops.DropoutState(seed, device) if cfg.dropout else None
 
     @torch.no_grad()
     def _init_weights(self, seed: int):
@@ -92,7 +125,7 @@ class GPT2(torch.nn.Module):
             v = self.flat.view(self.flat.master, e.name)
             if e.name.endswith(".b"):
                 v.zero_()
-            elif e.name.endswith("ln1.w") or e.name.endswith("ln2.w") or e.name == "lnf.w":
+            elif e.name.endswith(("ln1.w", "ln2.w", "head_norm.w")) or e.name == "lnf.w":
                 v.fill_(1.0)
             elif e.name.endswith("proj.w"):
                 v.normal_(0.0, proj_std, generator=g)
@@ -107,12 +140,20 @@ class GPT2(torch.nn.Module):
         B, T = idx.shape
         C, H = cfg.n_embd, cfg.n_head
         hd = C // H
-        x = ops.embedding(idx, p["wte"], p["wpe"]).view(B * T, C)
+        drop, state = (cfg.dropout, self.dropout_state) if self.training else (0.0, None)
+        x = ops.embedding(idx, p["wte"], p.get("wpe")).view(B * T, C)
+        if drop:
+            x = ops.dropout(x, drop, state, site=0)
         h = ops.layer_norm(x, p["h0.ln1.w"], p["h0.ln1.b"], cfg.ln_eps)
         for l in range(cfg.n_layer):
             q = f"h{l}."
             qkv = ops.linear(h, p[q + "attn.w"], p[q + "attn.b"])
-            if self.own_attention and ops.attention_supported(B, T, H, hd):
+            if self.rotary_table is not None:
+                qkv = ops.rotary(qkv.view(B, T, 3 * H, hd), self.rotary_table, heads=2 * H).view(B * T, 3 * C)
+            if cfg.mixer == "decay":
+                y = ops.decay_attention_qkv(qkv.view(B, T, 3, H, hd), self.log_decay).view(B * T * H, hd)
+                y = ops.layer_norm(y, p[q + "head_norm.w"], p[q + "head_norm.b"], cfg.ln_eps).view(B * T, C)
+            elif self.own_attention and ops.attention_supported(B, T, H, hd):
                 y = ops.attention(qkv, B, T, H, causal=True)
             else:
                 qkv = qkv.view(B, T, 3, H, hd)
@@ -122,15 +163,17 @@ class GPT2(torch.nn.Module):
                 y = y.transpose(1, 2).reshape(B * T, C)
             # projection bias is folded into the residual add of the next LayerNorm
             a = ops.linear(y, p[q + "proj.w"])
-            x, h = ops.residual_layer_norm(x, a, p[q + "ln2.w"], p[q + "ln2.b"], cfg.ln_eps, rbias=p[q + "proj.b"])
+            x, h = ops.residual_layer_norm(x, a, p[q + "ln2.w"], p[q + "ln2.b"], cfg.ln_eps, rbias=p[q + "proj.b"],
+                                           p=drop, dropout=state, site=1 + 2 * l)
             f = ops.linear(h, p[q + "fc.w"], p[q + "fc.b"], act="gelu")
             m = ops.linear(f, p[q + "fcproj.w"])
             if l + 1 < cfg.n_layer:
                 nq = f"h{l + 1}."
                 x, h = ops.residual_layer_norm(x, m, p[nq + "ln1.w"], p[nq + "ln1.b"], cfg.ln_eps,
-                                               rbias=p[q + "fcproj.b"])
+                                               rbias=p[q + "fcproj.b"], p=drop, dropout=state, site=2 + 2 * l)
             else:
-                x, h = ops.residual_layer_norm(x, m, p["lnf.w"], p["lnf.b"], cfg.ln_eps, rbias=p[q + "fcproj.b"])
+                x, h = ops.residual_layer_norm(x, m, p["lnf.w"], p["lnf.b"], cfg.ln_eps, rbias=p[q + "fcproj.b"],
+                                               p=drop, dropout=state, site=2 + 2 * l)
         # tied head: its weight gradient is completed by the embedding backward
         logits = ops.linear(h, p["wte"], ready=False)  # [B*T, Vp]
         if targets is None:

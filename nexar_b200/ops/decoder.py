@@ -132,12 +132,14 @@ class DropoutState:
 
     def __init__(self, seed: int, device=None, step: int = 0):
         device = torch.device("cuda") if device is None else torch.device(device)
-        self.tensor = torch.empty(2, dtype=torch.int64, device=device)
-        self.set(seed, step)
+        self.tensor = torch.tensor(self._values(seed, step), dtype=torch.int64, device=device)
+
+    @staticmethod
+    def _values(seed: int, step: int):  # any whole numbers, as signed 64-bit ones
+        return [(int(v) + (1 << 63)) % (1 << 64) - (1 << 63) for v in (seed, step)]
 
     def set(self, seed: int, step: int = 0) -> None:
-        wrap = lambda v: (int(v) + (1 << 63)) % (1 << 64) - (1 << 63)  # noqa: E731
-        self.tensor.copy_(torch.tensor([wrap(seed), wrap(step)], dtype=torch.int64))
+        self.tensor.copy_(torch.tensor(self._values(seed, step), dtype=torch.int64))
 
     def advance(self) -> None:
         self.tensor[1:].add_(1)

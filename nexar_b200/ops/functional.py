@@ -417,7 +417,7 @@ class _Embedding(torch.autograd.Function):
         out = torch.empty(B, T, C, dtype=wte.dtype, device=wte.device)
         _native.cuda().embed_fwd(tok, wte, wpe, out, T)
         ctx.save_for_backward(tok)
-        ctx.shapes = (wte.shape, wpe.shape)
+        ctx.shapes = (wte.shape, None if wpe is None else wpe.shape)
         ctx.params = (wte, wpe)
         return out
 
@@ -429,8 +429,13 @@ class _Embedding(torch.autograd.Function):
         wte, wpe = ctx.params
         # wte's sink already holds the tied head's gradient (written earlier
         # in backward): the token scatter adds onto it. wpe is overwritten.
-        swte, swpe = _sink(wte), _sink(wpe)
+        swte, swpe = _sink(wte), None if wpe is None else _sink(wpe)
         dwte = swte if swte is not None else torch.zeros(wte_shape, dtype=dout.dtype, device=dout.device)
+        if wpe is None:
+            _native.cuda().embed_bwd(tok, dout.contiguous(), dwte, None, B, T)
+            if swte is not None:
+                _ready(wte)
+            return None, (None if swte is not None else dwte), None
         dwpe = swpe if swpe is not None else torch.zeros(wpe_shape, dtype=dout.dtype, device=dout.device)
         _native.cuda().embed_bwd(tok, dout.contiguous(), dwte, dwpe, B, T)
         if T < wpe_shape[0]:
@@ -442,7 +447,8 @@ class _Embedding(torch.autograd.Function):
         return None, (None if swte is not None else dwte), (None if swpe is not None else dwpe)
 
 
-def embedding(tok, wte, wpe):
+def embedding(tok, wte, wpe=None):
+    """wte[tok] + wpe[position]; without ``wpe`` (rotary positions) the token rows alone."""
     return _Embedding.apply(tok, wte, wpe)
 
 

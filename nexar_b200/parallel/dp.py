@@ -53,6 +53,8 @@ class DataParallelTrainer:
             grad_alloc = lambda n: comm.symmetric_empty(  # noqa: E731
                 [n], torch.bfloat16, nvls=getattr(comm, "nvls_preferred", False))
         self.model = GPT2(cfg, self.device, grad_alloc=grad_alloc, seed=seed)
+        self._dropout_seed = seed
+        self._seed_dropout(seed, 0)
         flat = self.model.flat
         flat.grad.zero_()  # padding between parameters is never written
         if self.world > 1:
@@ -107,6 +109,12 @@ class DataParallelTrainer:
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.graph_launches = 0
         self._host_loss = torch.zeros((), dtype=torch.float32).pin_memory()
+
+    def _seed_dropout(self, seed: int, step: int) -> None:
+        """Each rank draws masks of its own for its own tokens."""
+        if self.model.dropout_state is not None:
+            rank = self.comm.rank if self.comm is not None else 0
+            self.model.dropout_state.set(seed + 1_000_003 * rank, step)
 
     # ---------------------------------------------------------------- hooks
     def _make_hook(self, name):
@@ -185,6 +193,8 @@ class DataParallelTrainer:
         C.grad_norm_clip(flat.grad, self.clip, self.norm_scratch, self.norm_counter, self.grad_norm,
                          self.clip_coef)
         self.step_dev.add_(1)
+        if self.model.dropout_state is not None:
+            self.model.dropout_state.advance()  # on the device: a replayed step draws anew
         C.adamw(flat.master, flat.exp_avg, flat.exp_avg_sq, flat.grad, flat.param_bf16, flat.decay_end,
                 self.lr, self.betas[0], self.betas[1], self.eps, self.wd, 1, self.clip_coef,
                 self.step_dev, self.lr_dev)
@@ -276,6 +286,8 @@ class DataParallelTrainer:
             "exp_avg_sq": flat.exp_avg_sq.detach().cpu(),
             "step": int(self.step_dev.item()),
             "lr": float(self.lr_dev.item()),
+            "dropout": None if self.model.dropout_state is None else {
+                "seed": self._dropout_seed, "step": int(self.model.dropout_state.tensor[1].item())},
             "optim": {"betas": list(self.betas), "eps": self.eps, "weight_decay": self.wd, "grad_clip": self.clip},
         }
 
@@ -288,7 +300,9 @@ class DataParallelTrainer:
         re-derived from the fp32 master weights."""
         if sd.get("format") != self.CHECKPOINT_FORMAT:
             raise ValueError(f"not a {self.CHECKPOINT_FORMAT} checkpoint: {sd.get('format')!r}")
-        if sd["config"] != dataclasses.asdict(self.cfg):
+        # fields that a checkpoint written before they existed does not have stand at their defaults
+        saved = {**{f.name: f.default for f in dataclasses.fields(self.cfg)}, **sd["config"]}
+        if saved != dataclasses.asdict(self.cfg):
             raise ValueError(f"checkpoint is for model {sd['config']}, this trainer runs {dataclasses.asdict(self.cfg)}")
         flat = self.model.flat
         layout = [[e.name, list(e.shape), e.offset, e.numel] for e in flat.entries]
@@ -301,6 +315,9 @@ class DataParallelTrainer:
         flat.param_bf16.copy_(flat.master)
         self.step_dev.fill_(int(sd["step"]))
         self.lr_dev.fill_(float(sd["lr"]))
+        if sd.get("dropout") is not None:
+            self._dropout_seed = int(sd["dropout"]["seed"])
+            self._seed_dropout(self._dropout_seed, int(sd["dropout"]["step"]))
         o = sd.get("optim", {})
         new = (tuple(o.get("betas", self.betas)), o.get("eps", self.eps), o.get("weight_decay", self.wd),
                o.get("grad_clip", self.clip))

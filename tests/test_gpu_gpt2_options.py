@@ -1,0 +1,151 @@
+"""GPT-2 with rotary positions, dropout and the decay mixer together: against a plain fp32 model with the same masks,
+in a captured step, and across a checkpoint."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+import decoder_oracle as oracle
+from nexar_b200 import ops
+from nexar_b200.models.gpt2 import GPT2, GPT2Config
+from nexar_b200.parallel.dp import DataParallelTrainer
+
+gpu = pytest.mark.gpu
+
+
+def _config(**kw):
+    return GPT2Config(**{**dict(n_layer=2, n_head=2, n_embd=128, vocab_size=1000, padded_vocab=1024, block_size=96), **kw})
+
+
+OPTIONS = [dict(positions="rotary"), dict(dropout=0.2), dict(mixer="decay"),
+           dict(positions="rotary", dropout=0.1, mixer="decay")]
+
+
+def _keep(cfg, shape, seed, step, site, device):
+    """Factors of the model's dropout calls: draws of the published generator."""
+    n = shape[0] * shape[1]
+    keep, scale = oracle.dropout_keep(n, seed, step, site, cfg.dropout)
+    return (keep.double() * scale).view(shape).to(device).float()
+
+
+def _reference(cfg, p, idx, tgt, seed, step, drop=True):
+    """The model written out in fp32 (rotations and decays in 64 bits)."""
+    B, T = idx.shape
+    C, H = cfg.n_embd, cfg.n_head
+    hd = C // H
+    dev = idx.device
+
+    def dropped(x, site):
+        return x * _keep(cfg, (B * T, C), seed, step, site, dev) if cfg.dropout and drop else x
+    x = p["wte"][idx].view(B * T, C)
+    if cfg.positions == "learned":
+        x = x + p["wpe"][:T].repeat(B, 1)
+    x = dropped(x, 0)
+    for l in range(cfg.n_layer):
+        q = f"h{l}."
+        h = F.layer_norm(x, (C,), p[q + "ln1.w"], p[q + "ln1.b"])
+        qkv = (h @ p[q + "attn.w"].t() + p[q + "attn.b"]).view(B, T, 3, H, hd)
+        if cfg.positions == "rotary":
+            freq, m = ops.rotary_frequencies(hd)
+            turned = oracle.rotate(qkv[:, :, :2].reshape(B, T, 2 * H, hd).double(), torch.arange(T, device=dev), freq, m, "half")
+            qkv = torch.cat([turned.float().view(B, T, 2, H, hd), qkv[:, :, 2:]], 2)
+        qq, kk, vv = qkv.unbind(2)
+        if cfg.mixer == "decay":
+            lam = torch.log1p(-torch.exp2(-(5.0 + torch.arange(H, device=dev, dtype=torch.float64))))
+            y = oracle.decay_attention(qq.double(), kk.double(), vv.double(), lam)[0].float()
+            y = F.layer_norm(y, (hd,), p[q + "head_norm.w"], p[q + "head_norm.b"])
+        else:
+            y = F.scaled_dot_product_attention(qq.transpose(1, 2), kk.transpose(1, 2), vv.transpose(1, 2),
+                                               is_causal=True).transpose(1, 2)
+        x = x + dropped(y.reshape(B * T, C) @ p[q + "proj.w"].t() + p[q + "proj.b"], 1 + 2 * l)
+        h = F.layer_norm(x, (C,), p[q + "ln2.w"], p[q + "ln2.b"])
+        f = F.gelu(h @ p[q + "fc.w"].t() + p[q + "fc.b"], approximate="tanh")
+        x = x + dropped(f @ p[q + "fcproj.w"].t() + p[q + "fcproj.b"], 2 + 2 * l)
+    h = F.layer_norm(x, (C,), p["lnf.w"], p["lnf.b"])
+    return F.cross_entropy((h @ p["wte"].t())[:, :cfg.vocab_size], tgt.reshape(-1))
+
+
+@gpu
+@pytest.mark.parametrize("options", OPTIONS, ids=lambda o: "-".join(o))
+def test_loss_and_gradients_match_the_plain_model(cuda0, options):
+    cfg = _config(**options)
+    m = GPT2(cfg, cuda0, seed=6)
+    g = torch.Generator(device=cuda0).manual_seed(3)
+    with torch.no_grad():  # biases and norms away from their initial values
+        for name, p in m.p.items():
+            if name.endswith(".b"):
+                p.copy_(0.05 * torch.randn(p.shape, device=cuda0, generator=g))
+            elif "norm" in name or ".ln" in name or name.startswith("lnf"):
+                p.copy_(1 + 0.1 * torch.randn(p.shape, device=cuda0, generator=g))
+        m.flat.grad.fill_(7.0)  # stale values must be overwritten
+    if cfg.dropout:
+        m.dropout_state.set(6, 11)
+    idx = torch.randint(0, cfg.vocab_size, (2, 96), device=cuda0, generator=g)
+    tgt = torch.randint(0, cfg.vocab_size, (2, 96), device=cuda0, generator=g)
+    loss = m(idx, tgt, unit_grad=True)
+    loss.backward()
+    p = {k: v.detach().float().requires_grad_(True) for k, v in m.p.items()}
+    ref = _reference(cfg, p, idx, tgt, 6, 11)
+    ref.backward()
+    # bf16 activations through two layers: the same bounds as the model without options
+    assert abs(loss.item() - ref.item()) < 0.05
+    bad = []
+    for name in m.p:
+        ours, want = m.flat.view(m.flat.grad, name).float(), p[name].grad
+        err = ((ours - want).norm() / (want.norm() + 1e-6)).item()
+        if not err < 0.05:
+            bad.append((name, round(err, 4)))
+    assert not bad, bad
+    m.eval()  # no dropout outside training
+    with torch.no_grad():
+        ref = _reference(cfg, p, idx, tgt, 6, 11, drop=False)
+        assert abs(m(idx, tgt).item() - ref.item()) < 0.05
+
+
+@gpu
+def test_captured_steps_draw_what_eager_steps_draw(cuda0):
+    cfg = _config(positions="rotary", dropout=0.3, mixer="decay")
+    g = torch.Generator().manual_seed(1)
+    idx = torch.randint(0, cfg.vocab_size, (2, 96), generator=g)
+    tgt = torch.randint(0, cfg.vocab_size, (2, 96), generator=g)
+    losses = []
+    for graph in (False, True):
+        # lr 0: the weights stay, so the losses differ by their masks alone
+        tr = DataParallelTrainer(cfg, 2, 96, use_cuda_graph=graph, seed=5, lr=0.0)
+        tr.set_batch(idx, tgt)
+        tr.capture(warmup=3)
+        tr.model.dropout_state.set(5, 3)
+        losses.append([tr.step(idx, tgt) for _ in range(3)])
+        assert tr.model.dropout_state.tensor.tolist() == [5, 6]
+    assert losses[0] == pytest.approx(losses[1], rel=1e-5) and len(set(losses[0])) == 3
+
+
+@gpu
+def test_checkpoint_carries_the_generator(cuda0, tmp_path):
+    cfg = _config(dropout=0.2)
+    g = torch.Generator().manual_seed(2)
+    batch = lambda: [torch.randint(0, cfg.vocab_size, (2, 96), generator=g) for _ in range(2)]  # noqa: E731
+    a = DataParallelTrainer(cfg, 2, 96, use_cuda_graph=False, seed=9)
+    a.step(*batch())
+    path = str(tmp_path / "d.pt")
+    a.save(path)
+    b = DataParallelTrainer(cfg, 2, 96, use_cuda_graph=False, seed=1)
+    b.load(path)
+    assert torch.equal(a.model.dropout_state.tensor, b.model.dropout_state.tensor)
+    x = batch()
+    assert a.step(*x) == pytest.approx(b.step(*x), rel=1e-5)
+    # a checkpoint from before the options existed loads into a model without them
+    plain = DataParallelTrainer(_config(), 2, 96, use_cuda_graph=False)
+    sd = plain.state_dict()
+    for k in ("dropout", "positions", "mixer"):
+        del sd["config"][k]
+    del sd["dropout"]
+    plain.load_state_dict(sd)
+    with pytest.raises(ValueError, match="model"):
+        a.load_state_dict(sd)
+
+
+@pytest.mark.parametrize("bad", [dict(positions="none"), dict(mixer="mlp"), dict(dropout=1.0), dict(dropout=-0.1),
+                                 dict(mixer="decay", n_head=4)])
+def test_configuration_refusals(bad):
+    with pytest.raises(ValueError):
+        GPT2(_config(**bad), "cpu")
