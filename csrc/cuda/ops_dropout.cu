@@ -139,9 +139,11 @@ NEXAR_D uint4 pack8(const float* f) {
 }
 NEXAR_D uint4 stream16(const __nv_bfloat16* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }
 
-// One warp per row, NP packs of 8 columns per lane. The sum is rounded to the
-// stored bf16 before the statistics, as in the operator without dropout.
-template <int NP>
+// RW warps per row, NP packs of 8 columns per lane; rows of more than 1024 columns
+// take two warps, which leaves registers for twice the rows in flight. The sum is
+// rounded to the stored bf16 before the statistics, as in the operator without
+// dropout.
+template <int NP, int RW>
 __global__ void __launch_bounds__(kRowWarps * 32) k_dropout_ln_fwd(
     const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ r, const __nv_bfloat16* __restrict__ rb,
     __nv_bfloat16* __restrict__ sum_out, const __nv_bfloat16* __restrict__ w, const __nv_bfloat16* __restrict__ b,
@@ -149,16 +151,27 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_dropout_ln_fwd(
     const int64_t* __restrict__ state, uint32_t site, uint32_t threshold, float scale,
     int64_t* __restrict__ snapshot) {
   if (blockIdx.x == 0 && threadIdx.x < 2) snapshot[threadIdx.x] = state[threadIdx.x];
-  const int lane = threadIdx.x & 31;
-  const int row = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-  if (row >= R) return;
+  const int lane = threadIdx.x & (32 * RW - 1), slot = threadIdx.x / (32 * RW);
+  const int row = blockIdx.x * (kRowWarps / RW) + slot;
+  if (row >= R) return;  // all warps of the row
+  __shared__ float red[2][kRowWarps];
+  auto row_total = [&](float v, int which) {
+    v = row_sum(v);
+    if constexpr (RW == 2) {
+      const int warp = threadIdx.x >> 5;
+      if ((threadIdx.x & 31) == 0) red[which][warp] = v;
+      asm volatile("bar.sync %0, 64;" ::"r"(slot + 1) : "memory");
+      v = red[which][warp & ~1] + red[which][warp | 1];  // the same order in both warps
+    }
+    return v;
+  };
   const Draws draws(state, site);
   const uint32_t below = (threshold << 16) - 1;
   const size_t base = (size_t)row * C;
   uint4 vx[NP], vr[NP];
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    const int col = (lane + 32 * k) * 8;
+    const int col = (lane + 32 * RW * k) * 8;
     if (col < C) {
       vx[k] = stream16(x + base + col);
       vr[k] = stream16(r + base + col);
@@ -167,7 +180,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_dropout_ln_fwd(
   float s = 0.f;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    const int col = (lane + 32 * k) * 8;
+    const int col = (lane + 32 * RW * k) * 8;
     if (col < C) {
       float a[8], d[8];
       unpack8(vx[k], a);
@@ -188,21 +201,21 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_dropout_ln_fwd(
       for (int e = 0; e < 8; ++e) s += a[e];
     }
   }
-  const float mu = row_sum(s) / C;
+  const float mu = row_total(s, 0) / C;
   float q = 0.f;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    if ((lane + 32 * k) * 8 < C) {
+    if ((lane + 32 * RW * k) * 8 < C) {
       float a[8];
       unpack8(vx[k], a);
 #pragma unroll
       for (int e = 0; e < 8; ++e) q += (a[e] - mu) * (a[e] - mu);
     }
   }
-  const float rs = rsqrtf(row_sum(q) / C + eps);
+  const float rs = rsqrtf(row_total(q, 1) / C + eps);
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    const int col = (lane + 32 * k) * 8;
+    const int col = (lane + 32 * RW * k) * 8;
     if (col < C) {
       float a[8], wf[8], bf[8];
       unpack8(vx[k], a);
@@ -408,16 +421,15 @@ cudaError_t dropout_ln_fwd(const __nv_bfloat16* x, const __nv_bfloat16* r, const
                            float* mean, float* rstd, int R, int C, float eps, const int64_t* state, uint32_t site,
                            uint32_t threshold, float scale, int64_t* snapshot, cudaStream_t s) {
   if (C % 8 || C > 2048 || R < 1 || threshold < 1 || threshold > 65536) return cudaErrorInvalidValue;
-  const int grid = (R + kRowWarps - 1) / kRowWarps;
-#define NEXAR_DROP_FWD(NP)                                                                                     \
-  k_dropout_ln_fwd<NP><<<grid, kRowWarps * 32, 0, s>>>(x, r, rb, sum_out, w, b, y, mean, rstd, R, C, eps, state, \
-                                                       site, threshold, scale, snapshot)
-  if (C <= 256) NEXAR_DROP_FWD(1);
-  else if (C <= 512) NEXAR_DROP_FWD(2);
-  else if (C <= 768) NEXAR_DROP_FWD(3);
-  else if (C <= 1024) NEXAR_DROP_FWD(4);
-  else if (C <= 1536) NEXAR_DROP_FWD(6);
-  else NEXAR_DROP_FWD(8);
+#define NEXAR_DROP_FWD(NP, RW)                                                                              \
+  k_dropout_ln_fwd<NP, RW><<<(R + kRowWarps / RW - 1) / (kRowWarps / RW), kRowWarps * 32, 0, s>>>(            \
+      x, r, rb, sum_out, w, b, y, mean, rstd, R, C, eps, state, site, threshold, scale, snapshot)
+  if (C <= 256) NEXAR_DROP_FWD(1, 1);
+  else if (C <= 512) NEXAR_DROP_FWD(2, 1);
+  else if (C <= 768) NEXAR_DROP_FWD(3, 1);
+  else if (C <= 1024) NEXAR_DROP_FWD(4, 1);
+  else if (C <= 1536) NEXAR_DROP_FWD(3, 2);
+  else NEXAR_DROP_FWD(4, 2);
 #undef NEXAR_DROP_FWD
   return cudaGetLastError();
 }
