@@ -189,7 +189,7 @@ std::vector<at::Tensor> op_dropout_ln_fwd(const at::Tensor& x, const at::Tensor&
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) % 8 == 0 && x.size(-1) >= 8 && x.size(-1) <= 2048,
               "nexar_b200: residual_layer_norm with dropout needs rows of a multiple of 8, at most 2048");
   const int64_t C = x.size(-1), R = x.numel() / C;
-  TORCH_CHECK(R <= std::numeric_limits<int>::max() - 16, "nexar_b200: too many rows");
+  TORCH_CHECK(R <= std::numeric_limits<int>::max() - 65536, "nexar_b200: too many rows");
   need_rows(x, x, R * C, "x");
   need_rows(r, x, R * C, "r");
   need_rows(w, x, C, "weight");

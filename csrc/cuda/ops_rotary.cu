@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kRotThreads, 4) k_rotary(const __grid_constant
   const T* x = reinterpret_cast<const T*>(p.x) + b * p.sb + t * p.st + hg * p.sh;
   T* y = reinterpret_cast<T*>(p.y) + (n * p.heads + hg) * a.D;
   const long long dx = HG * p.sh;
-  const int dy = HG * a.D;
+  const long long dy = (long long)HG * a.D;
 #pragma unroll 1
   for (int h0 = hg; h0 < p.heads; h0 += kRotUnroll * HG) {
     Pack<T, W> u[kRotUnroll], v[kRotUnroll];

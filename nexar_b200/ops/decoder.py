@@ -177,11 +177,12 @@ def decay_attention(q, k, v, log_decay, state=None, lengths=None, scale: Optiona
         S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,    o_t = scale S_t^T q_t.
 
     q, k, v: bf16 [B, T, H, D] of the same shape, D 64 or 128, any strides. ``log_decay``: fp32 [H],
-    each finite and at most 0 (0: no decay); not trained. ``state``: fp32 [B, H, D, D] before the
-    first token (default zero). ``lengths``: int32 [B]; tokens from there on do not exist (not read, zero
-    output and gradients, the final state is the one behind the last token). ``scale`` defaults to D^-0.5.
-    Returns o [B, T, H, D] bf16, or (o, final state) with ``return_state``; differentiable in q, k, v
-    and state (lengths are kept by reference until the backward pass)."""
+    each at most 0 (0: no decay); not trained. ``state``: contiguous fp32 [B, H, D, D] before the first
+    token (default zero). ``lengths``: int32 [B], clipped to 0 .. T; tokens from there on do not exist
+    (not read, zero output and gradients, the final state is the one behind the last token). ``scale``
+    defaults to D^-0.5. Returns o [B, T, H, D] bf16, or (o, final state) with ``return_state``;
+    differentiable in q, k, v and state, once. Tokens are worked on in chunks of 64: a value that is
+    not finite can show in the output of every token of its chunk."""
     return _decay(q, k, v, log_decay, state, lengths, _decay_scale(scale, q.shape[-1]), return_state)
 
 
@@ -194,7 +195,7 @@ def decay_attention_qkv(qkv, log_decay, state=None, lengths=None, scale: Optiona
 
 def decay_attention_step(q, k, v, log_decay, state, scale: Optional[float] = None):
     """One token of :func:`decay_attention` for inference: q, k, v bf16 [B, H, D]; updates ``state``
-    (fp32 [B, H, D, D]) in place and returns o [B, H, D]."""
+    (contiguous fp32 [B, H, D, D]) in place and returns o [B, H, D]."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
         raise ValueError("decay_attention_step has no gradient; call it under torch.no_grad() or train with "
                          "decay_attention")
