@@ -17,7 +17,8 @@
 // Few sequences and heads: the tokens are split into segments. k_decay_chunk in
 // its state-only form gives each segment's own contribution to the state,
 // k_decay_scan turns these into the state before each segment, and the main
-// kernel then runs all segments at once.
+// kernel then runs all segments at once. The backward pass takes the states of
+// the forward direction from the forward pass, and dk those of dv, transposed.
 //
 // All products run on tcgen05 in two groups (K': the chunk's keys decayed to its
 // end; P: the decayed and masked scores):
@@ -177,8 +178,9 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
   const int b = bh / a.H, h = bh % a.H;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int len = a.lengths ? max(0, min(a.lengths[b], a.T)) : a.T;
-  const int t_begin = seg * a.seg_tokens;
-  const int t_end = min(a.T, t_begin + a.seg_tokens);   // index i, counted from the first token of the direction
+  const int tokens = STATES ? a.seg_tokens : a.seg_tokens * a.step;
+  const int t_begin = seg * tokens;
+  const int t_end = min(a.T, t_begin + tokens);   // index i, counted from the first token of the direction
   const int live = max(0, min(len, t_end) - t_begin);   // tokens of this segment that exist
   const int nchunks = (live + kChunk - 1) / kChunk;
 
@@ -251,9 +253,8 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
   bool x0_t = false;
   if constexpr (!STATES) {
     if (a.nseg > 1) {
-      const bool own = R.segments_from < 0;
-      x0 = (own ? R.segments : a.role[R.segments_from].segments) + ((size_t)bh * a.nseg + seg) * D * D;
-      x0_t = !own;
+      x0 = R.segments + ((size_t)bh * a.nseg + seg * a.step) * D * D;
+      x0_t = !R.seg_own;
     } else if (R.init) {
       x0 = R.init + (size_t)bh * D * D;
       x0_t = R.init_transposed;
@@ -585,7 +586,6 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
 // the state behind the last. One thread per 4 elements of a head's state.
 template <int D> __global__ void __launch_bounds__(256) k_decay_scan(const __grid_constant__ DecayArgs a) {
   const DecayRole& R = a.role[blockIdx.z];
-  if (R.segments_from >= 0) return;  // reads another role's segments
   const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H;
   const int e = blockIdx.y * 256 + threadIdx.x;  // < D * D / 4
   const int len = a.lengths ? max(0, min(a.lengths[b], a.T)) : a.T;
@@ -685,20 +685,21 @@ cudaError_t launch_chunks(const DecayArgs& a, int roles, cudaStream_t s) {
   const cudaError_t e =
       cudaFuncSetAttribute(k_decay_chunk<D, STATES>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
-  k_decay_chunk<D, STATES><<<dim3(a.B * a.H, a.nseg, roles), S::kThreads, S::kSmem, s>>>(a);
+  k_decay_chunk<D, STATES><<<dim3(a.B * a.H, STATES ? a.nseg : (a.nseg + a.step - 1) / a.step, roles), S::kThreads, S::kSmem, s>>>(a);
   return cudaGetLastError();
 }
 
 template <int D> cudaError_t decay_typed(const DecayArgs& a, cudaStream_t s, int* launches) {
   *launches = 0;
   if (a.nseg > 1) {
-    // roles that read another role's segment states come last and need no states of their own
     int own = 0;
-    while (own < a.nroles && a.role[own].segments_from < 0) ++own;
-    const cudaError_t e = launch_chunks<D, true>(a, own, s);
-    if (e != cudaSuccess) return e;
-    k_decay_scan<D><<<dim3(a.B * a.H, D * D / 1024, own), 256, 0, s>>>(a);
-    *launches += 2;
+    while (own < a.nroles && a.role[own].seg_own) ++own;
+    if (own > 0) {
+      const cudaError_t e = launch_chunks<D, true>(a, own, s);
+      if (e != cudaSuccess) return e;
+      k_decay_scan<D><<<dim3(a.B * a.H, D * D / 1024, own), 256, 0, s>>>(a);
+      *launches += 2;
+    }
   }
   *launches += 1;
   return launch_chunks<D, false>(a, a.nroles, s);
@@ -729,7 +730,7 @@ int decay_segments(int B, int T, int H, int D, int roles) {
 }
 
 cudaError_t decay_attention(const DecayArgs& a, cudaStream_t s, int* launches) {
-  if (a.nroles < 1 || a.nroles > 3 || a.B < 1 || a.H < 1 || a.T < 1 || (long long)a.B * a.H > 0x7fffffffLL || a.nseg > 65535 || a.nseg < 1 ||
+  if (a.nroles < 1 || a.nroles > 3 || a.B < 1 || a.H < 1 || a.T < 1 || (long long)a.B * a.H > 0x7fffffffLL || a.nseg > 65535 || a.nseg < 1 || a.step < 1 ||
       (long long)a.nseg * a.seg_tokens < a.T || (a.nseg > 1 && a.seg_tokens % kChunk))
     return cudaErrorInvalidValue;
   if (a.D == 64) return decay_typed<64>(a, s, launches);

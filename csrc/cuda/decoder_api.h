@@ -67,15 +67,21 @@ struct DecayRole {
   const float* init;        // [B, H, D, D] state before the first token, or null
   int init_transposed;
   float* final_state;       // state behind the last token, or null
-  float* segments;          // [B, H, nseg, D, D] scratch when the tokens are split
-  int segments_from;        // index of the role whose segment states this one reads, transposed (-1: its own)
+  // When the tokens are split: states before every piece of seg_tokens, [B, H, nseg, D, D]. seg_own: computed here and
+  // read as they are; else another role's or the forward pass's, read transposed. Roles with states of their own come
+  // first.
+  float* segments;
+  int seg_own;
 };
 struct DecayArgs {
   DecayRole role[3];
   int nroles;
   const float* log_decay;   // [H]
   const int* lengths;       // [B] or null
-  int B, T, H, D, nseg, seg_tokens;
+  int B, T, H, D;
+  // The states are computed for nseg pieces of seg_tokens, side by side; the outputs then by blocks that take `step`
+  // pieces one after the other.
+  int nseg, seg_tokens, step;
 };
 int decay_segments(int B, int T, int H, int D, int roles);  // number of token segments worked on side by side
 cudaError_t decay_attention(const DecayArgs& a, cudaStream_t s, int* launches);

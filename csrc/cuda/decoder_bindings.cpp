@@ -293,30 +293,37 @@ void set_out(const at::Tensor& t, DecayRole& r) {
   r.out = mbf(t);
   r.ob = t.stride(0), r.ot = t.stride(1), r.oh = t.stride(2);
 }
-void launch_decay(DecayArgs& a, const DecayShape& s, const at::Tensor& log_decay, const OptTensor& lengths,
-                  const at::Tensor& q, const std::vector<at::Tensor*>& segments) {
+void set_tokens(DecayArgs& a, const DecayShape& s, const at::Tensor& log_decay, const OptTensor& lengths,
+                const at::Tensor& q) {
   a.log_decay = log_decay.data_ptr<float>();
   a.lengths = decay_lengths(lengths, q);
   a.B = (int)s.B, a.T = (int)s.T, a.H = (int)s.H, a.D = (int)s.D;
-  a.nseg = decay_segments(a.B, a.T, a.H, a.D, a.nroles);
-  const int chunks = (a.T + 63) / 64;
-  const int per = (chunks + a.nseg - 1) / a.nseg;
-  a.seg_tokens = per * 64;
-  a.nseg = (chunks + per - 1) / per;
-  if (a.nseg > 1) {
-    for (int i = 0; i < a.nroles; ++i) {
-      if (a.role[i].segments_from >= 0) continue;
-      *segments[i] = at::empty({s.B * s.H * a.nseg * s.D * s.D}, log_decay.options());
-      a.role[i].segments = segments[i]->data_ptr<float>();
-    }
-  }
+}
+// Chunks of 64 tokens to a segment.
+int chunks_to_a_segment(const DecayArgs& a, int roles) {
+  const int chunks = (a.T + 63) / 64, n = decay_segments(a.B, a.T, a.H, a.D, roles);
+  return (chunks + n - 1) / n;
+}
+void set_segments(DecayArgs& a, int chunks, int step) {
+  a.seg_tokens = chunks * 64, a.step = step;
+  a.nseg = (a.T + a.seg_tokens - 1) / a.seg_tokens;
+}
+// Memory for a role's own segment states.
+at::Tensor own_segments(DecayArgs& a, DecayRole& r, const DecayShape& s, const at::Tensor& like) {
+  at::Tensor t = at::empty({s.B * s.H * a.nseg, s.D, s.D}, like.options());
+  r.segments = t.data_ptr<float>();
+  r.seg_own = 1;
+  return t;
+}
+void launch_decay(DecayArgs& a, const at::Tensor& q) {
   int launches = 0;
   check(decay_attention(a, stream_on(q), &launches), "decay_attention");
   count_launch(launches);
 }
 
-// Returns o [B, T, H, D] and, if asked for, the final state.
-std::tuple<at::Tensor, OptTensor> op_decay_fwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+// Returns o [B, T, H, D], if asked for the final state, and where the tokens were split the states before the segments
+// with the chunks of a segment.
+std::tuple<at::Tensor, OptTensor, at::Tensor, int64_t> op_decay_fwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
                                                const at::Tensor& log_decay, const OptTensor& state,
                                                const OptTensor& lengths, double scale, bool want_state) {
   const DecayShape s = decay_shape(q_in, log_decay);
@@ -331,7 +338,7 @@ std::tuple<at::Tensor, OptTensor> op_decay_fwd(const at::Tensor& q_in, const at:
   if (want_state) fin = at::empty({s.B, s.H, s.D, s.D}, log_decay.options());
   if (o.numel() == 0) {
     if (fin && fin->numel()) state ? fin->copy_(*state) : fin->zero_();
-    return {o, fin};
+    return {o, fin, at::Tensor(), 0};
   }
   DecayArgs a{};
   a.nroles = 1;
@@ -344,17 +351,19 @@ std::tuple<at::Tensor, OptTensor> op_decay_fwd(const at::Tensor& q_in, const at:
   r.kv = 1.f;
   r.init = state ? state->data_ptr<float>() : nullptr;
   r.final_state = fin ? fin->data_ptr<float>() : nullptr;
-  r.segments_from = -1;
+  set_tokens(a, s, log_decay, lengths, q);
+  set_segments(a, chunks_to_a_segment(a, 1), 1);
   at::Tensor seg;
-  launch_decay(a, s, log_decay, lengths, q, {&seg});
-  return {o, fin};
+  if (a.nseg > 1) seg = own_segments(a, r, s, log_decay);
+  launch_decay(a, q);
+  return {o, fin, seg, a.seg_tokens / 64};
 }
 
 // Writes dq, dk, dv ([B, T, H, D] views with unit inner stride); returns the gradient of the initial state if asked for.
 OptTensor op_decay_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& do_in,
                        const at::Tensor& log_decay, const OptTensor& state, const OptTensor& dstate,
                        const OptTensor& lengths, double scale, const at::Tensor& dq, const at::Tensor& dk,
-                       const at::Tensor& dv, bool want_dstate) {
+                       const at::Tensor& dv, bool want_dstate, const at::Tensor& fwd_segments, int64_t fwd_chunks) {
   const DecayShape s = decay_shape(q_in, log_decay);
   need_decay_input(k_in, q_in, "k");
   need_decay_input(v_in, q_in, "v");
@@ -386,7 +395,6 @@ OptTensor op_decay_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at:
   rv.reverse = 1, rv.intra = sc, rv.inter = 1.f, rv.kv = sc;
   rv.init = ds;
   rv.final_state = ds0 ? ds0->data_ptr<float>() : nullptr;
-  rv.segments_from = -1;
   DecayRole& rq = a.role[1];  // dq: state S transposed, first token to last
   set_in(dO, rq.q, rq.qb, rq.qt, rq.qh);
   set_in(v, rq.k, rq.kb, rq.kt, rq.kh);
@@ -395,7 +403,6 @@ OptTensor op_decay_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at:
   rq.intra = rq.inter = sc, rq.kv = 1.f;
   rq.init = state ? state->data_ptr<float>() : nullptr;
   rq.init_transposed = 1;
-  rq.segments_from = -1;
   DecayRole& rk = a.role[2];  // dk: dS transposed, last token to first
   set_in(v, rk.q, rk.qb, rk.qt, rk.qh);
   set_in(dO, rk.k, rk.kb, rk.kt, rk.kh);
@@ -404,9 +411,19 @@ OptTensor op_decay_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at:
   rk.reverse = 1, rk.intra = sc, rk.inter = 1.f, rk.kv = sc;
   rk.init = ds;
   rk.init_transposed = 1;
-  rk.segments_from = 0;
-  at::Tensor seg0, seg1;
-  launch_decay(a, s, log_decay, lengths, q, {&seg0, &seg1, nullptr});
+  set_tokens(a, s, log_decay, lengths, q);
+  const int per = chunks_to_a_segment(a, 3);
+  at::Tensor seg;
+  if (per * 64 >= a.T) {
+    set_segments(a, per, 1);
+  } else {  // fewer blocks for each role than the forward pass had: they take several of its segments each
+    TORCH_CHECK(fwd_segments.defined(), "nexar_b200: decay attention: the forward pass kept no states");
+    set_segments(a, (int)fwd_chunks, (int)((per + fwd_chunks - 1) / fwd_chunks));
+    seg = own_segments(a, rv, s, log_decay);
+    rk.segments = rv.segments;
+    rq.segments = fwd_segments.data_ptr<float>();
+  }
+  launch_decay(a, q);
   return ds0;
 }
 
@@ -580,9 +597,10 @@ struct DecayFn : public torch::autograd::Function<DecayFn> {
                                double scale, bool want_state) {
     ctx->set_materialize_grads(false);
     const auto a = parts(q, or_none(k), or_none(v));
-    auto [o, fin] = op_decay_fwd(a[0], a[1], a[2], log_decay, state, lengths, scale, want_state);
-    ctx->save_for_backward({q, or_none(k), or_none(v), log_decay, or_none(state), or_none(lengths)});
+    auto [o, fin, segments, chunks] = op_decay_fwd(a[0], a[1], a[2], log_decay, state, lengths, scale, want_state);
+    ctx->save_for_backward({q, or_none(k), or_none(v), log_decay, or_none(state), or_none(lengths), segments});
     ctx->saved_data["scale"] = scale;
+    ctx->saved_data["chunks"] = chunks;
     if (!want_state) return {o};
     return {o, *fin};
   }
@@ -604,7 +622,8 @@ struct DecayFn : public torch::autograd::Function<DecayFn> {
     if (d.size() > 1 && d[1].defined()) ds = d[1].contiguous();
     const OptTensor ds0 = op_decay_bwd(a[0], a[1], a[2], dO, saved[3], opt(saved[4]), ds, opt(saved[5]),
                                        ctx->saved_data["scale"].toDouble(), g[0], g[1], g[2],
-                                       saved[4].defined() && ctx->needs_input_grad(k.defined() ? 4 : 2));
+                                       saved[4].defined() && ctx->needs_input_grad(k.defined() ? 4 : 2), saved[6],
+                                       ctx->saved_data["chunks"].toInt());
     out[0] = k.defined() ? g[0] : packed;
     if (k.defined()) out[1] = g[1], out[2] = g[2];
     out[4] = or_none(ds0);
@@ -620,9 +639,9 @@ variable_list decay(const at::Tensor& q, const OptTensor& k, const OptTensor& v,
   if (any_grad({&q, ptr(k), ptr(v), ptr(state)}))
     return DecayFn::apply(q, k, v, log_decay, state, lengths, scale, want_state);
   const auto a = DecayFn::parts(q, or_none(k), or_none(v));
-  auto [o, fin] = op_decay_fwd(a[0], a[1], a[2], log_decay, state, lengths, scale, want_state);
-  if (!want_state) return {o};
-  return {o, *fin};
+  const auto out = op_decay_fwd(a[0], a[1], a[2], log_decay, state, lengths, scale, want_state);
+  if (!want_state) return {std::get<0>(out)};
+  return {std::get<0>(out), *std::get<1>(out)};
 }
 }  // namespace
 

@@ -72,8 +72,14 @@ def test_short_sequences(cuda0, T, D):
 @pytest.mark.parametrize("state", [True, False])
 def test_split_over_the_tokens(cuda0, B, T, H, D, state):
     """Few sequences and heads: several segments, the last one ragged."""
-    from nexar_b200 import _native  # noqa: F401
     _compare(cuda0, B, T, H, D, state=state)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,T,H,lengths", [(2, 3000, 4, [3000, 1234]), (1, 5000, 12, None), (3, 4097, 6, [0, 4097, 4000])])
+def test_long_sequences_split_in_both_passes(cuda0, B, T, H, lengths, D):
+    """The backward pass splits into fewer segments than the forward pass, whose states it reads."""
+    _compare(cuda0, B, T, H, D, lengths=lengths)
 
 
 @pytest.mark.parametrize("D", [64, 128])
