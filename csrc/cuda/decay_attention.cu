@@ -261,7 +261,19 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
     }
   }
 #pragma unroll
-  for (int n = 0; n < kX; ++n) X[n] = !x0 ? 0.f : x0[x0_t ? x_at_t(n) : x_at(n)];
+  for (int n = 0; n < kX; ++n) X[n] = 0.f;
+  if (x0) {
+    if (D == 128 && x0_t) {  // 256 bytes in a row for each thread
+#pragma unroll
+      for (int n = 0; n < kX; n += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(x0 + x_at_t(n));
+        X[n] = x.x, X[n + 1] = x.y, X[n + 2] = x.z, X[n + 3] = x.w;
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < kX; ++n) X[n] = x0[x0_t ? x_at_t(n) : x_at(n)];
+    }
+  }
   bool have = x0 != nullptr;  // a state that is known to be zero is not multiplied
   const bool want_final = STATES || (R.final_state != nullptr && a.nseg == 1);
   const int shift = R.reverse ? 0 : 1;  // exponents: i + shift and n - shift - j
@@ -712,21 +724,62 @@ unsigned int decay_error_flag() {
   return v;
 }
 
-// Whole sequences take `chunks` steps of a block that has its SM to itself (2.9 us
-// each for D = 64, 5.4 us for D = 128). n segments that fill every resident block
-// take ceil(chunks / n) steps of the main kernel beside its neighbours and of the
-// state-only one, 2.9 (D = 64) or 1.85 (D = 128) of those together, and the two
-// launches more 4.5 or 2.5. Measured whole / split, us: 12 heads of 64, T = 4096:
-// 184 / 33; 96 heads, T = 1024: 50 / 47; 60 heads, T = 1000: 49 / 37; 16 heads of
-// 128, T = 16385: 1386 / 165; 64 heads, T = 1024: 87 / 62; 128 heads: 93 / 102.
-int decay_segments(int B, int T, int H, int D, int roles) {
-  const int chunks = (T + kChunk - 1) / kChunk;
-  const long long blocks = (long long)B * H * roles, slots = 148LL * (D == 64 ? 3 : 2);
-  if (blocks > 148) return 1;
-  const long long n = slots / blocks < chunks ? slots / blocks : chunks;
-  const double steps = (double)((chunks + n - 1) / n);
-  const double split = D == 64 ? steps * 2.9 + 4.5 : steps * 1.85 + 2.5;
-  return split < chunks ? (int)n : 1;
+namespace {
+// us of one pass of the main kernel, by what it measured for 37 to 888 blocks of 4
+// to 32 chunks (within 8 %): a chunk takes 2.1, 3.2 or 4.2 us with one, two or three
+// blocks of heads of 64 on an SM and 4.2 or 5.6 us with one or two of heads of 128,
+// to which each wave of blocks and the launch add 2 to 2.5 us. The state-only kernel
+// takes half of each.
+double pass_us(long long blocks, long long chunks, int D) {
+  static const double kChunkUs[2][4] = {{0, 2.1, 3.2, 4.2}, {0, 4.2, 5.6, 5.6}};
+  const int slots = 148 * (D == 64 ? 3 : 2);
+  const double* us = kChunkUs[D != 64];
+  const long long waves = blocks / slots, rest = blocks % slots;
+  const double wave = D == 64 ? 2.5 : 2.0;
+  return 2.5 + waves * (wave + chunks * us[slots / 148]) + (rest ? wave + chunks * us[(rest + 147) / 148] : 0.);
+}
+double move_us(long long states, int D) { return states * (double)(D * D * 4) / 5e6; }  // out of L2 for the most part
+// States of n segments: written, then read and written by the scan, which has 8 of them in flight.
+double states_us(long long heads, long long n, long long chunks, int D) {
+  return 0.5 * pass_us(heads * n, chunks, D) + 3 * move_us(heads * n, D) + 5.0 + 0.7 * ((n + 7) / 8);
+}
+}  // namespace
+
+// Splitting the tokens pays where the heads alone leave SMs idle. Measured whole /
+// split, us, heads of 64: 12 of T = 4096: 135 / 32; 60 of T = 1000: 38.6 / 35; 96 of
+// T = 1024: 39 / 43; of 128: 16 of T = 16385: 1030 / 149; 48 of T = 4096: 266 / 113;
+// 128 of T = 1024: 77 / 93. With lengths, segments without a token end at once and
+// finer ones share the work out better: as many as fill every resident block (60
+// heads of 64 with 1 to 1000 tokens: 27 against 31).
+int decay_segment_chunks(int B, int T, int H, int D, bool ragged) {
+  const long long heads = (long long)B * H, chunks = (T + kChunk - 1) / kChunk;
+  long long best = chunks;
+  double us = pass_us(heads, chunks, D);
+  for (const int blocks : {37, 74, 148, 296, 444, 592, 740, 888}) {
+    const long long want = blocks / heads < chunks ? blocks / heads : chunks;
+    if (want < 2 || (ragged && blocks != 148 * (D == 64 ? 3 : 2))) continue;
+    const long long per = (chunks + want - 1) / want, n = (chunks + per - 1) / per;
+    const double split = pass_us(heads * n, per, D) + move_us(heads * n, D) + states_us(heads, n, per, D);
+    if (n > 1 && split < us) us = split, best = per;
+  }
+  return (int)best;
+}
+
+// The three uses of the backward pass need fewer segments to fill the GPU: a block
+// then takes several, the most where that is as fast. Measured whole / split, us,
+// heads of 64: 12 of T = 4096: 137 / 49; 48 of T = 4096: 150 / 123; of 128: 16 of
+// T = 16385: 1037 / 336; 40 of T = 4096: 265 / 240.
+int decay_backward_step(int B, int T, int H, int D, int chunks) {
+  const long long heads = (long long)B * H, all = (T + kChunk - 1) / kChunk, n = (all + chunks - 1) / chunks;
+  if (n < 2) return 0;
+  double us = pass_us(heads * 3, all, D) - states_us(heads, n, chunks, D);
+  int best = 0;
+  for (int step = n < 16 ? (int)n - 1 : 16; step >= 1; --step) {
+    const long long blocks = heads * 3 * ((n + step - 1) / step);
+    const double split = pass_us(blocks, (long long)step * chunks, D) + move_us(blocks, D);
+    if (split < us) us = split, best = step;
+  }
+  return best;
 }
 
 cudaError_t decay_attention(const DecayArgs& a, cudaStream_t s, int* launches) {

@@ -83,7 +83,10 @@ struct DecayArgs {
   // pieces one after the other.
   int nseg, seg_tokens, step;
 };
-int decay_segments(int B, int T, int H, int D, int roles);  // number of token segments worked on side by side
+// Chunks of 64 tokens to a segment of the forward pass (ragged: sequences have lengths of their own).
+int decay_segment_chunks(int B, int T, int H, int D, bool ragged);
+// Segments of so many chunks that a block of the backward pass takes; 0: whole sequences.
+int decay_backward_step(int B, int T, int H, int D, int chunks);
 cudaError_t decay_attention(const DecayArgs& a, cudaStream_t s, int* launches);
 unsigned int decay_error_flag();  // current GPU: not 0 once a wait inside decay_attention has given up (synchronises)
 // One token: state = lam state + k v^T in place, o = scale * state^T q. q, k, v rows with strides, o contiguous.

@@ -299,11 +299,6 @@ void set_tokens(DecayArgs& a, const DecayShape& s, const at::Tensor& log_decay, 
   a.lengths = decay_lengths(lengths, q);
   a.B = (int)s.B, a.T = (int)s.T, a.H = (int)s.H, a.D = (int)s.D;
 }
-// Chunks of 64 tokens to a segment.
-int chunks_to_a_segment(const DecayArgs& a, int roles) {
-  const int chunks = (a.T + 63) / 64, n = decay_segments(a.B, a.T, a.H, a.D, roles);
-  return (chunks + n - 1) / n;
-}
 void set_segments(DecayArgs& a, int chunks, int step) {
   a.seg_tokens = chunks * 64, a.step = step;
   a.nseg = (a.T + a.seg_tokens - 1) / a.seg_tokens;
@@ -352,7 +347,7 @@ std::tuple<at::Tensor, OptTensor, at::Tensor, int64_t> op_decay_fwd(const at::Te
   r.init = state ? state->data_ptr<float>() : nullptr;
   r.final_state = fin ? fin->data_ptr<float>() : nullptr;
   set_tokens(a, s, log_decay, lengths, q);
-  set_segments(a, chunks_to_a_segment(a, 1), 1);
+  set_segments(a, decay_segment_chunks(a.B, a.T, a.H, a.D, a.lengths != nullptr), 1);
   at::Tensor seg;
   if (a.nseg > 1) seg = own_segments(a, r, s, log_decay);
   launch_decay(a, q);
@@ -412,13 +407,12 @@ OptTensor op_decay_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at:
   rk.init = ds;
   rk.init_transposed = 1;
   set_tokens(a, s, log_decay, lengths, q);
-  const int per = chunks_to_a_segment(a, 3);
+  const int step = fwd_segments.defined() ? decay_backward_step(a.B, a.T, a.H, a.D, (int)fwd_chunks) : 0;
   at::Tensor seg;
-  if (per * 64 >= a.T) {
-    set_segments(a, per, 1);
-  } else {  // fewer blocks for each role than the forward pass had: they take several of its segments each
-    TORCH_CHECK(fwd_segments.defined(), "nexar_b200: decay attention: the forward pass kept no states");
-    set_segments(a, (int)fwd_chunks, (int)((per + fwd_chunks - 1) / fwd_chunks));
+  if (step == 0) {
+    set_segments(a, (a.T + 63) / 64, 1);
+  } else {
+    set_segments(a, (int)fwd_chunks, step);
     seg = own_segments(a, rv, s, log_decay);
     rk.segments = rv.segments;
     rq.segments = fwd_segments.data_ptr<float>();
