@@ -34,8 +34,17 @@
 // With D = 128 the value dimension fills the 128 lanes, X^T stays with its rows'
 // threads and goes back through TMEM, over the columns of U, which is done by then;
 // o = lam^(i+1) O2 + O1 at the end. Rows come by cp.async, each thread its 16-byte
-// groups (a reversed role simply reads its rows from the end): tensor-map loads of
-// the same tiles measured 17 to 25 % slower here, with D = 128.
+// groups (a reversed role simply reads its rows from the end): with D = 128 the
+// state fills the 128 registers that two blocks per SM leave a thread, and a form
+// with tensor-map loads, which spilled some, took 17 to 25 % longer.
+//
+// Measured, forward / backward: 8 x 1024 tokens of 12 heads of 64: 37 / 55 us (the
+// 138 MB that they have to move take 21 us); 16385 tokens of 16 heads of 128: 142 /
+// 309 us (742 MB, 113 us), of which the states before the segments and the scan are
+// 57 us each. With a full grid an SM issues in 53 to 58 % of its cycles and the
+// tensor pipe works in 34 to 36 %: bound by the instructions that decay, round and
+// split operands between one chunk's two groups of products and by the latency of
+// that chain, which the two or three blocks of an SM do not cover in full.
 //
 // Roundings. Products are bf16 tensor-core products with fp32 sums. The decayed
 // keys that enter the state are split into three bf16 parts (24 bits, all of an
@@ -46,7 +55,8 @@
 // thousands of tokens would add up.
 //
 // Every wait is bounded (2 s); one that gives up sets an error word of its GPU
-// (decay_error_flag), the block leaves together and frees its TMEM.
+// (decay_error_flag), and its block leaves together, with NaN in its rows and its
+// state, and frees its TMEM.
 #include "common.cuh"
 #include "decoder_api.h"
 #include "sm100.cuh"
@@ -573,17 +583,22 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
     tc_fence_before();
   }
 
+  ok = __syncthreads_and(ok);
   if constexpr (!STATES) {
-    // rows of the batch that hold no token (index >= length) give zeros
+    // rows of the batch that hold no token (index >= length) give zeros; where a wait gave up, all are NaN
     __nv_bfloat16* rows = R.out + b * R.ob + h * R.oh;
-    const int from = max(t_begin, min(len, t_end));
-    for (int e = tid; e < (t_end - from) * kGroups; e += S::kThreads)
-      *reinterpret_cast<uint4*>(rows + (long long)(from + e / kGroups) * R.ot + (e % kGroups) * 8) = make_uint4(0, 0, 0, 0);
+    const uint32_t fill = ok ? 0u : 0x7fc07fc0u;
+    const int from = ok ? max(t_begin, min(len, t_end)) : t_begin;
+    for (int e = tid; e < (t_end - from) * kGroups; e += S::kThreads) {
+      const int i = from + e / kGroups;
+      *reinterpret_cast<uint4*>(rows + (long long)(i < len ? origin + dir * i : i) * R.ot + (e % kGroups) * 8) =
+          make_uint4(fill, fill, fill, fill);
+    }
   }
   if (want_final) {
     float* dst = STATES ? R.segments + ((size_t)bh * a.nseg + seg) * D * D : R.final_state + (size_t)bh * D * D;
 #pragma unroll
-    for (int n = 0; n < kX; ++n) dst[x_at(n)] = X[n];
+    for (int n = 0; n < kX; ++n) dst[x_at(n)] = ok ? X[n] : __int_as_float(0x7fc00000);
   }
   cp_wait<0>();
   tc_fence_before();
@@ -644,7 +659,9 @@ template <int D> __global__ void __launch_bounds__(256) k_decay_scan(const __gri
 
 // One token: a block per (sequence, head). Each thread holds 4 columns of every
 // eighth row (D = 64: 16 threads to a row; D = 128: a warp), updates them in
-// place and sums its part of q^T S; bound by reading and writing the state.
+// place and sums its part of q^T S; bound by reading and writing the state: 192
+// sequences of 32 heads of 128 in 119 us, 6.8 TB/s (812 MB). A few heads take 2.2
+// us, the latency of one load, one barrier and one store.
 template <int D> __global__ void __launch_bounds__(D * 2) k_decay_step(const DecayStepArgs a) {
   constexpr int kRow = D / 4;             // threads per row
   constexpr int kRows = 8;                // rows at a time

@@ -212,6 +212,11 @@ std::vector<at::Tensor> op_dropout_ln_fwd(const at::Tensor& x, const at::Tensor&
   return {s, y, mean, rstd, snap};
 }
 
+// Kernels read gradients in 16-byte groups: one that autograd was handed at another address is copied.
+at::Tensor grad_rows(const at::Tensor& t) {
+  return t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t
+                                                                                  : t.clone(at::MemoryFormat::Contiguous);
+}
 // Returns dx, dr; writes dw, db (and drb).
 std::vector<at::Tensor> op_dropout_ln_bwd(const at::Tensor& dy, const at::Tensor& s, const at::Tensor& mean,
                                           const at::Tensor& rstd, const at::Tensor& w, const OptTensor& dres,
@@ -250,7 +255,7 @@ std::vector<at::Tensor> op_dropout_ln_bwd(const at::Tensor& dy, const at::Tensor
 at::Tensor row_view(const at::Tensor& t) {
   bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
-  return ok ? t : t.contiguous();
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);  // not contiguous(): it may be, at an odd address
 }
 void need_decay_input(const at::Tensor& t, const at::Tensor& q, const char* name) {
   same_device(t, q, name);
@@ -564,9 +569,9 @@ struct DropoutLayerNormFn : public torch::autograd::Function<DropoutLayerNormFn>
   static variable_list backward(AutogradContext* ctx, variable_list d) {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &s = saved[0], &w = saved[1], &rb = saved[5];
-    const at::Tensor dy = d[1].defined() ? d[1].contiguous() : at::zeros_like(s);
+    const at::Tensor dy = d[1].defined() ? grad_rows(d[1]) : at::zeros_like(s);
     OptTensor ds, drb;
-    if (d[0].defined()) ds = d[0].contiguous();
+    if (d[0].defined()) ds = grad_rows(d[0]);
     if (rb.defined()) drb = at::empty_like(rb);
     at::Tensor dw = at::empty_like(w), db = at::empty_like(w);
     auto g = op_dropout_ln_bwd(dy, s, saved[2], saved[3], w, ds, dw, db, drb, saved[4],
@@ -613,7 +618,7 @@ struct DecayFn : public torch::autograd::Function<DecayFn> {
     }
     const at::Tensor dO = d[0].defined() ? d[0] : at::zeros(a[0].sizes(), q.options());
     OptTensor ds;
-    if (d.size() > 1 && d[1].defined()) ds = d[1].contiguous();
+    if (d.size() > 1 && d[1].defined()) ds = grad_rows(d[1]);
     const OptTensor ds0 = op_decay_bwd(a[0], a[1], a[2], dO, saved[3], opt(saved[4]), ds, opt(saved[5]),
                                        ctx->saved_data["scale"].toDouble(), g[0], g[1], g[2],
                                        saved[4].defined() && ctx->needs_input_grad(k.defined() ? 4 : 2), saved[6],

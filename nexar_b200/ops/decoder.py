@@ -3,7 +3,8 @@ counter-based dropout and attention with a decay per head.
 
 Every function calls the sm_100a kernels on the current stream of its input's
 GPU and allocates its outputs and workspaces there, so calls can be captured
-into CUDA graphs and run on any stream or device.
+into CUDA graphs and run on any stream or device. (As for every operator of torch, a
+backward pass is captured only when no eager graph of the same leaves is alive.)
 """
 from __future__ import annotations
 
@@ -128,7 +129,9 @@ class DropoutState:
     Every call takes its numbers from (seed, step, site, element): ``site`` tells the calls of one
     step apart, :meth:`advance` moves to the next step. The kernels read the values on the device, so a
     captured graph that contains :meth:`advance` draws anew at every replay. Data-parallel ranks use
-    different seeds; calls with the same seed, step and site draw the same mask."""
+    different seeds; calls with the same seed, step (modulo 2^32) and site draw the same mask. A backward
+    pass uses the values that its forward pass found; a forward pass that is run again (recomputation)
+    has to run before :meth:`advance`."""
 
     def __init__(self, seed: int, device=None, step: int = 0):
         device = torch.device("cuda") if device is None else torch.device(device)

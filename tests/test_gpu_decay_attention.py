@@ -93,6 +93,38 @@ def test_steep_and_absent_decays(cuda0, decays, T):
     _compare(cuda0, 1, T, 4, 64, decays=decays)
 
 
+@pytest.mark.parametrize("T", [70, 600])
+def test_a_decay_to_nothing(cuda0, T):
+    """exp(-inf) and exp(-1e4) are both 0: a token sees itself alone."""
+    from nexar_b200 import ops
+    q, k, v, do, s0, ds, _ = _inputs(cuda0, 2, T, 3, 128, 5)
+    got = []
+    for g in (float("-inf"), -1e4):
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v, s0)]
+        o, s = ops.decay_attention(*leaves[:3], torch.full((3,), g, device=cuda0), state=leaves[3], return_state=True)
+        got.append((o.detach(), s.detach()) + torch.autograd.grad((o, s), leaves, (do, ds)))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_tensors_at_any_address(cuda0):
+    """Inputs and gradients that are handed over as contiguous views at odd addresses."""
+    from nexar_b200 import ops
+    q, k, v, do, s0, ds, lam = _inputs(cuda0, 1, 70, 2, 64, 6)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+
+    def moved(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=cuda0)
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view_as(t)
+
+    def run(qkv, a, b):
+        o, s = ops.decay_attention(*qkv, lam, return_state=True)
+        return (o.detach(), s.detach()) + torch.autograd.grad((o, s), qkv, (a, b))
+    odd = [moved(t.detach()).requires_grad_(True) for t in leaves]
+    assert all(t.data_ptr() % 16 == 2 for t in odd)
+    assert all(torch.equal(x, y) for x, y in zip(run(leaves, do, ds), run(odd, moved(do), moved(ds))))
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("T,lengths", [(100, [0, 1, 64, 99, 100, 37]), (900, [900, 0, 1, 128, 513, 899]), (5, [0, 0])])
 def test_lengths(cuda0, T, lengths, D):

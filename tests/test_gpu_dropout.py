@@ -196,6 +196,22 @@ def test_residual_partial_gradients_and_rerun(cuda0):
     assert torch.equal(only_s[0], ds) and not only_s[2].any()
 
 
+def test_residual_gradients_at_any_address(cuda0):
+    from nexar_b200 import ops
+    x, r, ds, dy, w, b, rb = _inputs(cuda0, 20, 64, True, 8)
+    leaves = [t.requires_grad_(True) for t in (x, r, w, b, rb)]
+    state = ops.DropoutState(4, cuda0)
+
+    def moved(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=cuda0)
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view_as(t)
+
+    def run(a, c):
+        return torch.autograd.grad(ops.residual_layer_norm(x, r, w, b, 1e-5, rbias=rb, p=0.1, dropout=state), leaves, (a, c))
+    assert all(torch.equal(a, c) for a, c in zip(run(ds, dy), run(moved(ds), moved(dy))))
+
+
 def test_residual_without_dropout_is_unchanged(cuda0):
     from nexar_b200 import ops
     x, r, ds, dy, w, b, rb = _inputs(cuda0, 64, 768, True)

@@ -91,6 +91,21 @@ def test_strided_heads_of_a_packed_projection(cuda0, layout):
         oracle.assert_within(y, want, _bound(x, want, m))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cut", [1, 2, 4])
+def test_heads_at_any_address(cuda0, dtype, cut):
+    """Rows that start `cut` elements behind an aligned address, with strides to match."""
+    from nexar_b200 import ops
+    g = torch.Generator(device=cuda0).manual_seed(cut)
+    wide = torch.randn(2, 9, 4, 64 + cut, device=cuda0, generator=g).to(dtype)
+    x = wide[..., cut:]
+    flat = torch.empty(x.numel() + cut, dtype=dtype, device=cuda0)[cut:].view(2, 9, 4, 64).copy_(x)
+    table = ops.rotary_table(16, 32, device=cuda0)
+    want = ops.rotary(x.contiguous(), table, start=3)
+    assert torch.equal(ops.rotary(x, table, start=3), want)
+    assert torch.equal(ops.rotary(flat, table, start=3), want)
+
+
 def test_pair_and_packed_forms_agree_with_the_single_one(cuda0):
     from nexar_b200 import ops
     B, T, H, Hk, D = 2, 33, 8, 2, 128
