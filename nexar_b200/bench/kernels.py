@@ -18,6 +18,13 @@ names:
                and torch SDPA (cuDNN) forward and forward + backward
   compress     top-1 % + e4m3 compression of 64 Mi bf16 values
   ln_bwd       LayerNorm backward, 8192 x 768 with the bias-gradient sums
+  rotary       rotary positions of 65537 tokens of 32 query and 8 key heads of
+               128, 96 elements of each turned (k_rotary)
+  dropout_ln   residual add + dropout + LayerNorm of 32768 rows of 2048, forward
+               (k_dropout_ln_fwd) and backward (k_dropout_ln_bwd, _columns)
+  decay        attention with a decay per head, 16385 tokens of 16 heads of 128,
+               forward and backward (k_decay_chunk, k_decay_scan)
+  decay_step   one token of 192 sequences of 32 heads of 128 (k_decay_step)
 
 Each run prints one JSON line with the CUDA-event time per launch (after two
 warm-up launches). Inputs are a few hundred MB at most.
@@ -139,6 +146,43 @@ def main():
         ds = torch.randn_like(s)
         ms = _time(lambda: torch.autograd.grad([s, y], [x, w, b, rb], [ds, dy], retain_graph=True), args.iters)
         rec.update(R=R, C=Cn, us=round(ms * 1e3, 1), gbs=round(R * Cn * 2 * 4 / ms / 1e6, 1))
+    elif args.name == "rotary":
+        T, D, R = 65537, 128, 96
+        q, k = (torch.randn(1, T, h, D, device=dev, generator=g).to(torch.bfloat16) for h in (32, 8))
+        table = ops.rotary_table(T, R, device=dev)
+        ms = _time(lambda: ops.rotary_qk(q, k, table, layout="interleaved"), args.iters)
+        rec.update(T=T, heads=40, D=D, R=R, us=round(ms * 1e3, 1), gbs=round(T * 40 * D * 4 / ms / 1e6, 1))
+    elif args.name == "dropout_ln":
+        R, Cn = 32768, 2048
+        x, r, ds, dy = (torch.randn(R, Cn, device=dev, generator=g).to(torch.bfloat16) for _ in range(4))
+        w, b, rb = (torch.ones(Cn, device=dev, dtype=torch.bfloat16) for _ in range(3))
+        state = ops.DropoutState(0, dev)
+        ms = _time(lambda: C.dropout_ln_fwd(x, r, rb, w, b, 1e-5, state.tensor, 0, 0.1), args.iters)
+        s, _, mean, rstd, used = C.dropout_ln_fwd(x, r, rb, w, b, 1e-5, state.tensor, 0, 0.1)
+        dw, db, drb = (torch.empty_like(w) for _ in range(3))
+        bms = _time(lambda: C.dropout_ln_bwd(dy, s, mean, rstd, w, ds, dw, db, drb, used, 0, 0.1), args.iters)
+        rec.update(R=R, C=Cn, fwd_us=round(ms * 1e3, 1), bwd_us=round(bms * 1e3, 1),
+                   fwd_gbs=round(R * Cn * 8 / ms / 1e6, 1), bwd_gbs=round(R * Cn * 10 / bms / 1e6, 1))
+    elif args.name == "decay":
+        T, H, D = 16385, 16, 128
+        q, k, v = (torch.randn(1, T, H, D, device=dev, generator=g).to(torch.bfloat16).requires_grad_(True)
+                   for _ in range(3))
+        do = torch.randn(1, T, H, D, device=dev, generator=g).to(torch.bfloat16)
+        lam = torch.linspace(-0.05, -0.001, H, device=dev)
+        with torch.no_grad():
+            ms = _time(lambda: ops.decay_attention(q, k, v, lam), args.iters)
+        o = ops.decay_attention(q, k, v, lam)
+        bms = _time(lambda: torch.autograd.grad(o, [q, k, v], do, retain_graph=True), args.iters)
+        rec.update(T=T, H=H, D=D, fwd_us=round(ms * 1e3, 1), bwd_us=round(bms * 1e3, 1),
+                   fwd_gbs=round(T * H * D * 8 / ms / 1e6, 1), bwd_gbs=round(T * H * D * 14 / bms / 1e6, 1),
+                   wait_flag=int(C.decay_error_flag()))
+    elif args.name == "decay_step":
+        Bn, H, D = 192, 32, 128
+        q, k, v = (torch.randn(Bn, H, D, device=dev, generator=g).to(torch.bfloat16) for _ in range(3))
+        lam = torch.linspace(-0.05, -0.001, H, device=dev)
+        state = torch.zeros(Bn, H, D, D, device=dev)
+        ms = _time(lambda: ops.decay_attention_step(q, k, v, lam, state), args.iters)
+        rec.update(B=Bn, H=H, D=D, us=round(ms * 1e3, 1), gbs=round(Bn * H * (D * D * 8 + D * 8) / ms / 1e6, 1))
     else:
         raise SystemExit(f"unknown kernel workload {args.name}")
     rec["err_flag"] = int(C.gemm_error_flag())

@@ -335,3 +335,22 @@ def test_empty_and_refusals(cuda0):
     for f in bad:
         with pytest.raises(RuntimeError, match="nexar_b200"):
             f()
+
+
+def test_inference_mode(cuda0):
+    """Under inference_mode, on inference tensors, every operator gives what it gives outside."""
+    from nexar_b200 import ops
+    q, k, v, do, s0, ds, lam = _inputs(cuda0, 2, 70, 2, 64, 7)
+    drop = ops.DropoutState(3, cuda0)
+    w = torch.ones(64, dtype=torch.bfloat16, device=cuda0)
+
+    def run():
+        table = ops.rotary_table(70, 64, device=cuda0)
+        a, b = ops.rotary_qk(q * 1, k * 1, table)
+        o, s = ops.decay_attention(a, b, v, lam, return_state=True)
+        t = ops.decay_attention_step(a[:, 0], b[:, 0], v[:, 0], lam, s)
+        return (o, s, t, ops.dropout(o, 0.2, drop)) + ops.residual_layer_norm(o, v, w, w, p=0.1, dropout=drop)
+    want = run()
+    with torch.inference_mode():
+        got = run()
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
