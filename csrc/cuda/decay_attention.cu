@@ -24,8 +24,8 @@
 // end; P: the decayed and masked scores):
 //     D = 64:   S [token, token] = Q K^T, O [token, dv] = Q X;
 //               then O = lam^(i+1) O + P V, U [dk, dv] = K'^T V
-//     D = 128:  S [token, token] = Q K^T;
-//               then O2 [dv, token] = X^T Q^T, O1 [dv, token] = V^T P^T, U [dv, dk] = V^T K'
+//     D = 128:  S [token, token] = Q K^T, O2 [dv, token] = X^T Q^T;
+//               then O1 [dv, token] = V^T P^T, U [dv, dk] = V^T K'
 // The first group runs while K' is written; two (D = 128) or three (D = 64) blocks
 // per SM fill each other's gaps during the second. With D = 64 the 64 rows of every
 // accumulator are read as matrix fragments (16 lanes per warp), X goes back as an
@@ -39,7 +39,7 @@
 // with tensor-map loads, which spilled some, took 17 to 25 % longer.
 //
 // Measured, forward / backward: 8 x 1024 tokens of 12 heads of 64: 37 / 55 us (the
-// 138 MB that they have to move take 21 us); 16385 tokens of 16 heads of 128: 142 /
+// 138 MB that they have to move take 21 us); 16385 tokens of 16 heads of 128: 141 /
 // 309 us (742 MB, 113 us), of which the states before the segments and the scan are
 // 57 us each. With a full grid an SM issues in 53 to 58 % of its cycles and the
 // tensor pipe works in 34 to 36 %: bound by the instructions that decay, round and
@@ -86,12 +86,24 @@ NEXAR_D void fma2(float& x0, float& x1, float f, float u0, float u1) {
       "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
       : "+f"(x0), "+f"(x1) : "f"(f), "f"(u0), "f"(u1));
 }
+// x, y times f.
+NEXAR_D void mul2(float& x, float& y, float f) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\t"
+      "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(x), "+f"(y) : "f"(f));
+}
 NEXAR_D uint32_t bf2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 NEXAR_D float bf_lo(uint32_t v) { return __uint_as_float(v << 16); }
 NEXAR_D float bf_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+NEXAR_D uint32_t split2(float& x, float& y) {  // the pair's bf16 part; x, y keep the rest
+  const uint32_t p = bf2(x, y);
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "sub.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(x), "+f"(y) : "f"(bf_lo(p)), "f"(bf_hi(p)));
+  return p;
+}
 
 // A tile of 64 rows x D bf16 is D / 64 boxes of 64 rows x 128 bytes in the
 // 128-byte-swizzled layout of the tcgen05 descriptors: 16-byte group g of row r.
@@ -124,13 +136,10 @@ NEXAR_D void warp_commit(uint64_t* bar) {
       "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
       :: "r"(smem_u32(bar)) : "memory");
 }
-NEXAR_D void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-      :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+NEXAR_D void tmem_st_x8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 // 16 lanes x 32 columns as matrix fragments: r[4 n + e] is row lane / 4 + 8 (e / 2), column 8 n + 2 (lane % 4) + e % 2.
 NEXAR_D void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {
@@ -304,11 +313,30 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
       if (have) {  // ---- the state as an operand: two bf16 parts
 #pragma unroll
         for (int n = 0; n < kX; n += 2) {
-          const uint32_t hi = bf2(X[n], X[n + 1]), lo = bf2(X[n] - bf_lo(hi), X[n + 1] - bf_hi(hi));
+          float x = X[n], y = X[n + 1];
+          const uint32_t hi = split2(x, y), lo = bf2(x, y);
           unsigned char* at = smem + S::kScores + tile_at(xr + (n & 2) * 4, half * 4 + (n >> 2)) + xc * 2;
           *reinterpret_cast<uint32_t*>(at) = hi;
           *reinterpret_cast<uint32_t*>(at + 8192) = lo;
         }
+      }
+    }
+    if constexpr (!STATES && D == 128) {
+      if (have) {  // ---- the same, X^T; everyone has read U, whose columns it takes, before the last barrier
+#pragma unroll
+        for (int n = 0; n < kX; n += 16) {
+          uint32_t hi[8], lo[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float x = X[n + 2 * e], y = X[n + 2 * e + 1];
+            hi[e] = split2(x, y);
+            lo[e] = bf2(x, y);
+          }
+          tmem_st_x8(lanes + half * 32 + n / 2, hi);
+          tmem_st_x8(lanes + 64 + half * 32 + n / 2, lo);
+        }
+        tmem_st_wait();
+        tc_fence_before();
       }
     }
     cp_wait<0>();
@@ -338,6 +366,14 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
               warp_mma(tbase + 64, kq + k * 2, mx + p * 512 + 128 * k, umma_idesc_bf16_f32(64, 64, false, true), p == 0 || k > 0);
         }
         warp_commit(s_done);
+        if (D == 128 && have) {
+#pragma unroll
+          for (int p = 1; p >= 0; --p)
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              warp_mma_ts(tbase + D + 64, tbase + p * 64 + k * 8, kq + (k >> 2) * 512 + (k & 3) * 2,
+                          umma_idesc_bf16_f32(D, 64), p == 0 || k > 0);
+        }
       }
       __syncwarp();
     }
@@ -353,11 +389,11 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
         uint32_t p0[4], p1[4], p2[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float x = bf_lo(kw[q]) * w, y = bf_hi(kw[q]) * w;
-          p0[q] = bf2(x, y);
-          const float x1 = x - bf_lo(p0[q]), y1 = y - bf_hi(p0[q]);
-          p1[q] = bf2(x1, y1);
-          p2[q] = bf2(x1 - bf_lo(p1[q]), y1 - bf_hi(p1[q]));
+          float x = bf_lo(kw[q]), y = bf_hi(kw[q]);
+          mul2(x, y, w);
+          p0[q] = split2(x, y);
+          p1[q] = split2(x, y);
+          p2[q] = bf2(x, y);
         }
         unsigned char* dst = smem + S::kKeys + at0 + u * kRows * 128;
         *reinterpret_cast<uint4*>(dst) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
@@ -366,23 +402,6 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
       }
     }
     if constexpr (!STATES) {
-      if (D == 128 && have) {  // ---- the state as an operand: two bf16 parts
-        if constexpr (D == 128) {
-#pragma unroll
-          for (int n = 0; n < kX; n += 32) {
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float x = X[n + 2 * e], y = X[n + 2 * e + 1];
-              hi[e] = bf2(x, y);
-              lo[e] = bf2(x - bf_lo(hi[e]), y - bf_hi(hi[e]));
-            }
-            tmem_st_x16(lanes + half * 32 + n / 2, hi);
-            tmem_st_x16(lanes + 64 + half * 32 + n / 2, lo);
-          }
-          tmem_st_wait();
-        }
-      }
       // ---- P: 16 query rows and 32 key columns per warp, up to the diagonal
       if (!wait_phase(s_done, c & 1)) {
         ok = false;
@@ -442,8 +461,8 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-              const float u = P[n][2 * p], v = P[n][2 * p + 1];
-              const uint32_t hi = bf2(u, v), lo = bf2(u - bf_lo(hi), v - bf_hi(hi));
+              float u = P[n][2 * p], v = P[n][2 * p + 1];
+              const uint32_t hi = split2(u, v), lo = bf2(u, v);
               unsigned char* at = smem + S::kScores + tile_at(xr + 8 * p, 2 * kb + n) + xc * 2;
               *reinterpret_cast<uint32_t*>(at) = hi;
               *reinterpret_cast<uint32_t*>(at + 8192) = lo;
@@ -461,15 +480,6 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
       if constexpr (!STATES) {
         constexpr uint32_t id1 = umma_idesc_bf16_f32(D, 64, D == 128, D == 64);
         const uint64_t kp = umma_desc_sw128_kmajor(base + S::kScores);
-        if (D == 128 && have) {
-          const uint64_t kq = umma_desc_sw128_kmajor(tq);
-#pragma unroll
-          for (int p = 1; p >= 0; --p)
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              warp_mma_ts(tbase + D + 64, tbase + p * 64 + k * 8, kq + (k >> 2) * 512 + (k & 3) * 2,
-                          umma_idesc_bf16_f32(D, 64), p == 0 || k > 0);
-        }
 #pragma unroll
         for (int p = 1; p >= 0; --p)
 #pragma unroll
@@ -744,11 +754,11 @@ unsigned int decay_error_flag() {
 namespace {
 // us of one pass of the main kernel, by what it measured for 37 to 888 blocks of 4
 // to 32 chunks (within 8 %): a chunk takes 2.1, 3.2 or 4.2 us with one, two or three
-// blocks of heads of 64 on an SM and 4.2 or 5.6 us with one or two of heads of 128,
+// blocks of heads of 64 on an SM and 3.8 or 5.4 us with one or two of heads of 128,
 // to which each wave of blocks and the launch add 2 to 2.5 us. The state-only kernel
 // takes half of each.
 double pass_us(long long blocks, long long chunks, int D) {
-  static const double kChunkUs[2][4] = {{0, 2.1, 3.2, 4.2}, {0, 4.2, 5.6, 5.6}};
+  static const double kChunkUs[2][4] = {{0, 2.1, 3.2, 4.2}, {0, 3.8, 5.4, 5.4}};
   const int slots = 148 * (D == 64 ? 3 : 2);
   const double* us = kChunkUs[D != 64];
   const long long waves = blocks / slots, rest = blocks % slots;
@@ -763,9 +773,9 @@ double states_us(long long heads, long long n, long long chunks, int D) {
 }  // namespace
 
 // Splitting the tokens pays where the heads alone leave SMs idle. Measured whole /
-// split, us, heads of 64: 12 of T = 4096: 135 / 32; 60 of T = 1000: 38.6 / 35; 96 of
-// T = 1024: 39 / 43; of 128: 16 of T = 16385: 1030 / 149; 48 of T = 4096: 266 / 113;
-// 128 of T = 1024: 77 / 93. With lengths, segments without a token end at once and
+// split, us, heads of 64: 12 of T = 4096: 135 / 33; 60 of T = 1000: 39 / 37; 96 of
+// T = 1024: 39 / 43; of 128: 16 of T = 16385: 936 / 144; 48 of T = 4096: 242 / 111;
+// 128 of T = 1024: 68 / 90. With lengths, segments without a token end at once and
 // finer ones share the work out better: as many as fill every resident block (60
 // heads of 64 with 1 to 1000 tokens: 27 against 31).
 int decay_segment_chunks(int B, int T, int H, int D, bool ragged) {
@@ -785,7 +795,7 @@ int decay_segment_chunks(int B, int T, int H, int D, bool ragged) {
 // The three uses of the backward pass need fewer segments to fill the GPU: a block
 // then takes several, the most where that is as fast. Measured whole / split, us,
 // heads of 64: 12 of T = 4096: 137 / 49; 48 of T = 4096: 150 / 123; of 128: 16 of
-// T = 16385: 1037 / 336; 40 of T = 4096: 265 / 240.
+// T = 16385: 940 / 300; 40 of T = 4096: 238 / 202.
 int decay_backward_step(int B, int T, int H, int D, int chunks) {
   const long long heads = (long long)B * H, all = (T + kChunk - 1) / kChunk, n = (all + chunks - 1) / chunks;
   if (n < 2) return 0;
