@@ -496,8 +496,9 @@ cudaError_t dropout_ln_bwd(const __nv_bfloat16* dy, const __nv_bfloat16* s_in, c
   const int grid = bwd_blocks(R, C), threads = (C / 8 + 31) / 32 * 32;
   const int ring = kBwdStages * kBwdRows * 3 * threads * 16;
   const auto kernel = drb ? k_dropout_ln_bwd<true> : k_dropout_ln_bwd<false>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       kBwdStages * kBwdRows * 3 * 256 * 16);
+  cudaError_t e = cudaSuccess;
+  if (ring > 48 * 1024)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdStages * kBwdRows * 3 * 256 * 16);
   if (e != cudaSuccess) return e;
   kernel<<<grid, threads, ring, s>>>(dy, s_in, mean, rstd, w, dres, dx, dr, scratch, R, C, state, site, threshold,
                                      scale);
