@@ -74,7 +74,9 @@ def rotary_frequencies(dim: int, base: float = 10000.0,
         def pair_of(turns):  # the (fractional) pair that turns this often in the original length
             return dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
         first = max(math.floor(pair_of(scaling.fast)), 0)
-        last = min(math.ceil(pair_of(scaling.slow)), n - 1)
+        # the ramp may end behind the last pair (n - 1): where every pair turns more than ``slow`` times,
+        # none is stretched in full
+        last = min(math.ceil(pair_of(scaling.slow)), dim - 1)
         keep = [1.0 - min(max((i - first) / max(last - first, 1e-3), 0.0), 1.0) for i in range(n)]
         magnitude = 0.1 * math.log(f) + 1.0 if scaling.magnitude is None else scaling.magnitude
     return [w / f * (1.0 - k) + w * k for w, k in zip(freq, keep)], magnitude

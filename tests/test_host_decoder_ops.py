@@ -42,6 +42,35 @@ def test_bands_and_yarn_keep_the_fast_pairs_and_stretch_the_slow_ones():
     assert m == 1.0
 
 
+def _yarn_by_definition(dim, base, factor, length, fast=32.0, slow=1.0):
+    """The ramp runs over the pairs from the one that turns ``fast`` times in the original length to the one that
+    turns ``slow`` times (a pair's number is real: turns(x) = length base^(-2 x / dim) / 2 pi), widened to whole
+    numbers and held inside 0 .. dim - 1."""
+    def pair_with(turns):
+        lo, hi = -2.0 * dim, 2.0 * dim
+        for _ in range(200):  # the number of turns falls with the pair
+            mid = (lo + hi) / 2
+            lo, hi = (mid, hi) if length * base ** (-2 * mid / dim) / (2 * math.pi) > turns else (lo, mid)
+        return (lo + hi) / 2
+    first, last = max(math.floor(pair_with(fast)), 0), min(math.ceil(pair_with(slow)), dim - 1)
+    out = []
+    for i in range(dim // 2):
+        plain = base ** (-2 * i / dim)
+        share = 0.0 if i <= first else min((i - first) / (last - first), 1.0)  # before the ramp: as trained
+        out.append(plain * (1 - share) + plain / factor * share)
+    return out
+
+
+@pytest.mark.parametrize("dim,base,factor,length", [
+    (128, 10000.0, 8.0, 4096), (64, 10000.0, 16.0, 8192),         # the slowest pairs turn less than once
+    (128, 10000.0, 4.0, 65536), (64, 10000.0, 4.0, 131072), (128, 10000.0, 4.0, 262144),  # all turn more than once
+    (96, 500.0, 2.0, 100000), (128, 10000.0, 4.0, 10 ** 12)])     # the ramp's end at the last number it may take
+def test_yarn_frequencies_by_definition(dim, base, factor, length):
+    f, _ = ops.rotary_frequencies(dim, base, ops.RotaryScaling("yarn", factor, length))
+    for got, want in zip(f, _yarn_by_definition(dim, base, factor, length)):
+        assert got == pytest.approx(want, rel=1e-12)
+
+
 def test_philox_known_answers():
     """The published test vectors of Philox4x32-10 (Random123)."""
     assert oracle.philox_words((0, 0, 0, 0), (0, 0)) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
