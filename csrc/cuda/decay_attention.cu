@@ -207,7 +207,8 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
                                                           // over hundreds of chunks that error would add up
   uint64_t* done = reinterpret_cast<uint64_t*>(smem + S::kMisc + 320);
   uint64_t* s_done = done + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kMisc + 336);
+  uint64_t* x_done = done + 2;  // D = 128: the products that read X^T
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kMisc + 344);
   const uint32_t base = smem_u32(smem);
 
   // A thread moves 16-byte group g0 of rows r0, r0 + kRows, ... of every tile. Token index i sits at row i, or at
@@ -240,6 +241,7 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
   if (tid == 0) {
     mbar_init(done, 1);
     mbar_init(s_done, 1);
+    mbar_init(x_done, 1);
     mbar_fence_init();
   }
   if (warp == 0) {
@@ -374,6 +376,7 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
               warp_mma_ts(tbase + D + 64, tbase + p * 64 + k * 8, kq + (k >> 2) * 512 + (k & 3) * 2,
                           umma_idesc_bf16_f32(D, 64), p == 0 || k > 0);
         }
+        if constexpr (D == 128) warp_commit(x_done);
       }
       __syncwarp();
     }
@@ -490,7 +493,16 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
               warp_mma(tbase + D, mv + 128 * k, kp + p * 512 + k * 2, id1, p == 0 || k > 0);
           }
       }
-      if (update) {  // behind the products that read X^T, whose columns U takes
+      if (update) {
+        // U takes the columns of X^T. Only products of one accumulator are sure to run in the order of their issue, so
+        // those that read X^T are waited for; they were issued a group earlier and have long finished.
+        if constexpr (!STATES && D == 128) {
+          if (!wait_phase(x_done, c & 1)) {
+            ok = false;
+            if (lane == 0) atomicExch(&g_decay_error, 1u);
+          }
+          tc_fence_after();
+        }
         constexpr uint32_t idu = umma_idesc_bf16_f32(D, D, true, true);
         const uint64_t mk = desc_mn(base + S::kKeys);
 #pragma unroll
@@ -579,7 +591,9 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
             stsm4t(smem_u32(o_tile) + tile_at(t, g), w[2 * n], w[2 * n + 1], w[2 * n + 2], w[2 * n + 3]);
           }
         }
+        tc_fence_before();
         __syncthreads();
+        tc_fence_after();  // the next chunk's X^T goes over columns of U that other warps have read
 #pragma unroll
         for (int u = 0; u < kPasses; ++u) {
           const int r = r0 + kRows * u;

@@ -354,3 +354,20 @@ def test_inference_mode(cuda0):
     with torch.inference_mode():
         got = run()
     assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_chains_repeat_to_the_bit(cuda0, D):
+    """Many chunks in a row with every place on the SMs taken: the order of the products inside a chunk may not depend
+    on how long they take beside another block's."""
+    from nexar_b200 import ops
+    q, k, v, do, s0, ds, lam = _inputs(cuda0, 4, 1024, 80, D, 21)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, s0)]
+
+    def call():
+        o, f = ops.decay_attention(*leaves[:3], lam, state=leaves[3], return_state=True)
+        return [o.detach(), f.detach(), *torch.autograd.grad((o, f), leaves, (do, ds))]
+    first = call()
+    for _ in range(6):
+        for a, b in zip(first, call()):
+            assert torch.equal(a, b)
