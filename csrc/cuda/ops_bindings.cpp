@@ -60,7 +60,8 @@ int64_t op_ln_bwd_scratch_floats(int64_t R, int64_t C, bool dsum) {
 void op_ln_bwd(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& mean, const at::Tensor& rstd,
                const at::Tensor& w, const c10::optional<at::Tensor>& dres, const at::Tensor& dx,
                const at::Tensor& dw, const at::Tensor& db, const at::Tensor& scratch,
-               const at::Tensor& counter, const c10::optional<at::Tensor>& dsum) {
+               const c10::optional<at::Tensor>& /* counter: not used any more */,
+               const c10::optional<at::Tensor>& dsum) {
   need_bf16(dy, "dy");
   need_bf16(x, "x");
   need_bf16(dx, "dx");
@@ -214,7 +215,7 @@ void register_ops(py::module& m) {
   m.def("ln_fwd", &op_ln_fwd, py::arg("x"), py::arg("res"), py::arg("sum_out"), py::arg("w"), py::arg("b"),
         py::arg("y"), py::arg("mean"), py::arg("rstd"), py::arg("eps"), py::arg("rbias") = py::none());
   m.def("ln_bwd", &op_ln_bwd, py::arg("dy"), py::arg("x"), py::arg("mean"), py::arg("rstd"), py::arg("w"),
-        py::arg("dres"), py::arg("dx"), py::arg("dw"), py::arg("db"), py::arg("scratch"), py::arg("counter"),
+        py::arg("dres"), py::arg("dx"), py::arg("dw"), py::arg("db"), py::arg("scratch"), py::arg("counter") = py::none(),
         py::arg("dsum") = py::none());
   m.def("ln_bwd_scratch_floats", &op_ln_bwd_scratch_floats, py::arg("R"), py::arg("C"), py::arg("dsum") = false);
   m.def("colsum", &op_colsum, py::arg("x"), py::arg("out"), py::arg("scratch"), py::arg("accumulate") = false);

@@ -19,27 +19,10 @@ import torch
 
 from .. import _native
 
-_SCRATCH = {}
-
-
-def _scratch(device, nfloats: int) -> torch.Tensor:
-    """Per-device reusable fp32 scratch plus a zeroed uint32 ticket counter."""
-    key = (device, "f")
-    buf = _SCRATCH.get(key)
-    if buf is None or buf.numel() < nfloats:
-        buf = torch.empty(max(nfloats, 1 << 16), dtype=torch.float32, device=device)
-        _SCRATCH[key] = buf
-    return buf
-
-
-def _gemm_ws(device, nfloats: int) -> torch.Tensor:
-    """Per-device fp32 split-K workspace (grown on demand, never shrunk)."""
-    key = (device, "gemm_ws")
-    buf = _SCRATCH.get(key)
-    if buf is None or buf.numel() < nfloats:
-        buf = torch.empty(max(nfloats, 1 << 20), dtype=torch.float32, device=device)
-        _SCRATCH[key] = buf
-    return buf
+def _workspace(device, nfloats: int) -> torch.Tensor:
+    """fp32 memory of one call, from the current stream's (or the capturing graph's) pool: calls on other streams and
+    captured graphs that are replayed later have their own."""
+    return torch.empty(nfloats, dtype=torch.float32, device=device)
 
 
 def _sink(p):
@@ -79,7 +62,7 @@ def matmul_nt(a, b, out=None, bias=None, act: int = 0, pre=None, a_t: bool = Fal
     if out is None:
         out = torch.empty(M, N, dtype=a.dtype, device=a.device)
     sp = C.gemm_choose_splits(M, N, K) if splits == 0 else splits
-    ws = _gemm_ws(a.device, C.gemm_split_workspace_bytes(M, N, sp) // 4) if sp > 1 else None
+    ws = _workspace(a.device, C.gemm_split_workspace_bytes(M, N, sp) // 4) if sp > 1 else None
     C.gemm_ex(a, b, out, a_t, b_t, bias, None, pre, act, 1.0, accumulate, sp, ws)
     return out
 
@@ -88,7 +71,7 @@ def colsum(x, out, accumulate: bool = False):
     """out[c] (+)= sum over rows of x[:, c] (bf16 in/out, fp32 accumulation)."""
     C = _native.cuda()
     x2 = x.reshape(-1, x.shape[-1])
-    scratch = _scratch(x.device, C.colsum_scratch_floats(x2.shape[0], x2.shape[1]))
+    scratch = _workspace(x.device, C.colsum_scratch_floats(x2.shape[0], x2.shape[1]))
     C.colsum(x2, out, scratch, accumulate)
     return out
 
@@ -161,15 +144,6 @@ def linear(x, w, b=None, act: str = None, ready: bool = True):
     return _Linear.apply(x, w, b, 1 if act == "gelu" else 0, ready)
 
 
-def _counter(device, slot: int = 0) -> torch.Tensor:
-    key = (device, "c")
-    c = _SCRATCH.get(key)
-    if c is None:
-        c = torch.zeros(64, dtype=torch.int32, device=device)
-        _SCRATCH[key] = c
-    return c[slot:slot + 1]
-
-
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, eps):
@@ -198,8 +172,8 @@ class _LayerNorm(torch.autograd.Function):
         if db is None:
             db = ret_b = torch.empty_like(w)
         C_ = _native.cuda()
-        scratch = _scratch(x2.device, C_.ln_bwd_scratch_floats(x2.shape[0], C))
-        C_.ln_bwd(dy2, x2, mean, rstd, w, None, dx, dw, db, scratch, _counter(x2.device))
+        scratch = _workspace(x2.device, C_.ln_bwd_scratch_floats(x2.shape[0], C))
+        C_.ln_bwd(dy2, x2, mean, rstd, w, None, dx, dw, db, scratch)
         if ret_w is None:
             _ready(w)
         if ret_b is None:
@@ -253,11 +227,11 @@ class _ResidualLayerNorm(torch.autograd.Function):
         if ctx.rb is not None:
             drb = outs[2][0] if outs[2][0] is not None else outs[2][1]
         C_ = _native.cuda()
-        scratch = _scratch(s.device, C_.ln_bwd_scratch_floats(s.shape[0], C, drb is not None))
+        scratch = _workspace(s.device, C_.ln_bwd_scratch_floats(s.shape[0], C, drb is not None))
         dres = None if ds is None else ds.contiguous().view(-1, C)
         if dy is None:
             dy = torch.zeros_like(s)
-        C_.ln_bwd(dy.contiguous().view(-1, C), s, mean, rstd, w, dres, dx, dw, db, scratch, _counter(s.device), drb)
+        C_.ln_bwd(dy.contiguous().view(-1, C), s, mean, rstd, w, dres, dx, dw, db, scratch, dsum=drb)
         for p, (sink, _) in zip((w, ctx.b, ctx.rb), outs):
             if p is not None and sink is not None:
                 _ready(p)

@@ -149,3 +149,59 @@ def test_checkpoint_carries_the_generator(cuda0, tmp_path):
 def test_configuration_refusals(bad):
     with pytest.raises(ValueError):
         GPT2(_config(**bad), "cpu")
+
+
+def test_workspaces_belong_to_their_call():
+    from nexar_b200.ops import functional
+    a, b = functional._workspace("cpu", 16), functional._workspace("cpu", 16)
+    assert a.numel() == 16 and a.data_ptr() != b.data_ptr()
+
+
+@gpu
+def test_a_captured_step_keeps_its_workspaces(cuda0):
+    """Calls that need larger workspaces, and memory that is handed out afterwards, neither change a captured step nor
+    are written by it."""
+    cfg = _config(mixer="decay", positions="rotary")
+    g = torch.Generator().manual_seed(4)
+    idx = torch.randint(0, cfg.vocab_size, (2, 96), generator=g)
+    tgt = torch.randint(0, cfg.vocab_size, (2, 96), generator=g)
+    tr = DataParallelTrainer(cfg, 2, 96, seed=5, lr=0.0, weight_decay=0.0)
+    tr.set_batch(idx, tgt)
+    tr.capture(warmup=1)
+    flat = tr.model.flat
+
+    def grads():
+        tr.run_step()
+        torch.cuda.synchronize()
+        return {n: flat.view(flat.grad, n).clone() for n in tr.model.p if n != "wte"}  # wte: atomic sums
+    first = grads()
+    wide = torch.randn(20000, 2048, device=cuda0).to(torch.bfloat16).requires_grad_(True)
+    w, b = (torch.ones(2048, device=cuda0, dtype=torch.bfloat16).requires_grad_(True) for _ in range(2))
+    torch.autograd.grad(ops.layer_norm(wide, w, b), (wide, w, b), torch.ones_like(wide))
+    held = [torch.full((n,), 3.25, device=cuda0) for n in (1 << 16, 1 << 18, 1 << 20) for _ in range(24)]
+    again = grads()
+    for n in first:
+        assert torch.equal(first[n], again[n]), n
+    assert all(bool((t == 3.25).all()) for t in held)
+
+
+@gpu
+def test_layer_norm_backward_on_streams_side_by_side(cuda0):
+    g = torch.Generator(device=cuda0).manual_seed(8)
+    streams = [torch.cuda.Stream(cuda0) for _ in range(4)]
+    cases = []
+    for _ in streams:
+        x, dy = (torch.randn(6000, 768, device=cuda0, generator=g).to(torch.bfloat16) for _ in range(2))
+        w, b = (torch.randn(768, device=cuda0, generator=g).to(torch.bfloat16).requires_grad_(True) for _ in range(2))
+        x.requires_grad_(True)
+        cases.append((x, w, b, dy))
+    want = [torch.autograd.grad(ops.layer_norm(x, w, b), (x, w, b), dy) for x, w, b, dy in cases]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for s, (x, w, b, dy) in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(torch.autograd.grad(ops.layer_norm(x, w, b), (x, w, b), dy))
+        torch.cuda.synchronize()
+        for a, c in zip(got, want):
+            assert all(torch.equal(i, j) for i, j in zip(a, c))
