@@ -426,9 +426,12 @@ OptTensor op_decay_bwd(const at::Tensor& q_in, const at::Tensor& k_in, const at:
   return ds0;
 }
 
+void no_tangents(std::initializer_list<const at::Tensor*> ts, const char* what);
+
 // One token: q, k, v [B, H, D]; updates state [B, H, D, D] in place and returns o [B, H, D].
 at::Tensor op_decay_step(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
                          const at::Tensor& log_decay, const at::Tensor& state, double scale) {
+  no_tangents({&q_in, &k_in, &v_in, &log_decay, &state}, "decay attention");
   need_cuda(q_in, "q");
   TORCH_CHECK(q_in.scalar_type() == at::kBFloat16 && q_in.dim() == 3,
               "nexar_b200: decay_attention_step: q must be bf16 [B, H, D]");
@@ -471,6 +474,12 @@ bool any_grad(std::initializer_list<const at::Tensor*> ts) {
   return false;
 }
 const at::Tensor* ptr(const OptTensor& t) { return t ? &*t : nullptr; }
+// A tangent (forward-mode derivative) would be lost in the kernels, which torch reads as a derivative of zero.
+void no_tangents(std::initializer_list<const at::Tensor*> ts, const char* what) {
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(0).defined(), "nexar_b200: ", what,
+                                " has no forward-mode derivative");
+}
 at::Tensor or_none(const OptTensor& t) { return t ? *t : at::Tensor(); }
 OptTensor opt(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
@@ -528,6 +537,7 @@ std::vector<at::Tensor> rotate(const at::Tensor& x0, const OptTensor& x1, const 
                                const OptTensor& positions, int64_t start, int64_t heads, bool interleaved,
                                bool inverse) {
   TORCH_CHECK_VALUE(!table.requires_grad(), "nexar_b200: the rotary table takes no gradient");
+  no_tangents({&x0, ptr(x1), &table}, "rotary");
   if (any_grad({&x0, ptr(x1)})) return RotaryFn::apply(x0, x1, table, positions, start, heads, interleaved, inverse);
   return op_rotary(x0, x1, table, positions, start, heads, interleaved, inverse);
 }
@@ -549,6 +559,7 @@ struct DropoutFn : public torch::autograd::Function<DropoutFn> {
   }
 };
 at::Tensor drop(const at::Tensor& x, const at::Tensor& state, int64_t site, double p) {
+  no_tangents({&x}, "dropout");
   if (any_grad({&x})) return DropoutFn::apply(x, state, site, p);
   return std::get<0>(op_dropout(x, state, site, p, false));
 }
@@ -583,6 +594,7 @@ struct DropoutLayerNormFn : public torch::autograd::Function<DropoutLayerNormFn>
 };
 variable_list dropout_layer_norm(const at::Tensor& x, const at::Tensor& r, const OptTensor& rb, const at::Tensor& w,
                                  const at::Tensor& b, double eps, const at::Tensor& state, int64_t site, double p) {
+  no_tangents({&x, &r, ptr(rb), &w, &b}, "residual_layer_norm with dropout");
   return DropoutLayerNormFn::apply(x, r, rb, w, b, eps, state, site, p);
 }
 
@@ -635,6 +647,7 @@ variable_list decay(const at::Tensor& q, const OptTensor& k, const OptTensor& v,
   TORCH_CHECK_VALUE(k || q.size(2) == 3, "nexar_b200: decay_attention_qkv takes qkv [B, T, 3, H, D]");
   TORCH_CHECK_VALUE(!log_decay.requires_grad(),
                     "nexar_b200: decay attention: the decays are fixed; log_decay takes no gradient (detach it)");
+  no_tangents({&q, ptr(k), ptr(v), &log_decay, ptr(state)}, "decay attention");
   if (any_grad({&q, ptr(k), ptr(v), ptr(state)}))
     return DecayFn::apply(q, k, v, log_decay, state, lengths, scale, want_state);
   const auto a = DecayFn::parts(q, or_none(k), or_none(v));

@@ -172,3 +172,31 @@ def test_decay_refusals_on_the_host():
         ops.decay_attention_step(one.clone().requires_grad_(True), one, one, lam.detach(), torch.zeros(1, 2, 64, 64))
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.decay_attention_step(one, one, one, lam.detach(), torch.zeros(1, 2, 64, 64))
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives: an error, not a result without a tangent (on the host the check comes before that of
+    the device)."""
+    from torch.autograd import forward_ad
+    state = ops.DropoutState(1, device="cpu")
+    x, t = torch.zeros(4, 2, 8), torch.zeros(4, 8)
+    w = torch.ones(8, dtype=torch.bfloat16)
+    rows = torch.zeros(4, 8, dtype=torch.bfloat16)
+    q, lam, s0 = torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16), torch.zeros(2), torch.zeros(1, 2, 64, 64)
+    qkv, one = torch.zeros(1, 4, 3, 2, 64, dtype=torch.bfloat16), q[:, 0].clone()
+    with forward_ad.dual_level():
+        def dual(v):
+            return forward_ad.make_dual(v, torch.ones_like(v))
+        calls = [
+            lambda: ops.rotary(dual(x), t), lambda: ops.rotary(x, dual(t)), lambda: ops.rotary_qk(x, dual(x), t),
+            lambda: ops.dropout(dual(x), 0.1, state), lambda: ops.dropout(dual(x), 0.0, state),
+            lambda: ops.residual_layer_norm(dual(rows), rows, w, w, p=0.1, dropout=state),
+            lambda: ops.residual_layer_norm(rows, rows, w, dual(w), p=0.1, dropout=state),
+            lambda: ops.decay_attention(dual(q), q, q, lam), lambda: ops.decay_attention(q, q, dual(q), lam),
+            lambda: ops.decay_attention(q, q, q, dual(lam)), lambda: ops.decay_attention(q, q, q, lam, state=dual(s0)),
+            lambda: ops.decay_attention_qkv(dual(qkv), lam), lambda: ops.decay_attention_step(one, dual(one), one, lam, s0),
+            lambda: ops.decay_attention_step(one, one, one, lam, dual(s0))]
+        for i, call in enumerate(calls):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
