@@ -181,11 +181,21 @@ void need_rows(const at::Tensor& t, const at::Tensor& x, int64_t n, const char* 
               "nexar_b200: ", name, " must be a contiguous, 16-byte aligned bf16 tensor of ", num(n), " elements");
 }
 
+// Kernels read rows in 16-byte groups: a tensor at another address, or with other strides, is copied.
+at::Tensor aligned_rows(const at::Tensor& t) {
+  return t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t
+                                                                                  : t.clone(at::MemoryFormat::Contiguous);
+}
+OptTensor aligned_rows(const OptTensor& t) { return t ? OptTensor(aligned_rows(*t)) : OptTensor(); }
+
 // s = x + drop(r + rb), y = LayerNorm(s): returns s, y, mean, rstd, (seed, step).
-std::vector<at::Tensor> op_dropout_ln_fwd(const at::Tensor& x, const at::Tensor& r, const OptTensor& rb,
-                                          const at::Tensor& w, const at::Tensor& b, double eps,
+std::vector<at::Tensor> op_dropout_ln_fwd(const at::Tensor& x_in, const at::Tensor& r_in, const OptTensor& rb_in,
+                                          const at::Tensor& w_in, const at::Tensor& b_in, double eps,
                                           const at::Tensor& state, int64_t site, double p) {
-  need_cuda(x, "x");
+  need_cuda(x_in, "x");
+  c10::cuda::CUDAGuard g(x_in.get_device());
+  const at::Tensor x = aligned_rows(x_in), r = aligned_rows(r_in), w = aligned_rows(w_in), b = aligned_rows(b_in);
+  const OptTensor rb = aligned_rows(rb_in);
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) % 8 == 0 && x.size(-1) >= 8 && x.size(-1) <= 2048,
               "nexar_b200: residual_layer_norm with dropout needs rows of a multiple of 8, at most 2048");
   const int64_t C = x.size(-1), R = x.numel() / C;
@@ -198,7 +208,6 @@ std::vector<at::Tensor> op_dropout_ln_fwd(const at::Tensor& x, const at::Tensor&
   const Drop d = drop_of(p, site);
   TORCH_CHECK(d.threshold > 0, "nexar_b200: residual_layer_norm: a probability of ", std::to_string(p), " drops nothing");
   const int64_t* st = drop_state(state, x);
-  c10::cuda::CUDAGuard g(x.get_device());
   at::Tensor s = at::empty_like(x), y = at::empty_like(x);
   at::Tensor mean = at::empty({R}, x.options().dtype(at::kFloat)), rstd = at::empty_like(mean);
   at::Tensor snap = at::empty({2}, state.options());
@@ -212,17 +221,15 @@ std::vector<at::Tensor> op_dropout_ln_fwd(const at::Tensor& x, const at::Tensor&
   return {s, y, mean, rstd, snap};
 }
 
-// Kernels read gradients in 16-byte groups: one that autograd was handed at another address is copied.
-at::Tensor grad_rows(const at::Tensor& t) {
-  return t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t
-                                                                                  : t.clone(at::MemoryFormat::Contiguous);
-}
 // Returns dx, dr; writes dw, db (and drb).
-std::vector<at::Tensor> op_dropout_ln_bwd(const at::Tensor& dy, const at::Tensor& s, const at::Tensor& mean,
-                                          const at::Tensor& rstd, const at::Tensor& w, const OptTensor& dres,
+std::vector<at::Tensor> op_dropout_ln_bwd(const at::Tensor& dy_in, const at::Tensor& s, const at::Tensor& mean,
+                                          const at::Tensor& rstd, const at::Tensor& w_in, const OptTensor& dres_in,
                                           const at::Tensor& dw, const at::Tensor& db, const OptTensor& drb,
                                           const at::Tensor& snap, int64_t site, double p) {
   need_cuda(s, "s");
+  c10::cuda::CUDAGuard g(s.get_device());
+  const at::Tensor dy = aligned_rows(dy_in), w = aligned_rows(w_in);
+  const OptTensor dres = aligned_rows(dres_in);
   const int64_t C = s.size(-1), R = s.numel() / C;
   need_rows(s, s, R * C, "s");
   need_rows(dy, s, R * C, "dy");
@@ -233,7 +240,6 @@ std::vector<at::Tensor> op_dropout_ln_bwd(const at::Tensor& dy, const at::Tensor
   if (drb) need_rows(*drb, s, C, "drbias");
   const Drop d = drop_of(p, site);
   const int64_t* st = drop_state(snap, s);
-  c10::cuda::CUDAGuard g(s.get_device());
   at::Tensor dx = at::empty_like(s), dr = at::empty_like(s);
   if (R == 0) {
     dw.zero_();
@@ -570,7 +576,7 @@ struct DropoutLayerNormFn : public torch::autograd::Function<DropoutLayerNormFn>
                                const at::Tensor& w, const at::Tensor& b, double eps, const at::Tensor& state,
                                int64_t site, double p) {
     ctx->set_materialize_grads(false);
-    auto out = op_dropout_ln_fwd(x.contiguous(), r.contiguous(), rb, w, b, eps, state, site, p);
+    auto out = op_dropout_ln_fwd(x, r, rb, w, b, eps, state, site, p);
     ctx->save_for_backward({out[0], w, out[2], out[3], out[4], or_none(rb)});
     ctx->saved_data["site"] = site;
     ctx->saved_data["p"] = p;
@@ -580,9 +586,9 @@ struct DropoutLayerNormFn : public torch::autograd::Function<DropoutLayerNormFn>
   static variable_list backward(AutogradContext* ctx, variable_list d) {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &s = saved[0], &w = saved[1], &rb = saved[5];
-    const at::Tensor dy = d[1].defined() ? grad_rows(d[1]) : at::zeros_like(s);
-    OptTensor ds, drb;
-    if (d[0].defined()) ds = grad_rows(d[0]);
+    const at::Tensor dy = d[1].defined() ? d[1] : at::zeros_like(s);
+    const OptTensor ds = opt(d[0]);
+    OptTensor drb;
     if (rb.defined()) drb = at::empty_like(rb);
     at::Tensor dw = at::empty_like(w), db = at::empty_like(w);
     auto g = op_dropout_ln_bwd(dy, s, saved[2], saved[3], w, ds, dw, db, drb, saved[4],
@@ -630,7 +636,7 @@ struct DecayFn : public torch::autograd::Function<DecayFn> {
     }
     const at::Tensor dO = d[0].defined() ? d[0] : at::zeros(a[0].sizes(), q.options());
     OptTensor ds;
-    if (d.size() > 1 && d[1].defined()) ds = grad_rows(d[1]);
+    if (d.size() > 1 && d[1].defined()) ds = aligned_rows(d[1]);
     const OptTensor ds0 = op_decay_bwd(a[0], a[1], a[2], dO, saved[3], opt(saved[4]), ds, opt(saved[5]),
                                        ctx->saved_data["scale"].toDouble(), g[0], g[1], g[2],
                                        saved[4].defined() && ctx->needs_input_grad(k.defined() ? 4 : 2), saved[6],

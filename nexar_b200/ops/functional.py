@@ -250,8 +250,7 @@ class _ResidualDropoutLayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, r, w, b, rb, eps, state, site, p):
         ctx.set_materialize_grads(False)
-        x2, r2 = x.contiguous(), r.contiguous()
-        s, y, mean, rstd, used = _native.cuda().dropout_ln_fwd(x2, r2, rb, w, b, eps, state, site, p)
+        s, y, mean, rstd, used = _native.cuda().dropout_ln_fwd(x, r, rb, w, b, eps, state, site, p)
         ctx.save_for_backward(s, w, mean, rstd, used)
         ctx.b, ctx.rb = b, rb
         ctx.how = (site, p)
@@ -267,8 +266,7 @@ class _ResidualDropoutLayerNorm(torch.autograd.Function):
             g = _sink(p) if p is not None else None
             outs.append((g, None) if g is not None or p is None else (None, torch.empty_like(p)))
         dw, db, drb = (g if g is not None else t for g, t in outs)
-        dy = torch.zeros_like(s) if dy is None else dy.contiguous()
-        ds = None if ds is None else ds.contiguous()
+        dy = torch.zeros_like(s) if dy is None else dy
         dx, dr = _native.cuda().dropout_ln_bwd(dy, s, mean, rstd, w, ds, dw, db, drb, used, *ctx.how)
         for p, (sink, _) in zip((w, ctx.b, ctx.rb), outs):
             if sink is not None:

@@ -212,6 +212,33 @@ def test_residual_gradients_at_any_address(cuda0):
     assert all(torch.equal(a, c) for a, c in zip(run(ds, dy), run(moved(ds), moved(dy))))
 
 
+@pytest.mark.parametrize("sinks", [False, True])
+def test_residual_tensors_at_any_address(cuda0, sinks):
+    from nexar_b200 import ops
+
+    def moved(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=cuda0)
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view_as(t)
+
+    def strided(t):
+        return torch.stack([t, t + 1], -1)[..., 0]
+
+    def run(how):
+        x, r, ds, dy, w, b, rb = (how(t).detach() for t in _inputs(cuda0, 20, 64, True, 8))
+        leaves = [t.requires_grad_(True) for t in (x, r, w, b, rb)]
+        if sinks:
+            for t in (w, b, rb):
+                t.main_grad = torch.empty(64, dtype=t.dtype, device=cuda0)
+        out = ops.residual_layer_norm(x, r, w, b, 1e-5, rbias=rb, p=0.1, dropout=ops.DropoutState(4, cuda0))
+        got = torch.autograd.grad(out, leaves, (ds, dy), allow_unused=True)
+        return [*out, *got[:2], *([t.main_grad for t in (w, b, rb)] if sinks else got[2:])]
+    want = run(lambda t: t)
+    for how in (moved, strided):
+        for a, c in zip(want, run(how)):
+            assert torch.equal(a, c)
+
+
 def test_residual_without_dropout_is_unchanged(cuda0):
     from nexar_b200 import ops
     x, r, ds, dy, w, b, rb = _inputs(cuda0, 64, 768, True)
