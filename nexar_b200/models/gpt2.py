@@ -181,8 +181,11 @@ class GPT2(torch.nn.Module):
         return ops.cross_entropy(logits, targets, cfg.vocab_size, unit_grad=unit_grad)
 
     def flops_per_token(self, T: int) -> float:
-        """Training FLOPs per token: 6*N (dense) + 6*L*T*C (causal attention, halved)."""
+        """Training FLOPs per token: 6*N (dense) + those of the mixer, forward and twice that back: 6*L*T*C for
+        softmax attention (causal, halved) or 12*L*C*head for attention with a decay, whose state update and read
+        (2 * 2 * head^2 per head) do not grow with T."""
         cfg = self.cfg
         C, L = cfg.n_embd, cfg.n_layer
         n_dense = L * 12 * C * C + cfg.padded_vocab * C
-        return 6.0 * n_dense + 6.0 * L * T * C
+        mixer = 12.0 * L * C * (C // cfg.n_head) if cfg.mixer == "decay" else 6.0 * L * T * C
+        return 6.0 * n_dense + mixer

@@ -205,3 +205,20 @@ def test_layer_norm_backward_on_streams_side_by_side(cuda0):
         torch.cuda.synchronize()
         for a, c in zip(got, want):
             assert all(torch.equal(i, j) for i, j in zip(a, c))
+
+
+def test_flops_per_token():
+    """6 per weight; softmax attention grows with the length, the decay mixer with the head's size alone."""
+    small = GPT2Config.small()
+    dense = 6.0 * (12 * 12 * 768 * 768 + 50304 * 768)
+
+    def flops(cfg, T):
+        class Model:
+            pass
+        m = Model()
+        m.cfg = cfg
+        return GPT2.flops_per_token(m, T)
+    assert flops(small, 1024) == dense + 6.0 * 12 * 1024 * 768
+    decay = GPT2Config(mixer="decay")
+    # per head and token: S += k v^T and S^T q, 2 * 64^2 each; backward twice that
+    assert flops(decay, 1024) == flops(decay, 64) == dense + 12 * 12 * 3 * (2 + 2) * 64 * 64
