@@ -269,6 +269,8 @@ class DataParallelTrainer:
 
     # ---------------------------------------------------------------- checkpoint / resume
     CHECKPOINT_FORMAT = "nexar_b200.dp_trainer/1"
+    # configuration fields younger than the format, with the model that a checkpoint without them was written for
+    CONFIG_ADDED = {"dropout": 0.0, "positions": "learned", "mixer": "attention"}
 
     def state_dict(self) -> dict:
         """Everything a resumed run needs, as CPU tensors and plain values:
@@ -300,9 +302,7 @@ class DataParallelTrainer:
         re-derived from the fp32 master weights."""
         if sd.get("format") != self.CHECKPOINT_FORMAT:
             raise ValueError(f"not a {self.CHECKPOINT_FORMAT} checkpoint: {sd.get('format')!r}")
-        # fields that a checkpoint written before they existed does not have stand at their defaults
-        saved = {**{f.name: f.default for f in dataclasses.fields(self.cfg)}, **sd["config"]}
-        if saved != dataclasses.asdict(self.cfg):
+        if {**self.CONFIG_ADDED, **sd["config"]} != dataclasses.asdict(self.cfg):
             raise ValueError(f"checkpoint is for model {sd['config']}, this trainer runs {dataclasses.asdict(self.cfg)}")
         flat = self.model.flat
         layout = [[e.name, list(e.shape), e.offset, e.numel] for e in flat.entries]

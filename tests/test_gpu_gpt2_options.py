@@ -1,5 +1,7 @@
 """GPT-2 with rotary positions, dropout and the decay mixer together: against a plain fp32 model with the same masks,
 in a captured step, and across a checkpoint."""
+import dataclasses
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -222,3 +224,34 @@ def test_flops_per_token():
     decay = GPT2Config(mixer="decay")
     # per head and token: S += k v^T and S^T q, 2 * 64^2 each; backward twice that
     assert flops(decay, 1024) == flops(decay, 64) == dense + 12 * 12 * 3 * (2 + 2) * 64 * 64
+
+
+@pytest.mark.parametrize("missing", ["n_head", "ln_eps", "vocab_size", "block_size"])
+def test_checkpoint_without_a_model_field_is_refused(missing):
+    """Only the options that are younger than the format may be absent."""
+    class Trainer:
+        CHECKPOINT_FORMAT = DataParallelTrainer.CHECKPOINT_FORMAT
+        CONFIG_ADDED = getattr(DataParallelTrainer, "CONFIG_ADDED", None)
+    tr = Trainer()
+    # the saved model stands at the defaults, so nothing but the missing field tells the two apart
+    tr.cfg = GPT2Config()
+    sd = {"format": tr.CHECKPOINT_FORMAT, "config": dataclasses.asdict(tr.cfg)}
+    del sd["config"][missing]
+    with pytest.raises(ValueError, match="checkpoint is for model"):
+        DataParallelTrainer.load_state_dict(tr, sd)
+
+
+def test_ranks_draw_masks_of_their_own():
+    """The trainer's seeds: one per rank, the same for the rank whenever it is seeded again."""
+    from types import SimpleNamespace
+    states = []
+    for rank in (None, 0, 1, 2, 7):
+        tr = SimpleNamespace(model=SimpleNamespace(dropout_state=ops.DropoutState(0, "cpu")),
+                             comm=None if rank is None else SimpleNamespace(rank=rank))
+        DataParallelTrainer._seed_dropout(tr, 5, 3)
+        states.append(tuple(tr.model.dropout_state.tensor.tolist()))
+    assert states[0] == states[1] == (5, 3)
+    assert len(set(states[1:])) == 4 and all(s[1] == 3 for s in states)
+    # the masks behind two ranks' seeds differ in about 2 p (1 - p) of their elements
+    a, b = (oracle.dropout_keep(4096, s[0], s[1], 1, 0.5)[0] for s in (states[1], states[2]))
+    assert 0.4 < (a != b).double().mean() < 0.6
