@@ -212,6 +212,28 @@ def test_residual_gradients_at_any_address(cuda0):
     assert all(torch.equal(a, c) for a, c in zip(run(ds, dy), run(moved(ds), moved(dy))))
 
 
+@pytest.mark.parametrize("C", [64, 256, 1024, 2048])
+def test_residual_constant_rows(cuda0, C):
+    """Rows of one value each, far from zero: nothing is left of them after the mean, so dw is exactly 0 and dx is
+    that of a norm at its mean. (The sums of C equal bf16 values and the division by a power of two are exact.)"""
+    from nexar_b200 import ops
+    R = 40
+    g = torch.Generator(device=cuda0).manual_seed(C)
+    x = (torch.randn(R, 1, device=cuda0, generator=g) * 1000).to(torch.bfloat16).expand(R, C).contiguous()
+    _, _, ds, dy, w, b, _ = _inputs(cuda0, R, C, False, 3)
+    leaves = [x.requires_grad_(True), torch.zeros_like(x).requires_grad_(True), w.requires_grad_(True), b]
+    s, y = ops.residual_layer_norm(*leaves, 1e-5, p=0.2, dropout=ops.DropoutState(3, cuda0))
+    dx, dw = torch.autograd.grad((s, y), (leaves[0], w), (ds, dy))
+    assert torch.equal(s, x) and torch.equal(y, b.expand(R, C))
+    assert torch.count_nonzero(dw) == 0
+    # dx = ds + rstd (gw - mean gw): C products and sums in fp32, rstd by an approximate root, rounded once
+    gw = dy.double() * w.detach().double()
+    rstd, f32, half = 1e-5 ** -0.5, 2.0 ** -24, oracle.half_step(torch.bfloat16)
+    want = ds.double() + rstd * (gw - gw.mean(-1, keepdim=True))
+    extra = ((C / 32 + 16) * f32 + 4 * 2.0 ** -22) * (ds.double().abs() + rstd * (gw.abs() + gw.abs().mean(-1, keepdim=True)))
+    oracle.assert_within(dx, want, half * (want.abs() + extra) + extra, "dx")
+
+
 @pytest.mark.parametrize("sinks", [False, True])
 def test_residual_tensors_at_any_address(cuda0, sinks):
     from nexar_b200 import ops
