@@ -371,3 +371,71 @@ def test_long_chains_repeat_to_the_bit(cuda0, D):
     for _ in range(6):
         for a, b in zip(first, call()):
             assert torch.equal(a, b)
+
+
+def _parts(x, n):
+    """x as n bf16 parts, each the rounding of what the ones before leave."""
+    out = torch.zeros_like(x)
+    for _ in range(n):
+        out = out + (x - out).to(torch.bfloat16).double()
+    return out
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [2, 33, 64, 130])
+def test_a_state_holds_fp32_values(cuda0, T, D):
+    """One token per sequence has a key (a query, for the gradient of the first state), and its value (output
+    gradient) is a power of two: a state is then one product, lam^x k 2^e, that only the roundings of its way can
+    touch. Relative, in units of 2^-24: the power of the decay 1, its product with the key 1, what three bf16 parts
+    leave 1/8, what the accumulator cuts off 2, and for each chunk behind the token 3 (the factor and two sums). Two
+    parts leave up to 64, which the bound has to catch."""
+    from nexar_b200 import ops
+    B, H = 24, 4
+    g = torch.Generator(device=cuda0).manual_seed(T + D)
+    lam = torch.tensor([-0.0021, -0.0307, -0.011, -0.0043], device=cuda0)
+    at = torch.randint(0, T, (B,), device=cuda0, generator=g)
+    at[0], at[1] = 0, T - 1
+    only = torch.zeros(B, T, 1, 1, device=cuda0)
+    only[torch.arange(B, device=cuda0), at] = 1.0
+    x = (only * torch.randn(B, T, H, D, device=cuda0, generator=g)).to(torch.bfloat16)
+    two = torch.exp2(torch.randint(-3, 4, (B, T, H, D), device=cuda0, generator=g).float())
+    two = (two * (1 - 2 * torch.randint(0, 2, two.shape, device=cuda0, generator=g))).to(torch.bfloat16)
+    zero = torch.zeros_like(x)
+    _, state = ops.decay_attention(zero, x, two, lam, return_state=True)
+    s0 = torch.zeros(B, H, D, D, device=cuda0, requires_grad=True)
+    o = ops.decay_attention(x, zero, zero, lam, state=s0, scale=0.25)
+    (dstate,) = torch.autograd.grad(o, s0, two)
+    row, val = (t.double()[torch.arange(B, device=cuda0), at] for t in (x, two))  # [B, H, D]
+    chunks = -(-T // 64)
+    bound = (4.125 + 3 * (chunks - 1)) * 2.0 ** -24
+    for got, steps, scale, what in ((state, T - 1 - at, 1.0, "state"), (dstate, at + 1, 0.25, "dstate")):
+        weight = scale * torch.exp(lam.double()[None] * steps.double()[:, None])[..., None]
+        want = (row * weight)[..., :, None] * val[..., None, :]
+        oracle.assert_within(got, want, bound * want.abs() + 1e-30, what)
+        rough = _parts(row * weight, 2)[..., :, None] * val[..., None, :]
+        assert ((rough - want).abs() > bound * want.abs()).any() or T == 2
+
+
+def test_a_long_sum_has_no_bias(cuda0):
+    """All keys and values positive, so that errors of one sign add up. Relative root mean square error of a head's
+    state, in units of 2^-24: 2 x 13 for the cuts of a chunk's twelve accumulations and of its largest product, 3 for
+    each of the 1 / (1 - lam^64) chunks that are left in the sum. One bf16 part for the decayed keys would leave
+    about 2^-10.3 / sqrt(tokens left), 2^-15 and more."""
+    from nexar_b200 import ops
+    T, H, D = 3000, 4, 64
+    q, k, v, _, _, _, _ = _inputs(cuda0, 2, T, H, D, 31)
+    k, v = k.abs(), v.abs()
+    lam = torch.tensor([-0.002, -0.03, -0.008, -0.1], device=cuda0)
+    _, got = ops.decay_attention(q, k, v, lam, return_state=True)
+    _, want = oracle.decay_attention(*(t.double() for t in (q, k, v)), lam)
+    t = torch.arange(T, device=cuda0, dtype=torch.float64)
+    end = (64 * (t // 64 + 1)).clamp(max=T) - 1  # of the token's chunk
+    g = lam.double()[None, :, None]
+    keys = _parts(k.double() * torch.exp(g * (end - t)[:, None, None]), 1) * torch.exp(g * (T - 1 - end)[:, None, None])
+    rough = torch.einsum("bthi,bthj->bhij", keys, v.double())
+
+    def error(x):
+        return ((x.double() - want).square().sum((0, 2, 3)) / want.square().sum((0, 2, 3))).sqrt()
+    bound = (26 + 3 / (1 - torch.exp(64 * lam.double()))) * 2.0 ** -24
+    assert (error(got) <= bound).all(), error(got)
+    assert (error(rough) > bound).all(), error(rough)
