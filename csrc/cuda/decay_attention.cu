@@ -26,33 +26,36 @@
 //               then O = lam^(i+1) O + P V, U [dk, dv] = K'^T V
 //     D = 128:  S [token, token] = Q K^T, O2 [dv, token] = X^T Q^T;
 //               then O1 [dv, token] = V^T P^T, U [dv, dk] = V^T K'
-// The first group runs while K' is written; two (D = 128) or three (D = 64) blocks
-// per SM fill each other's gaps during the second. With D = 64 the 64 rows of every
-// accumulator are read as matrix fragments (16 lanes per warp), X goes back as an
-// operand through shared memory, in the place that P takes later, S lies over U, and
-// Q X is scaled in place so that P V adds to it: 128 TMEM columns and 64 KB a block.
-// With D = 128 the value dimension fills the 128 lanes, X^T stays with its rows'
-// threads and goes back through TMEM, over the columns of U, which is done by then;
-// o = lam^(i+1) O2 + O1 at the end. Rows come by cp.async, each thread its 16-byte
-// groups (a reversed role simply reads its rows from the end): with D = 128 the
-// state fills the 128 registers that two blocks per SM leave a thread, and a form
-// with tensor-map loads, which spilled some, took 17 to 25 % longer.
+// With D = 64 the first group runs while K' is written; two (D = 128) or three (D =
+// 64) blocks per SM fill each other's gaps during the second. With D = 64 the 64 rows
+// of every accumulator are read as matrix fragments (16 lanes per warp), X goes back
+// as an operand through shared memory, in the place that P takes later, S lies over U,
+// and Q X is scaled in place so that P V adds to it: 128 TMEM columns and 72 KB a
+// block. With D = 128 the value dimension fills the 128 lanes, X^T stays with its
+// rows' threads and goes back through TMEM, over the columns of U, which is done by
+// then, but for its last 8 bits, which find room in shared memory only where K' goes:
+// their product is the first of the group, and K' is written behind it, its first part
+// over the keys; o = lam^(i+1) O2 + O1 at the end. Rows come by cp.async, each thread
+// its 16-byte groups (a reversed role simply reads its rows from the end): with D =
+// 128 the state fills the 128 registers that two blocks per SM leave a thread, and a
+// form with tensor-map loads, which spilled some, took 17 to 25 % longer.
 //
-// Measured, forward / backward: 8 x 1024 tokens of 12 heads of 64: 37 / 55 us (the
-// 138 MB that they have to move take 21 us); 16385 tokens of 16 heads of 128: 141 /
-// 309 us (742 MB, 113 us), of which the states before the segments and the scan are
+// Measured, forward / backward: 8 x 1024 tokens of 12 heads of 64: 40 / 58 us (the
+// 138 MB that they have to move take 21 us); 16385 tokens of 16 heads of 128: 157 /
+// 349 us (742 MB, 113 us), of which the states before the segments and the scan are
 // 57 us each. With a full grid an SM issues in 53 to 58 % of its cycles and the
 // tensor pipe works in 34 to 36 %: bound by the instructions that decay, round and
 // split operands between one chunk's two groups of products and by the latency of
 // that chain, which the two or three blocks of an SM do not cover in full.
 //
-// Roundings. Products are bf16 tensor-core products with fp32 sums. The decayed
-// keys that enter the state are split into three bf16 parts (24 bits, all of an
-// fp32 value), so the state is an fp32 state; scores and states that enter the
-// bf16 output are split into two parts (16 bits), well below the output's
-// rounding. U is formed apart and added to X once per chunk: the tensor cores cut
-// off what does not fit their accumulator, which on a state that grows over
-// thousands of tokens would add up.
+// Roundings. Products are bf16 tensor-core products with fp32 sums. Whatever is fp32
+// and enters one - decayed keys, decayed scores, the state - does so in three bf16
+// parts, which hold all of its 24 bits: the state is an fp32 state, and an output is
+// rounded once, to bf16. (Scores and state in two parts, 16 bits: forward / backward 37 /
+// 55 us and 148 / 306 us, with ten times as many outputs rounded to the wrong
+// neighbour, one in 400.) U is formed apart and added to X once per chunk: the tensor
+// cores cut off what does not fit their accumulator, which on a state that grows
+// over thousands of tokens would add up.
 //
 // Every wait is bounded (2 s); one that gives up sets an error word of its GPU
 // (decay_error_flag), and its block leaves together, with NaN in its rows and its
@@ -80,6 +83,11 @@ NEXAR_D void stsm4t(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};"
                :: "r"(addr), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
 }
+// The same, not transposed.
+NEXAR_D void stsm4(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};"
+               :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
 // Packed fp32 pairs: x = x * f + u.
 NEXAR_D void fma2(float& x0, float& x1, float f, float u0, float u1) {
   asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmov.b64 c, {%3, %4};\n\t"
@@ -98,10 +106,15 @@ NEXAR_D uint32_t bf2(float lo, float hi) {
 NEXAR_D float bf_lo(uint32_t v) { return __uint_as_float(v << 16); }
 NEXAR_D float bf_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
-NEXAR_D uint32_t split2(float& x, float& y) {  // the pair's bf16 part; x, y keep the rest
-  const uint32_t p = bf2(x, y);
+// An fp32 value as three bf16 parts: the upper 8 bits of its significand, cut off, then those of the rest, then the
+// last 8, so the parts hold all of it. top2 gives a pair's part, split2 also leaves the rest in x, y.
+NEXAR_D uint32_t top2(float x, float y) { return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632); }
+NEXAR_D uint32_t split2(float& x, float& y) {
+  const uint32_t p = top2(x, y);
   asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
-      "sub.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(x), "+f"(y) : "f"(bf_lo(p)), "f"(bf_hi(p)));
+      "sub.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(__uint_as_float(__float_as_uint(x) & 0xffff0000u)), "f"(__uint_as_float(__float_as_uint(y) & 0xffff0000u)));
   return p;
 }
 
@@ -178,9 +191,13 @@ template <int D, bool STATES> struct Shape {
   static constexpr int kTile = kChunk * D * 2;     // bytes of one tile of q, k or v
   static constexpr int kTiles = STATES ? 2 : 3;    // (q,) k, v
   static constexpr int kStages = STATES ? 2 : 1;   // chunks of tiles: the main blocks leave no room for a second
-  static constexpr int kKeys = kStages * kTiles * kTile;  // three parts of the decayed keys; then the output
-  static constexpr int kScores = kKeys + 3 * kTile;       // two parts of P (D = 64: first of X), 8 KB each
-  static constexpr int kMisc = kScores + (STATES ? 0 : 16384);
+  // Three parts of the decayed keys. Main kernel, D = 128: the first part replaces the keys themselves, and the other
+  // two lie where the third part of X^T was.
+  static constexpr bool kInPlace = !STATES && D == 128;
+  static constexpr int kKeys = kStages * kTiles * kTile;
+  static constexpr int kScores = kKeys + (kInPlace ? 2 : 3) * kTile;  // three parts of P (D = 64: first of X), 8 KB each
+  static constexpr int kOut = D == 64 ? kKeys : kScores;              // then the output
+  static constexpr int kMisc = kScores + (STATES ? 0 : 24576);
   static constexpr int kSmem = kMisc + 512;
   // TMEM columns. U at 0 (D = 64: first S; D = 128: first both parts of X^T); D = 64: O at 64;
   // D = 128: O1 (first S) at 128, O2 at 192.
@@ -252,10 +269,6 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
     const double g = (double)a.log_decay[h], p = tid == 0 ? 1.0 : exp(g * min(tid, kChunk));
     pw[tid] = tid <= kChunk ? (float)p : (float)(p - (double)(float)p);
   }
-  if constexpr (!STATES && D == 128) {  // the blocks of P above the diagonal stay zero
-    for (int e = tid; e < 1024; e += S::kThreads)
-      reinterpret_cast<uint4*>(smem + S::kScores)[e] = make_uint4(0, 0, 0, 0);
-  }
 
   // ---- state. D = 64: fragments of X, rows dk = xr (+ 8), columns dv = 32 half + 8 n + xc (+ 1). D = 128: row dv of
   // X^T, columns 64 half .. 64 half + 63.
@@ -312,30 +325,44 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
     const uint32_t tq = base + stage, tk = tq + (STATES ? 0 : S::kTile), tv = tk + S::kTile;
     const bool update = want_final || c + 1 < nchunks;
     if constexpr (!STATES && D == 64) {
-      if (have) {  // ---- the state as an operand: two bf16 parts
+      if (have) {  // ---- the state as an operand: three bf16 parts
 #pragma unroll
-        for (int n = 0; n < kX; n += 2) {
-          float x = X[n], y = X[n + 1];
-          const uint32_t hi = split2(x, y), lo = bf2(x, y);
-          unsigned char* at = smem + S::kScores + tile_at(xr + (n & 2) * 4, half * 4 + (n >> 2)) + xc * 2;
-          *reinterpret_cast<uint32_t*>(at) = hi;
-          *reinterpret_cast<uint32_t*>(at + 8192) = lo;
+        for (int n = 0; n < kX; n += 8) {  // two groups of 8 columns, 16 rows
+          uint32_t hi[4], mid[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = X[n + 2 * e], y = X[n + 2 * e + 1];
+            hi[e] = split2(x, y);
+            mid[e] = split2(x, y);
+            lo[e] = top2(x, y);
+          }
+          const uint32_t at = base + S::kScores + tile_at(quarter * 16 + (lane & 15), half * 4 + n / 4 + (lane >> 4));
+          stsm4(at, hi);
+          stsm4(at + 8192, mid);
+          stsm4(at + 16384, lo);
         }
       }
     }
     if constexpr (!STATES && D == 128) {
-      if (have) {  // ---- the same, X^T; everyone has read U, whose columns it takes, before the last barrier
+      if (have) {  // ---- the same, X^T: two parts over U, which everyone has read before the last barrier, the third in
+                   // the place of the keys' parts (boxes of 128 rows of 128 bytes)
+        unsigned char* row = smem + S::kKeys + half * 16384 + dv * 128;
 #pragma unroll
         for (int n = 0; n < kX; n += 16) {
-          uint32_t hi[8], lo[8];
+          uint32_t hi[8], mid[8], lo[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             float x = X[n + 2 * e], y = X[n + 2 * e + 1];
             hi[e] = split2(x, y);
-            lo[e] = bf2(x, y);
+            mid[e] = split2(x, y);
+            lo[e] = top2(x, y);
           }
           tmem_st_x8(lanes + half * 32 + n / 2, hi);
-          tmem_st_x8(lanes + 64 + half * 32 + n / 2, lo);
+          tmem_st_x8(lanes + 64 + half * 32 + n / 2, mid);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<uint4*>(row + (((n / 8 + i) ^ (dv & 7)) << 4)) =
+                make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -354,6 +381,13 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
       if (__shfl_sync(0xffffffffu, warp, 0) == 4) {
         tc_fence_after();
         const uint64_t kq = umma_desc_sw128_kmajor(tq), kk = umma_desc_sw128_kmajor(tk);
+        if (D == 128 && have) {  // the third part of X^T first: s_done also says that it has been read
+          const uint64_t kx = umma_desc_sw128_kmajor(base + S::kKeys);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            warp_mma(tbase + D + 64, kx + (k >> 2) * 1024 + (k & 3) * 2, kq + (k >> 2) * 512 + (k & 3) * 2,
+                     umma_idesc_bf16_f32(D, 64), k > 0);
+        }
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t o = (k >> 2) * 512 + (k & 3) * 2;
@@ -362,10 +396,10 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
         if (D == 64 && have) {
           const uint64_t mx = desc_mn(base + S::kScores);
 #pragma unroll
-          for (int p = 1; p >= 0; --p)
+          for (int p = 2; p >= 0; --p)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              warp_mma(tbase + 64, kq + k * 2, mx + p * 512 + 128 * k, umma_idesc_bf16_f32(64, 64, false, true), p == 0 || k > 0);
+              warp_mma(tbase + 64, kq + k * 2, mx + p * 512 + 128 * k, umma_idesc_bf16_f32(64, 64, false, true), p < 2 || k > 0);
         }
         warp_commit(s_done);
         if (D == 128 && have) {
@@ -374,7 +408,7 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
               warp_mma_ts(tbase + D + 64, tbase + p * 64 + k * 8, kq + (k >> 2) * 512 + (k & 3) * 2,
-                          umma_idesc_bf16_f32(D, 64), p == 0 || k > 0);
+                          umma_idesc_bf16_f32(D, 64), 1);
         }
         if constexpr (D == 128) warp_commit(x_done);
       }
@@ -383,10 +417,11 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
     if constexpr (S::kStages == 2) {
       if (c + 1 < nchunks) prefetch(c + 1);
     }
-    if (update) {  // ---- keys decayed to the chunk's end, in bf16 parts
+    auto decay_keys = [&] {  // ---- keys decayed to the chunk's end, in bf16 parts
 #pragma unroll
       for (int u = 0; u < kPasses; ++u) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(smem + (tk - base) + at0 + u * kRows * 128);
+        unsigned char* src = smem + (tk - base) + at0 + u * kRows * 128;
+        const uint4 raw = *reinterpret_cast<const uint4*>(src);
         const uint32_t kw[4] = {raw.x, raw.y, raw.z, raw.w};
         const float w = R.kv * pw[max(n_tok - shift - r0 - kRows * u, 0)];  // rows behind the last token are zero
         uint32_t p0[4], p1[4], p2[4];
@@ -396,14 +431,16 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
           mul2(x, y, w);
           p0[q] = split2(x, y);
           p1[q] = split2(x, y);
-          p2[q] = bf2(x, y);
+          p2[q] = top2(x, y);
         }
         unsigned char* dst = smem + S::kKeys + at0 + u * kRows * 128;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
-        *reinterpret_cast<uint4*>(dst + S::kTile) = make_uint4(p1[0], p1[1], p1[2], p1[3]);
-        *reinterpret_cast<uint4*>(dst + 2 * S::kTile) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
+        *reinterpret_cast<uint4*>(S::kInPlace ? src : dst) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
+        if (!S::kInPlace) dst += S::kTile;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(p1[0], p1[1], p1[2], p1[3]);
+        *reinterpret_cast<uint4*>(dst + S::kTile) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
       }
-    }
+    };
+    if (!S::kInPlace && update) decay_keys();
     if constexpr (!STATES) {
       // ---- P: 16 query rows and 32 key columns per warp, up to the diagonal
       if (!wait_phase(s_done, c & 1)) {
@@ -420,15 +457,13 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
         for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * (n & 2 ? f1 : f0));
         tmem_st_frag(lanes + 64 + half * 32, o);
       }
-      if (D == 64) {  // above the diagonal, where the state's parts were
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-          if (half * 2 + m > quarter) {
-            unsigned char* at = smem + S::kScores + tile_at(quarter * 16 + (lane & 15), 4 * half + 2 * m + (lane >> 4));
-            *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(at + 8192) = make_uint4(0, 0, 0, 0);
-          }
-      }
+      for (int m = 0; m < 2; ++m)  // above the diagonal, where the state's parts or the output were
+        if (half * 2 + m > quarter) {
+          unsigned char* at = smem + S::kScores + tile_at(quarter * 16 + (lane & 15), 4 * half + 2 * m + (lane >> 4));
+#pragma unroll
+          for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(at + p * 8192) = make_uint4(0, 0, 0, 0);
+        }
       if (half * 2 <= quarter && quarter * 16 < n_tok) {
         uint32_t sc[16];
         tmem_ld_frag(lanes + (D == 64 ? 0 : D) + half * 32, sc);
@@ -460,19 +495,22 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
                 P[n][e] = gap >= 0 ? P[n][e] * (R.intra * pw[max(gap, 0)]) : 0.f;
               }
           }
+          uint32_t hi[4], mid[4], lo[4];
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-              float u = P[n][2 * p], v = P[n][2 * p + 1];
-              const uint32_t hi = split2(u, v), lo = bf2(u, v);
-              unsigned char* at = smem + S::kScores + tile_at(xr + 8 * p, 2 * kb + n) + xc * 2;
-              *reinterpret_cast<uint32_t*>(at) = hi;
-              *reinterpret_cast<uint32_t*>(at + 8192) = lo;
-            }
+          for (int e = 0; e < 4; ++e) {  // rows + 8 (e % 2), columns + 8 (e / 2)
+            float u = P[e >> 1][2 * (e & 1)], v = P[e >> 1][2 * (e & 1) + 1];
+            hi[e] = split2(u, v);
+            mid[e] = split2(u, v);
+            lo[e] = top2(u, v);
+          }
+          const uint32_t at = base + S::kScores + tile_at(quarter * 16 + (lane & 15), 2 * kb + (lane >> 4));
+          stsm4(at, hi);
+          stsm4(at + 8192, mid);
+          stsm4(at + 16384, lo);
         }
       }
     }
+    if (S::kInPlace && update) decay_keys();
     if (!STATES && D == 64) tmem_st_wait();
     fence_proxy_async_smem();
     tc_fence_before();
@@ -484,19 +522,19 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
         constexpr uint32_t id1 = umma_idesc_bf16_f32(D, 64, D == 128, D == 64);
         const uint64_t kp = umma_desc_sw128_kmajor(base + S::kScores);
 #pragma unroll
-        for (int p = 1; p >= 0; --p)
+        for (int p = 2; p >= 0; --p)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             if constexpr (D == 64)
-              warp_mma(tbase + 64, kp + p * 512 + k * 2, mv + 128 * k, id1, p == 0 || k > 0 || have);
+              warp_mma(tbase + 64, kp + p * 512 + k * 2, mv + 128 * k, id1, p < 2 || k > 0 || have);
             else
-              warp_mma(tbase + D, mv + 128 * k, kp + p * 512 + k * 2, id1, p == 0 || k > 0);
+              warp_mma(tbase + D, mv + 128 * k, kp + p * 512 + k * 2, id1, p < 2 || k > 0);
           }
       }
       if (update) {
-        // U takes the columns of X^T. Only products of one accumulator are sure to run in the order of their issue, so
-        // those that read X^T are waited for; they were issued a group earlier and have long finished.
-        if constexpr (!STATES && D == 128) {
+        // D = 128: U takes the columns of X^T. Only products of one accumulator are sure to run in the order of their
+        // issue, so those that read X^T are waited for; they were issued a group earlier and have long finished.
+        if constexpr (S::kInPlace) {
           if (!wait_phase(x_done, c & 1)) {
             ok = false;
             if (lane == 0) atomicExch(&g_decay_error, 1u);
@@ -509,7 +547,7 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
         for (int p = 2; p >= 0; --p)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint64_t part = mk + p * (S::kTile >> 4) + 128 * k;
+            const uint64_t part = (S::kInPlace ? (p ? mk + (p - 1) * (S::kTile >> 4) : desc_mn(tk)) : mk + p * (S::kTile >> 4)) + 128 * k;
             warp_mma(tbase, D == 64 ? part : mv + 128 * k, D == 64 ? mv + 128 * k : part, idu, p < 2 || k > 0);
           }
       }
@@ -544,8 +582,8 @@ __global__ void __launch_bounds__(Shape<D, STATES>::kThreads, Shape<D, STATES>::
       }
     }
     if constexpr (!STATES) {
-      // ---- the output, through the keys' space so that whole 16-byte groups are stored
-      unsigned char* o_tile = smem + S::kKeys;
+      // ---- the output, through the space of the keys or of P so that whole 16-byte groups are stored
+      unsigned char* o_tile = smem + S::kOut;
       const long long row = origin + dir * (t_begin + c * kChunk);
       __nv_bfloat16* out = R.out + b * R.ob + h * R.oh;
       if constexpr (D == 64) {
@@ -767,12 +805,12 @@ unsigned int decay_error_flag() {
 
 namespace {
 // us of one pass of the main kernel, by what it measured for 37 to 888 blocks of 4
-// to 32 chunks (within 8 %): a chunk takes 2.1, 3.2 or 4.2 us with one, two or three
-// blocks of heads of 64 on an SM and 3.8 or 5.4 us with one or two of heads of 128,
-// to which each wave of blocks and the launch add 2 to 2.5 us. The state-only kernel
-// takes half of each.
+// to 32 chunks (within 8 %, but for 13 % at 148 blocks of 32 chunks of heads of 64): a
+// chunk takes 2.35, 3.5 or 4.7 us with one, two or three blocks of heads of 64 on an SM
+// and 4.5 or 6.5 us with one or two of heads of 128, to which each wave of blocks and
+// the launch add 2 to 2.5 us. The state-only kernel takes half of each.
 double pass_us(long long blocks, long long chunks, int D) {
-  static const double kChunkUs[2][4] = {{0, 2.1, 3.2, 4.2}, {0, 3.8, 5.4, 5.4}};
+  static const double kChunkUs[2][4] = {{0, 2.35, 3.5, 4.7}, {0, 4.5, 6.5, 6.5}};
   const int slots = 148 * (D == 64 ? 3 : 2);
   const double* us = kChunkUs[D != 64];
   const long long waves = blocks / slots, rest = blocks % slots;
@@ -787,11 +825,11 @@ double states_us(long long heads, long long n, long long chunks, int D) {
 }  // namespace
 
 // Splitting the tokens pays where the heads alone leave SMs idle. Measured whole /
-// split, us, heads of 64: 12 of T = 4096: 135 / 33; 60 of T = 1000: 39 / 37; 96 of
-// T = 1024: 39 / 43; of 128: 16 of T = 16385: 936 / 144; 48 of T = 4096: 242 / 111;
-// 128 of T = 1024: 68 / 90. With lengths, segments without a token end at once and
+// split, us, heads of 64: 12 of T = 4096: 151 / 28; 60 of T = 1000: 40 / 32; 96 of
+// T = 1024: 40 / 42; of 128: 16 of T = 16385: 1143 / 157; 48 of T = 4096: 286 / 119;
+// 128 of T = 1024: 74 / 95. With lengths, segments without a token end at once and
 // finer ones share the work out better: as many as fill every resident block (60
-// heads of 64 with 1 to 1000 tokens: 27 against 31).
+// heads of 64 with 1 to 1000 tokens: 40 / 27.5).
 int decay_segment_chunks(int B, int T, int H, int D, bool ragged) {
   const long long heads = (long long)B * H, chunks = (T + kChunk - 1) / kChunk;
   long long best = chunks;
@@ -808,8 +846,8 @@ int decay_segment_chunks(int B, int T, int H, int D, bool ragged) {
 
 // The three uses of the backward pass need fewer segments to fill the GPU: a block
 // then takes several, the most where that is as fast. Measured whole / split, us,
-// heads of 64: 12 of T = 4096: 137 / 49; 48 of T = 4096: 150 / 123; of 128: 16 of
-// T = 16385: 940 / 300; 40 of T = 4096: 238 / 202.
+// heads of 64: 12 of T = 4096: 152 / 46; 48 of T = 4096: 162 / 129; of 128: 16 of
+// T = 16385: 1148 / 349; 40 of T = 4096: 285 / 224.
 int decay_backward_step(int B, int T, int H, int D, int chunks) {
   const long long heads = (long long)B * H, all = (T + kChunk - 1) / kChunk, n = (all + chunks - 1) / chunks;
   if (n < 2) return 0;

@@ -439,3 +439,63 @@ def test_a_long_sum_has_no_bias(cuda0):
     bound = (26 + 3 / (1 - torch.exp(64 * lam.double()))) * 2.0 ** -24
     assert (error(got) <= bound).all(), error(got)
     assert (error(rough) > bound).all(), error(rough)
+
+
+def _beside_ties(shape, dev, g):
+    """fp32 values 2^-12 of half a bf16 step beside the middle between two bf16 neighbours, on either side, as the
+    three bf16 numbers that add up to them. With the last 2^-12 lost a value is a tie, which rounds to the even
+    neighbour, half of the time the wrong one."""
+    base = 1 + torch.randint(0, 128, shape, device=dev, generator=g) / 128.0
+    sign = 1.0 - 2.0 * torch.randint(0, 2, shape, device=dev, generator=g)
+    tail = (1.0 - 2.0 * torch.randint(0, 2, shape, device=dev, generator=g)) * 2.0 ** -20
+    power = torch.exp2(torch.randint(-6, 7, shape, device=dev, generator=g).float())
+    return [sign * power * t for t in (base, torch.full_like(base, 2.0 ** -8), tail)]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("path", ["scores", "state"])
+@pytest.mark.parametrize("result", ["o", "dq", "dk", "dv"])
+@pytest.mark.parametrize("T", [64, 150, 1000])
+def test_outputs_are_rounded_once(cuda0, T, result, path, D):
+    """Scores and states enter the bf16 results with all of their fp32 bits. Without decay and with one-hot rows each
+    result is one score or one element of the state, exactly, so it has to be the nearest bf16 number."""
+    from nexar_b200 import ops
+    B, H = 2, 2
+    g = torch.Generator(device=cuda0).manual_seed(T + D)
+    zero = torch.zeros(B, T, H, D, device=cuda0)
+    t = torch.arange(T, device=cuda0)
+    hot = zero.clone()
+    hot[:, t, :, t % D] = 1.0
+    x = {n: zero for n in ("q", "k", "v", "do")}
+    state = torch.zeros(B, H, D, D, device=cuda0)
+    dstate = torch.zeros_like(state)
+    if path == "state":
+        s = sum(_beside_ties((B, H, D, D), cuda0, g))
+        rows = {"o": "q", "dq": "do", "dk": "v", "dv": "k"}[result]  # one-hot: picks a row or a column of the state
+        x[rows] = hot
+        if result in ("o", "dq"):
+            state = s
+        else:
+            dstate = s
+        pick = s if result in ("o", "dv") else s.transpose(-1, -2)
+        want = pick[:, :, t % D].transpose(1, 2)
+    else:
+        # the score of tokens i and j is the other token's value; tokens behind the 64th have none (one-hot rows end)
+        n = 64
+        value = _beside_ties((B, n, H), cuda0, g)
+        ones, parts = zero.clone(), zero.clone()
+        ones[..., :3] = 1.0
+        for i, p in enumerate(value):
+            parts[:, :n, :, i] = p
+        hot[:, n:] = 0.0
+        one, other, row = {"o": ("q", "k", "v"), "dq": ("do", "v", "k"), "dk": ("v", "do", "q"), "dv": ("k", "q", "do")}[result]
+        x[one], x[other], x[row] = ones, parts, hot
+        s = sum(value)  # [B, n, H]: at column j of every token that sees token j
+        sees = (t[:, None] >= t[None, :n]) if result in ("o", "dq") else (t[:, None] <= t[None, :n])
+        want = zero.clone()
+        want[..., :n] = torch.where(sees[None, :, None], s.transpose(1, 2)[:, None], 0.0)
+    leaves = [x[n].to(torch.bfloat16).requires_grad_(True) for n in ("q", "k", "v")]
+    state.requires_grad_(True)
+    o, f = ops.decay_attention(*leaves, torch.zeros(H, device=cuda0), state=state, scale=1.0, return_state=True)
+    got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad((o, f), leaves, (x["do"].to(torch.bfloat16), dstate))), o=o)[result]
+    assert torch.equal(got.detach(), want.to(torch.bfloat16))
