@@ -362,11 +362,7 @@ class _Attention(torch.autograd.Function):
         B, T, H, causal = ctx.shape
         C = _native.cuda()
         dqkv = torch.empty_like(qkv)
-        ws = _SCRATCH.get((qkv.device, "attn_ws"))
-        need = C.attn_bwd_workspace_floats(B, T, H)
-        if ws is None or ws.numel() < need:
-            ws = torch.empty(need, dtype=torch.float32, device=qkv.device)
-            _SCRATCH[(qkv.device, "attn_ws")] = ws
+        ws = _workspace(qkv.device, C.attn_bwd_workspace_floats(B, T, H))
         C.attn_bwd(qkv, y, dy.contiguous(), lse, dqkv, ws, B, T, H, causal)
         return dqkv, None, None, None, None
 

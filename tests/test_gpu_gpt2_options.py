@@ -209,6 +209,31 @@ def test_layer_norm_backward_on_streams_side_by_side(cuda0):
             assert all(torch.equal(i, j) for i, j in zip(a, c))
 
 
+@gpu
+def test_attention_backward_on_streams_side_by_side(cuda0):
+    """Bit for bit but for dq, whose sums over key blocks are atomic: there two runs of the same call may differ by
+    the order of T / 128 = 8 fp32 terms, a unit in the last place of the bf16 result."""
+    g = torch.Generator(device=cuda0).manual_seed(9)
+    B, T, H = 1, 1024, 2
+    streams = [torch.cuda.Stream(cuda0) for _ in range(4)]
+    cases = [[torch.randn(B * T, n * H * 64, device=cuda0, generator=g).to(torch.bfloat16) for n in (3, 1)] for _ in streams]
+    for qkv, _ in cases:
+        qkv.requires_grad_(True)
+    want = [torch.autograd.grad(ops.attention(qkv, B, T, H), qkv, dy)[0].float() for qkv, dy in cases]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for s, (qkv, dy) in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(torch.autograd.grad(ops.attention(qkv, B, T, H), qkv, dy)[0])
+        torch.cuda.synchronize()
+        for a, c in zip(got, want):
+            a = a.float()
+            assert torch.equal(a[:, 64 * H:], c[:, 64 * H:])
+            scale = c[:, :64 * H].abs().amax()
+            assert ((a - c)[:, :64 * H].abs() <= 2.0 ** -7 * c[:, :64 * H].abs() + 2.0 ** -20 * scale).all()
+
+
 def test_flops_per_token():
     """6 per weight; softmax attention grows with the length, the decay mixer with the head's size alone."""
     small = GPT2Config.small()
