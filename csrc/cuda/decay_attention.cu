@@ -41,12 +41,12 @@
 // form with tensor-map loads, which spilled some, took 17 to 25 % longer.
 //
 // Measured, forward / backward: 8 x 1024 tokens of 12 heads of 64: 40 / 58 us (the
-// 138 MB that they have to move take 21 us); 16385 tokens of 16 heads of 128: 157 /
-// 349 us (742 MB, 113 us), of which the states before the segments and the scan are
-// 57 us each. With a full grid an SM issues in 53 to 58 % of its cycles and the
-// tensor pipe works in 34 to 36 %: bound by the instructions that decay, round and
-// split operands between one chunk's two groups of products and by the latency of
-// that chain, which the two or three blocks of an SM do not cover in full.
+// 138 MB that they have to move take 21 us); 16385 tokens of 16 heads of 128: 160 /
+// 351 us (742 MB, 113 us), of which the states before the segments and the scan are
+// 57 us each. With a full grid an SM issues in 48 to 51 % of its cycles and the
+// tensor pipe works in 34 to 37 %: bound by the latency of a chunk's chain - products,
+// their way out of TMEM, the instructions that decay and split operands, products -
+// which the two or three blocks of an SM do not cover in full.
 //
 // Roundings. Products are bf16 tensor-core products with fp32 sums. Whatever is fp32
 // and enters one - decayed keys, decayed scores, the state - does so in three bf16

@@ -167,7 +167,7 @@ NEXAR_D uint4 stream16(const __nv_bfloat16* p) { return __ldcs(reinterpret_cast<
 
 // RW warps per row, NP packs of 8 columns per lane; rows of more than 1024 columns
 // take two warps, which leaves registers for twice the rows in flight (32768 x 2048:
-// 91 us, 5.9 TB/s, against 101 with one warp; 8192 x 768, one warp: 12.4 us). The sum
+// 91 us, 5.9 TB/s, against 101 with one warp; 8192 x 768, one warp: 10.8 us). The sum
 // is rounded to the stored bf16 before the statistics, as in the operator without
 // dropout.
 template <int NP, int RW>
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_dropout_ln_fwd(
 // The normalised value is (x - mean) rstd, as in the forward pass: x rstd - mean rstd
 // in one FMA would round mean rstd, which is far from 0 where x is the mean.
 // Measured with the columns: 32768 x 2048 in 117 us (671 MB, 5.7 TB/s), 8192 x 768
-// in 20. Through registers it took 155 and 23 (one pair ahead at most); three or
+// in 18. Through registers it took 155 and 23 (one pair ahead at most); three or
 // four blocks an SM, or one more stage, take 121 to 127.
 constexpr int kBwdRows = 2, kBwdStages = 3;
 template <bool BIAS>

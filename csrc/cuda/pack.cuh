@@ -8,8 +8,8 @@ namespace nexar {
 
 // W elements of T (bf16, fp16 or fp32; W even), read and written in up to
 // 16-byte accesses and kept as words until they are needed. Conversions to 16
-// bits go two at a time: one at a time they run on the SM's narrowest pipe,
-// which made a dropout kernel 1.4 times slower.
+// bits go two at a time: one at a time they run on the SM's narrowest pipe
+// (dropout of 64 Mi bf16 elements: 60 us, two at a time 49).
 template <typename T, int W> struct alignas(W * sizeof(T) < 16 ? W * sizeof(T) : 16) Pack {
   static constexpr int kWords = W * sizeof(T) / 4;
   uint32_t w[kWords];

@@ -187,7 +187,9 @@ def decay_attention(q, k, v, log_decay, state=None, lengths=None, scale: Optiona
     (not read, zero output and gradients, the final state is the one behind the last token). ``scale``
     defaults to D^-0.5. Returns o [B, T, H, D] bf16, or (o, final state) with ``return_state``;
     differentiable in q, k, v and state, once. Tokens are worked on in chunks of 64: a value that is
-    not finite can show in the output of every token of its chunk."""
+    not finite can show in the output of every token of its chunk. A kernel whose wait for its own
+    products is not answered within 2 s (never seen) leaves NaN in its rows and its state and ends;
+    ``_native.cuda().decay_error_flag()`` then reads 1 for the current GPU (the call synchronises)."""
     return _decay(q, k, v, log_decay, state, lengths, _decay_scale(scale, q.shape[-1]), return_state)
 
 
