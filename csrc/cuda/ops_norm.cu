@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kLnWarps * 32) k_ln_bwd(
     __nv_bfloat16* __restrict__ dx, float* __restrict__ part, int R, int C) {
   constexpr int K = DSUM ? 3 : 2;
   constexpr bool kPref = NP <= 3;  // wider rows have no registers left for a prefetch
-  extern __shared__ float smem[];  // [K][C]
+  extern __shared__ __align__(16) float smem[];  // [K][C]
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
   for (int i = threadIdx.x; i < K * C; i += blockDim.x) smem[i] = 0.f;
@@ -241,20 +241,31 @@ __global__ void __launch_bounds__(kLnWarps * 32) k_ln_bwd(
       }
     }
   }
-  // CTA partials: warps add their register sums into shared memory.
+  // CTA partials: warps add their register sums into shared memory one after the other, so the order of the sums, and
+  // with it every bit of the result, is the same in every run.
+  auto add8 = [&](float* at, const float (&v)[8]) {
 #pragma unroll
-  for (int k = 0; k < NP; ++k) {
-    const int col = (lane + 32 * k) * 8;
-    if (col < C) {
+    for (int h = 0; h < 2; ++h) {
+      float4 t = reinterpret_cast<float4*>(at)[h];
+      t.x += v[4 * h], t.y += v[4 * h + 1], t.z += v[4 * h + 2], t.w += v[4 * h + 3];
+      reinterpret_cast<float4*>(at)[h] = t;
+    }
+  };
+#pragma unroll 1
+  for (int turn = 0; turn < kLnWarps; ++turn) {
+    if (warp == turn) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        atomicAdd(&smem[col + e], aw[k][e]);
-        atomicAdd(&smem[C + col + e], ab[k][e]);
-        if constexpr (DSUM) atomicAdd(&smem[2 * C + col + e], ad[k][e]);
+      for (int k = 0; k < NP; ++k) {
+        const int col = (lane + 32 * k) * 8;
+        if (col < C) {
+          add8(smem + col, aw[k]);
+          add8(smem + C + col, ab[k]);
+          if constexpr (DSUM) add8(smem + 2 * C + col, ad[k]);
+        }
       }
     }
+    __syncthreads();
   }
-  __syncthreads();
   float* mine = part + (size_t)blockIdx.x * K * C;
   for (int i = threadIdx.x; i < K * C; i += blockDim.x) mine[i] = smem[i];
 }

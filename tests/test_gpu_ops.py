@@ -186,3 +186,25 @@ def test_adamw_and_clip(cuda0):
         C.adamw(p, m, v, g, pb, decay_end, 1e-3, 0.9, 0.95, 1e-8, 0.1, step, coef, step_dev, None)
     torch.testing.assert_close(p, ref_p.detach(), rtol=1e-4, atol=1e-5)
     torch.testing.assert_close(pb.float(), p, rtol=1e-2, atol=1e-2)
+
+
+@pytest.mark.parametrize("R,C", [(192, 128), (3000, 64), (8192, 768), (500, 2048)])
+def test_layernorm_backward_repeats_to_the_bit(cuda0, R, C):
+    """The column sums have one order, inside a block as over the blocks. Each column of the gradients holds a large
+    value and its negative in two of its rows: what the sum keeps of the rows added between the two, bits that any other
+    order changes."""
+    from nexar_b200 import ops
+    g = torch.Generator(device=cuda0).manual_seed(R + C)
+    x, r, ds, dy = (_bf(torch.randn(R, C, device=cuda0, generator=g)) for _ in range(4))
+    w, b, rb = (_bf(torch.randn(C, device=cuda0, generator=g)).requires_grad_(True) for _ in range(3))
+    rows = torch.rand(R, C, device=cuda0, generator=g).argsort(0)[:2]
+    for t in (ds, dy):
+        t.scatter_(0, rows, torch.tensor([[2.0 ** 20], [-2.0 ** 20]], device=cuda0).expand(2, C).to(t.dtype))
+    x.requires_grad_(True), r.requires_grad_(True)
+
+    def run():
+        out = ops.residual_layer_norm(x, r, w, b, rbias=rb)
+        return torch.autograd.grad(out, (x, r, w, b, rb), (ds, dy))
+    first = run()
+    for _ in range(40):
+        assert all(torch.equal(a, c) for a, c in zip(first, run()))
