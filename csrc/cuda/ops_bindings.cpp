@@ -24,6 +24,16 @@ void need_f32(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat && t.is_contiguous(), "nexar_b200: ", name,
               " must be a contiguous fp32 CUDA tensor");
 }
+// Kernels read rows in 16-byte groups: an input at another address is copied.
+at::Tensor aligned(const at::Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone();
+}
+c10::optional<at::Tensor> aligned(const c10::optional<at::Tensor>& t) {
+  return t ? c10::optional<at::Tensor>(aligned(*t)) : t;
+}
+void need_aligned(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "nexar_b200: ", name, " must be 16-byte aligned");
+}
 __nv_bfloat16* bf(const at::Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); }
 const __nv_bfloat16* bfc(const c10::optional<at::Tensor>& t) {
   return t ? reinterpret_cast<const __nv_bfloat16*>(t->data_ptr()) : nullptr;
@@ -32,21 +42,31 @@ const __nv_bfloat16* bfc(const c10::optional<at::Tensor>& t) {
 
 // LayerNorm forward; x: [R, C]. Returns nothing; writes y, mean, rstd (and
 // sum_out = x + res when res is given).
-void op_ln_fwd(const at::Tensor& x, const c10::optional<at::Tensor>& res,
-               const c10::optional<at::Tensor>& sum_out, const at::Tensor& w, const at::Tensor& b,
+void op_ln_fwd(const at::Tensor& x_in, const c10::optional<at::Tensor>& res_in,
+               const c10::optional<at::Tensor>& sum_out, const at::Tensor& w_in, const at::Tensor& b_in,
                const at::Tensor& y, const at::Tensor& mean, const at::Tensor& rstd, double eps,
-               const c10::optional<at::Tensor>& rbias) {
-  need_bf16(x, "x");
+               const c10::optional<at::Tensor>& rbias_in) {
+  need_bf16(x_in, "x");
   need_bf16(y, "y");
-  need_bf16(w, "weight");
-  need_bf16(b, "bias");
+  need_bf16(w_in, "weight");
+  need_bf16(b_in, "bias");
+  need_aligned(y, "y");
+  if (sum_out) need_aligned(*sum_out, "sum_out");
+  c10::cuda::CUDAGuard g(x_in.get_device());
+  const at::Tensor x = aligned(x_in), w = aligned(w_in), b = aligned(b_in);
+  const c10::optional<at::Tensor> res = aligned(res_in), rbias = aligned(rbias_in);
   need_f32(mean, "mean");
   need_f32(rstd, "rstd");
   const int C = x.size(-1);
   const int R = x.numel() / C;
   TORCH_CHECK(res.has_value() == sum_out.has_value(), "ln_fwd: res and sum_out go together");
+  TORCH_CHECK(w.numel() == C && b.numel() == C, "nexar_b200: ln_fwd: weight and bias need one value per column");
+  if (res) {
+    need_bf16(*res, "res");
+    TORCH_CHECK(res->numel() == x.numel(), "nexar_b200: ln_fwd: res must have as many elements as x");
+  }
+  if (rbias) need_bf16(*rbias, "rbias");
   TORCH_CHECK(!rbias || (res && rbias->numel() == C), "ln_fwd: rbias needs res and C elements");
-  c10::cuda::CUDAGuard g(x.get_device());
   chk(ln_fwd_ex(bf(x), bfc(res), bfc(rbias), sum_out ? bf(*sum_out) : nullptr, bf(w), bf(b), bf(y),
                 mean.data_ptr<float>(), rstd.data_ptr<float>(), R, C, (float)eps, stream_of(x)),
       "ln_fwd");
@@ -57,24 +77,30 @@ int64_t op_ln_bwd_scratch_floats(int64_t R, int64_t C, bool dsum) {
   return (int64_t)ln_bwd_scratch_floats_ex((int)C, ln_bwd_blocks((int)R), dsum);
 }
 
-void op_ln_bwd(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& mean, const at::Tensor& rstd,
-               const at::Tensor& w, const c10::optional<at::Tensor>& dres, const at::Tensor& dx,
+void op_ln_bwd(const at::Tensor& dy_in, const at::Tensor& x_in, const at::Tensor& mean, const at::Tensor& rstd,
+               const at::Tensor& w_in, const c10::optional<at::Tensor>& dres_in, const at::Tensor& dx,
                const at::Tensor& dw, const at::Tensor& db, const at::Tensor& scratch,
                const c10::optional<at::Tensor>& /* counter: not used any more */,
                const c10::optional<at::Tensor>& dsum) {
-  need_bf16(dy, "dy");
-  need_bf16(x, "x");
+  need_bf16(dy_in, "dy");
+  need_bf16(x_in, "x");
   need_bf16(dx, "dx");
+  need_aligned(dx, "dx");
+  c10::cuda::CUDAGuard g(x_in.get_device());
+  const at::Tensor dy = aligned(dy_in), x = aligned(x_in), w = aligned(w_in);
+  const c10::optional<at::Tensor> dres = aligned(dres_in);
   need_bf16(dw, "dw");
   need_bf16(db, "db");
   need_f32(scratch, "scratch");
   const int C = x.size(-1);
   const int R = x.numel() / C;
   const int blocks = ln_bwd_blocks(R);
+  TORCH_CHECK(dy.numel() == x.numel() && w.numel() == C && (!dres || dres->numel() == x.numel()),
+              "nexar_b200: ln_bwd: gradients must have as many elements as x, weight one per column");
+  if (dres) need_bf16(*dres, "dres");
   TORCH_CHECK((size_t)scratch.numel() >= ln_bwd_scratch_floats_ex(C, blocks, dsum.has_value()),
               "ln_bwd: scratch too small");
   if (dsum) need_bf16(*dsum, "dsum");
-  c10::cuda::CUDAGuard g(x.get_device());
   chk(ln_bwd_ex(bf(dy), bf(x), mean.data_ptr<float>(), rstd.data_ptr<float>(), bf(w), bfc(dres), bf(dx),
                 bf(dw), bf(db), dsum ? bf(*dsum) : nullptr, scratch.data_ptr<float>(), R, C, blocks, stream_of(x)),
       "ln_bwd");
@@ -155,18 +181,25 @@ void op_embed_fwd(const at::Tensor& tok, const at::Tensor& wte, const c10::optio
   if (wpe) need_bf16(*wpe, "wpe");
   need_bf16(out, "out");
   const int C = wte.size(-1);
+  TORCH_CHECK(tok.is_cuda() && tok.get_device() == wte.get_device(), "nexar_b200: embed: tokens must be on the GPU of wte");
+  TORCH_CHECK(!wpe || (wpe->size(-1) == C && wpe->size(0) >= T), "nexar_b200: embed: no position row for every token");
+  need_aligned(wte, "wte");
+  if (wpe) need_aligned(*wpe, "wpe");
   c10::cuda::CUDAGuard g(wte.get_device());
   chk(embed_fwd(tok.data_ptr<int64_t>(), bf(wte), bfc(wpe), bf(out), tok.numel(), (int)T, C, stream_of(wte)),
       "embed_fwd");
   count_launch(1);
 }
-void op_embed_bwd(const at::Tensor& tok, const at::Tensor& dout, const at::Tensor& dwte,
+void op_embed_bwd(const at::Tensor& tok, const at::Tensor& dout_in, const at::Tensor& dwte,
                   const c10::optional<at::Tensor>& dwpe, int64_t B, int64_t T) {
-  need_bf16(dout, "dout");
+  need_bf16(dout_in, "dout");
   need_bf16(dwte, "dwte");
   if (dwpe) need_bf16(*dwpe, "dwpe");
-  const int C = dout.size(-1);
-  c10::cuda::CUDAGuard g(dout.get_device());
+  need_aligned(dwte, "dwte");
+  if (dwpe) need_aligned(*dwpe, "dwpe");
+  const int C = dout_in.size(-1);
+  c10::cuda::CUDAGuard g(dout_in.get_device());
+  const at::Tensor dout = aligned(dout_in);
   chk(embed_bwd(tok.data_ptr<int64_t>(), bf(dout), bf(dwte), dwpe ? bf(*dwpe) : nullptr, (int)B, (int)T, C,
                 stream_of(dout)),
       "embed_bwd");

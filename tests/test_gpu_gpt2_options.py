@@ -280,3 +280,59 @@ def test_ranks_draw_masks_of_their_own():
     # the masks behind two ranks' seeds differ in about 2 p (1 - p) of their elements
     a, b = (oracle.dropout_keep(4096, s[0], s[1], 1, 0.5)[0] for s in (states[1], states[2]))
     assert 0.4 < (a != b).double().mean() < 0.6
+
+
+def _moved(t):
+    """The same values in a contiguous view at an address that is not a multiple of 16."""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    flat[1:] = t.reshape(-1)
+    return flat[1:].view_as(t)
+
+
+@gpu
+@pytest.mark.parametrize("residual", [False, True])
+def test_layer_norm_tensors_at_any_address(cuda0, residual):
+    """The norms that the model uses without dropout, as those with it."""
+    g = torch.Generator(device=cuda0).manual_seed(12)
+    x, r, ds, dy = (torch.randn(30, 64, device=cuda0, generator=g).to(torch.bfloat16) for _ in range(4))
+    w, b, rb = (torch.randn(64, device=cuda0, generator=g).to(torch.bfloat16) for _ in range(3))
+
+    def run(how):
+        xx, rr, ww, bb, rbb = (how(t).requires_grad_(True) for t in (x, r, w, b, rb))
+        if residual:
+            out = ops.residual_layer_norm(xx, rr, ww, bb, rbias=rbb)
+            return [*out, *torch.autograd.grad(out, (xx, rr, ww, bb, rbb), (how(ds), how(dy)))]
+        out = ops.layer_norm(xx, ww, bb)
+        return [out, *torch.autograd.grad(out, (xx, ww, bb), how(dy))]
+    assert all(torch.equal(a, c) for a, c in zip(run(lambda t: t.clone()), run(_moved)))
+
+
+@gpu
+def test_embedding_refusals_and_addresses(cuda0):
+    tok = torch.randint(0, 50, (2, 12), device=cuda0)
+    wte, wpe = (torch.randn(n, 64, device=cuda0).to(torch.bfloat16).requires_grad_(True) for n in (50, 12))
+    dout = torch.randn(2, 12, 64, device=cuda0).to(torch.bfloat16)
+    for pos in (None, wpe):
+        leaves = [wte] + ([wpe] if pos is not None else [])
+        out = ops.embedding(tok, wte, pos)
+        want = torch.autograd.grad(out, leaves, dout, retain_graph=True)
+        got = torch.autograd.grad(out, leaves, _moved(dout))
+        # wte: at most 24 atomic bf16 sums per element, in any order
+        assert ((want[0] - got[0]).float().abs() <= 24 * 2.0 ** -8 * dout.float().abs().sum((0, 1))).all()
+        assert all(torch.equal(a, c) for a, c in zip(want[1:], got[1:]))
+    with pytest.raises(RuntimeError, match="position row"):
+        ops.embedding(tok, wte, wpe[:11].detach())
+    with pytest.raises(RuntimeError, match="aligned"):
+        ops.embedding(tok, _moved(wte.detach()))
+
+
+@gpu
+def test_layer_norm_refusals(cuda0):
+    x = torch.zeros(4, 64, device=cuda0, dtype=torch.bfloat16)
+    w = torch.ones(64, device=cuda0, dtype=torch.bfloat16)
+    for f in (lambda: ops.residual_layer_norm(x, x[:2], w, w), lambda: ops.layer_norm(x, w[:32], w),
+              lambda: ops.residual_layer_norm(x, x, w, w, rbias=w.float()),
+              lambda: ops.residual_layer_norm(x, x.float(), w, w)):
+        with pytest.raises(RuntimeError):
+            f()
+
